@@ -7,9 +7,10 @@ a CUDA device is an error, and so is a failed build of the kernel library.
 from __future__ import annotations
 
 import ctypes
+import itertools
 import math
 import os
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -51,6 +52,20 @@ def _need_contiguous(*tensors):
     for t in tensors:
         if t is not None and not t.is_contiguous():
             raise KernelError("kernel operands must be contiguous")
+
+
+def _need_here(what: str, *tensors):
+    """Launches go to the current device's current stream: operands of another device are refused."""
+    here = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.device.index != here:
+            raise KernelError(f"{what}: the operands must lie on the current device (cuda:{here}), got {t.device}")
+
+
+def _need_aligned(what: str, *tensors):
+    for t in tensors:
+        if t is not None and t.data_ptr() % 16:
+            raise KernelError(f"{what}: operands must begin on a 16-byte boundary")
 
 
 _launches = 0
@@ -2708,4 +2723,175 @@ def wkv(r: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor, 
     fn = _fn("time_mixing", "pbe_wkv_steps", types + [c_void_p] * 3 + [c_int] * 5 + [c_void_p])
     _check(fn(*heads_of, _ptr(q_start), _ptr(q_len), _ptr(slots), int(num_requests), H, D, E, 1 if update_state else 0,
               _stream()), "wkv_steps")
+    return out
+
+
+# ------------------------------------------------------------------ a step's integers, made on the device
+class PageMaps(NamedTuple):
+    """What ``page_maps`` makes, int32 on the device."""
+    q_start: torch.Tensor           # [R]
+    seq_len: torch.Tensor           # [R]
+    positions: torch.Tensor         # [rows]
+    request_of_row: torch.Tensor    # [rows]
+    slots: torch.Tensor             # [rows]
+    block_table: torch.Tensor       # [R, width]
+
+
+MAPS_MAX_REQUESTS = 8192
+
+
+def page_maps(q_len: torch.Tensor, context: torch.Tensor, pages: Optional[torch.Tensor], page_tokens: int, rows: int,
+              width: int, stride: int = 1) -> PageMaps:
+    """Row maps and block tables of a step from its requests' lengths.  Request r brings ``q_len[r]`` rows behind
+    ``context[r]`` tokens (int32 [R]; either may be 0) and holds ceil((context + q_len) / (page_tokens * stride)) pages, which
+    stand in ``pages`` (int32, one request's behind the other's; None: numbered from 0 on).  The rows of all requests are laid
+    end to end: ``q_start`` is a request's first row and ``seq_len`` its tokens with them; a row has its request, its position
+    and the slot (page * page_tokens + place) of its entry, one entry for every ``stride`` tokens.  ``block_table`` has
+    ``width`` entries a request, -1 behind its last page.  Of ``rows`` rows those behind the last request have request and
+    slot -1 and position 0.  A row whose page is negative or lies behind the end of ``pages`` has slot -1.  At most
+    ``MAPS_MAX_REQUESTS`` requests."""
+    _need_contiguous(q_len, context, pages)
+    R = q_len.numel()
+    if q_len.dtype != torch.int32 or context.dtype != torch.int32 or q_len.dim() != 1 or context.shape != q_len.shape:
+        raise KernelError("page_maps: q_len and context must be int32 [R]")
+    if pages is not None and (pages.dtype != torch.int32 or pages.dim() != 1):
+        raise KernelError("page_maps: pages must be one int32 list")
+    if page_tokens < 1 or stride < 1 or rows < 0 or width < 0 or page_tokens * stride > 0x7fffffff:
+        raise KernelError("page_maps: page_tokens and stride are at least 1, rows and width not negative")
+    if not 1 <= R <= MAPS_MAX_REQUESTS:
+        raise KernelError(f"page_maps takes 1 to {MAPS_MAX_REQUESTS} requests, got {R}")
+    sizes = [R, R, rows, rows, rows, R * width]
+    ends = list(itertools.accumulate((n + 3) // 4 * 4 for n in sizes))        # each on a 16-byte boundary
+    if ends[-1] > 0x7fffffff:
+        raise KernelError("page_maps: more rows or table entries than int32 counts")
+    _need_cuda(q_len, context, pages)
+    _need_here("page_maps", q_len, context, pages)
+    held = torch.empty(ends[-1], dtype=torch.int32, device=q_len.device)
+    out = [held[e - (n + 3) // 4 * 4:][:n] for e, n in zip(ends, sizes)]
+    fn = _fn("page_maps", "pbe_page_maps", [c_void_p] * 3 + [c_ll] + [c_void_p] * 6 + [c_int] * 5 + [c_void_p])
+    _check(fn(_ptr(q_len), _ptr(context), _ptr(pages), pages.numel() if pages is not None else 1 << 31,
+              *[_ptr(t) for t in out], R, int(rows), int(width), int(page_tokens), int(stride), _stream()), "page_maps")
+    return PageMaps(*out[:5], out[5].view(R, width))
+
+
+# ------------------------------------------------------------------ key/value cache in four bits
+KV4_GROUP = 32              # channels that share a scale
+KV4_HEAD_DIMS = (64, 128)
+KV4_PAGE_UNIT = 16          # pages are whole records of this many tokens
+
+
+def kv4_width(head_dim: int) -> int:
+    """Bytes that the key and the value of one token of one head take together."""
+    if head_dim not in KV4_HEAD_DIMS:
+        raise KernelError(f"a 4-bit cache takes head sizes {KV4_HEAD_DIMS}, got {head_dim}")
+    return head_dim * 5 // 4
+
+
+def _kv4_pages(what: str, pages: torch.Tensor, kv_heads: int, page_tokens: int, head_dim: int) -> None:
+    _need_contiguous(pages)
+    if page_tokens < 1 or page_tokens % KV4_PAGE_UNIT:
+        raise KernelError(f"{what}: a page holds a multiple of {KV4_PAGE_UNIT} tokens, got {page_tokens}")
+    if pages.dtype != torch.uint8 or tuple(pages.shape[1:]) != (kv_heads, page_tokens, kv4_width(head_dim)):
+        raise KernelError(f"{what}: pages must be uint8 [page, kv_head, page_tokens, {kv4_width(head_dim)}]")
+    _need_aligned(what, pages)
+
+
+def kv4_write(qkv: torch.Tensor, bias: Optional[torch.Tensor], q_out: torch.Tensor, pages: Optional[torch.Tensor],
+              positions: torch.Tensor, slots: Optional[torch.Tensor], inv_freq: Optional[torch.Tensor], num_heads: int,
+              num_kv_heads: int, head_dim: int, rotary_dim: int, page_tokens: int, interleaved: bool = False) -> torch.Tensor:
+    """q_out = rope(q + b), and rope(k + b) and v + b into 4-bit pages: ``rope_kv_write`` for a cache in four bits.  ``pages``
+    is one layer's, uint8 [page, kv_head, page_tokens, kv4_width(head_dim)] (None: nothing is written); a row whose slot is
+    negative or behind the last page writes nothing.  Two rows of one call must not share a slot.  Groups of 32 channels are kept as lo + s * code, code 0..15, each off by at most s / 2 (s: a
+    fifteenth of the group's span, rounded up to bfloat16); NaN is kept as 0, what lies beyond 2^120 as 2^120."""
+    _need_contiguous(qkv, bias, q_out, positions, slots, inv_freq)
+    T, H, KV = qkv.shape[0], num_heads, num_kv_heads
+    width = (H + 2 * KV) * head_dim
+    kv4_width(head_dim)
+    dtype = _dtype_code(qkv)
+    if qkv.dim() != 2 or qkv.shape[1] != width or q_out.shape != (T, H * head_dim) or q_out.dtype != qkv.dtype:
+        raise KernelError("kv4_write: shapes or dtypes do not agree")
+    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != width):
+        raise KernelError("kv4_write: bias must be float32 of the fused width")
+    if positions.dtype != torch.int32 or positions.numel() != T:
+        raise KernelError("kv4_write: positions must be int32 [T]")
+    if pages is not None:
+        _kv4_pages("kv4_write", pages, KV, page_tokens, head_dim)
+        if slots is None or slots.dtype != torch.int32 or slots.numel() != T:
+            raise KernelError("kv4_write: slots must be int32 [T]")
+    if inv_freq is None:
+        rotary_dim = 0
+    elif rotary_dim % 2 or not 0 <= rotary_dim <= head_dim or inv_freq.dtype != torch.float32 \
+            or inv_freq.numel() != rotary_dim // 2:
+        raise KernelError("kv4_write: inv_freq must be float32 [rotary_dim / 2], rotary_dim even and at most head_dim")
+    if 2 * KV * head_dim * 4 + rotary_dim * 4 > 48 * 1024:
+        raise KernelError(f"kv4_write: {KV} key/value heads of {head_dim} do not fit in shared memory")
+    _need_aligned("kv4_write", qkv, bias, q_out)
+    _need_cuda(qkv, bias, q_out, pages, positions, slots, inv_freq)
+    _need_here("kv4_write", qkv, bias, q_out, pages, positions, slots, inv_freq)
+    fn = _fn("kv4_write", "pbe_kv4_write", [c_void_p] * 7 + [c_int] * 7 + [c_ll, c_int, c_void_p])
+    _check(fn(_ptr(qkv), _ptr(bias), _ptr(q_out), _ptr(pages), _ptr(positions), _ptr(slots), _ptr(inv_freq), T, H, KV, head_dim,
+              rotary_dim, page_tokens, 1 if interleaved else 0, pages.shape[0] if pages is not None else 0, dtype, _stream()),
+           "kv4_write")
+    return q_out
+
+
+def kv4_read(pages: torch.Tensor, slots: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16):
+    """The keys and values that the slots (int32 [T]) of 4-bit pages stand for, lo + s * code: two tensors [T, kv_head,
+    head_dim] in ``out_dtype``; zeros where a slot is negative or behind the last page."""
+    _need_contiguous(slots)
+    if out_dtype not in (torch.float32, torch.bfloat16):
+        raise KernelError(f"kernels take float32 or bfloat16 tensors, got {out_dtype}")
+    if pages.dim() != 4 or slots.dtype != torch.int32 or slots.dim() != 1:
+        raise KernelError("kv4_read: pages have four dimensions, slots are int32 [T]")
+    KV, page_tokens, head_dim = pages.shape[1], pages.shape[2], pages.shape[3] * 4 // 5
+    _kv4_pages("kv4_read", pages, KV, page_tokens, head_dim)
+    _need_cuda(pages, slots)
+    _need_here("kv4_read", pages, slots)
+    k, v = torch.empty((2, slots.numel(), KV, head_dim), dtype=out_dtype, device=pages.device)
+    fn = _fn("kv4_write", "pbe_kv4_read", [c_void_p] * 4 + [c_int] * 4 + [c_ll, c_int, c_void_p])
+    _check(fn(_ptr(pages), _ptr(slots), _ptr(k), _ptr(v), slots.numel(), KV, head_dim, page_tokens, pages.shape[0],
+              _dtype_code(k), _stream()), "kv4_read")
+    return k, v
+
+
+class Kv4AttnParams(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("q", "pages", "out", "q_start", "q_len", "seq_len", "block_table")] + \
+        [("bt_stride", c_ll)] + [(n, c_int) for n in ("table_pages", "num_pages", "requests", "rows", "heads", "kv_heads",
+                                                      "page_tokens", "window")] + [("scale", c_float)]
+
+
+def kv4_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor,
+                  seq_len: torch.Tensor, block_table: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int,
+                  scale: float, window: Optional[int], page_tokens: int, most_rows: int, most_keys: int) -> torch.Tensor:
+    """Causal attention of every row over 4-bit pages, ``paged_attention`` for a cache in four bits: row i of request r (row
+    ``q_start[r] + i`` of q and out, both [T, H * head_dim]) sees the request's first ``seq_len[r] - q_len[r] + i + 1`` keys, or the last ``window`` of
+    them, at ``block_table[r]`` (int32 [R, width], rows may be strided).  A row that sees no key is 0; rows of no request are left as
+    they are.  A key whose block-table entry is no page, or lies behind the table, is not seen.  ``most_rows`` and ``most_keys`` are the
+    largest of q_len and seq_len as far as the host knows them: they choose the shape of the launch, not the result."""
+    _need_contiguous(q, out, q_start, q_len, seq_len)
+    H, KV, R = num_heads, num_kv_heads, q_len.numel()
+    if H < 1 or KV < 1 or H % KV:
+        raise KernelError("kv4_attention: num_heads must be a multiple of num_kv_heads")
+    _kv4_pages("kv4_attention", pages, KV, page_tokens, head_dim)
+    if q.dim() != 2 or q.shape[1] != H * head_dim or out.shape != q.shape or out.dtype != q.dtype:
+        raise KernelError("kv4_attention: q and out must be [T, num_heads * head_dim] of one dtype")
+    for t in (q_start, q_len, seq_len):
+        if t.dtype != torch.int32 or t.numel() != R:
+            raise KernelError("kv4_attention: q_start, q_len and seq_len must be int32 [R]")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != R \
+            or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise KernelError("kv4_attention: block_table must be int32 [R, width] with neighbouring entries")
+    if window is not None and window < 0:
+        raise KernelError("kv4_attention: a window is at least 1")
+    dtype = _dtype_code(q)
+    _need_aligned("kv4_attention", q, out)
+    _need_cuda(q, pages, out, q_start, q_len, seq_len, block_table)
+    _need_here("kv4_attention", q, pages, out, q_start, q_len, seq_len, block_table)
+    p = Kv4AttnParams(
+        q=q.data_ptr(), pages=pages.data_ptr(), out=out.data_ptr(), q_start=q_start.data_ptr(), q_len=q_len.data_ptr(),
+        seq_len=seq_len.data_ptr(), block_table=block_table.data_ptr(), bt_stride=block_table.stride(0),
+        table_pages=block_table.shape[1], num_pages=pages.shape[0], requests=R, rows=q.shape[0], heads=H, kv_heads=KV,
+        page_tokens=page_tokens, window=int(window or 0), scale=float(scale))
+    fn = _fn("kv4_attention", "pbe_kv4_attention", [ctypes.POINTER(Kv4AttnParams), c_int, c_int, c_int, c_void_p])
+    _check(fn(ctypes.byref(p), head_dim, int(most_rows), dtype, _stream()), "kv4_attention")
     return out
