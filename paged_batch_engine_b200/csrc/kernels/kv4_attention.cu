@@ -1,13 +1,33 @@
-// Causal attention of every row over 4-bit pages (kv4.cuh).
+// Causal attention over 4-bit pages (kv4.cuh) for decoded tokens and short portions.
 //
-// A warp takes one row of one head and walks over its keys one by one: the dot product over the lanes, the running maximum and
-// sum of the softmax, and each lane's channels of the output in float32.
+// Codes are operands as they are.  A code shifted to the low bits of a bfloat16 is the number code * 2^-133 (in bits 4-7,
+// sixteen times that), exactly: one AND takes a pair of codes out of a word and makes a tensor-core operand of it, nothing is
+// converted and nothing rounded.  The group's numbers come in outside the products:
+//   scores   S[h, t] = sum_g s[t, g] (Q_g . code_g)[h, t] + sum_g lo[t, g] Qsum[h, g]
+//   output   O[h, c] = sum_t (P[h, t] s[t, g]) code[t, c] + sum_t P[h, t] lo[t, g]
+// The first sums run over each group's 32 channels (two mma.sync m16n8k16) and are scaled in float32; the second are one small
+// product each, Qsum in three bfloat16 terms.  Q and P carry a factor 2^64, so that the products of the tiny codes stay
+// in float32's normal range for |Q| < 2^63 and spans of values below 2^60.
+//
+// S is made with the rows (packed: query row x head of the group) as M and the keys as N, O transposed, with the channels as M
+// and the rows as N: the scores' registers are the second product's B operand as they lie, and eight rows cost it nothing in
+// vain.  A warp takes tiles of 16 keys, one record each, through a ring of its own in shared memory (cp.async, four deep), and
+// keeps a running maximum that moves only when it grew by 2^8.
+//
+// Work is cut by bytes, not by requests: the tiles of all (request, head, row tile) laid end to end are shared out evenly over
+// the blocks, so one long context among short ones leaves no block idle.  A block's warps merge their parts in shared memory;
+// an item that several blocks share is merged by a second kernel, always in the blocks' order.
+//
+// Float32: queries and weights as three bfloat16 terms each, the codes are exact as they are.
 #include "common.cuh"
 #include "kv4.cuh"
+#include "mma_sync.cuh"
+#include "opt_in.cuh"
 #include "pdl.cuh"
 
 using namespace pbe;
 using namespace pbe::kv4;
+using namespace pbe::mma_sync;
 
 namespace {
 struct Kv4AttnParams {
@@ -22,52 +42,521 @@ struct Kv4AttnParams {
   int table_pages, num_pages, requests, rows, heads, kv_heads, page_tokens, window;
   float scale;
 };
+struct Split {
+  float* part_o;               // [2 blocks][rows of a tile][D]
+  float* part_ml;              // [2 blocks][rows of a tile][2]
+  long long* ends;             // [1 + requests]: units a block, then where each request's units end
+  int most_packed;             // requests of more packed rows are another kernel's
+};
 
-template <typename T, int D>
-__global__ void kv4_attention_kernel(Kv4AttnParams p) {
-  pdl_wait();
-  constexpr int E = D / 32, G = D / GROUP;
-  const int r = blockIdx.x, lane = threadIdx.x & 31, H = p.heads, head = blockIdx.y, kvh = head / (H / p.kv_heads);
-  const int n = p.q_len[r], seq = p.seq_len[r], q0 = p.q_start[r];
-  for (int i = blockIdx.z * (blockDim.x >> 5) + (threadIdx.x >> 5); i < n; i += gridDim.z * (blockDim.x >> 5)) {
-    if (q0 + i >= p.rows) return;
-    const int pos = seq - n + i;
-    const size_t at = ((size_t)(q0 + i) * H + head) * D;
-    float q[E], o[E] = {}, m = -INFINITY, l = 0.f;
-    for (int e = 0; e < E; ++e) q[e] = to_float(((const T*)p.q)[at + e * 32 + lane]);
-    for (int key = p.window > 0 ? max(0, pos - p.window + 1) : 0; key <= pos; ++key) {
-      const int blk = key / p.page_tokens, off = key % p.page_tokens, tok = off % REC_TOKENS;
-      const int page = blk < p.table_pages ? p.block_table[r * p.bt_stride + blk] : -1;
-      if (page < 0 || page >= p.num_pages) continue;
-      const unsigned char* rec = p.pages + record_at(page, kvh, off, p.kv_heads, p.page_tokens, D);
-      auto number = [&](int kind, int g) { return __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(rec + number_at(D, kind, tok, g))); };
-      float dot = 0.f, v[E];
-      for (int g = 0; g < E; ++g) {                    // the lane's channel of each group
-        const int kb = 32 * ((tok * 4 + lane / 8) * G + g) + 16 * (lane & 1) + 4 * (lane % 8 >> 1);
-        const int vb = 32 * ((tok / 2 * 8 + lane / 4) * G + g) + 16 * (tok & 1) + 4 * (lane & 3);
-        dot = fmaf(q[g], fmaf(number(K_S, g), (float)(rec[kb / 8] >> (kb & 7) & 15), number(K_LO, g)), dot);
-        v[g] = fmaf(number(V_S, g), (float)(rec[v_codes(D) + vb / 8] >> (vb & 7) & 15), number(V_LO, g));
-      }
-      const float s = warp_sum(dot) * p.scale, m2 = fmaxf(m, s), a = expf(m - m2), w = expf(s - m2);
-      l = l * a + w;
-      m = m2;
-      for (int g = 0; g < E; ++g) o[g] = o[g] * a + w * v[g];
-    }
-    for (int e = 0; e < E; ++e) ((T*)p.out)[at + e * 32 + lane] = from_float<T>(l > 0.f ? o[e] / l : 0.f);
+constexpr int WARPS = 8;
+constexpr int STAGES = 4;
+constexpr int MIN_UNITS = 16;  // tiles a block takes at least: two a warp
+constexpr int MOST_REQUESTS = 8192;
+constexpr float UP = 18446744073709551616.f;           // 2^64
+constexpr float CODE = 590295810358705651712.f;        // 2^69 = 2^133 / 2^64
+
+struct Request {
+  int rows, seq, pos0, first, tiles, row_tiles;        // first: the first 16-key tile, tiles: how many, at least one
+};
+__device__ __forceinline__ Request request(const Kv4AttnParams& p, const Split& s, int r, int tile_rows) {
+  Request q;
+  q.rows = max(0, p.q_len[r]);
+  q.seq = max(0, p.seq_len[r]);
+  q.pos0 = q.seq - q.rows;
+  const int G = p.heads / p.kv_heads;
+  const long long packed = (long long)q.rows * G;
+  q.row_tiles = packed > s.most_packed ? 0 : (int)((packed + tile_rows - 1) / tile_rows);
+  const int low = p.window > 0 ? max(0, q.pos0 - p.window + 1) : 0;
+  q.first = low / REC_TOKENS;
+  q.tiles = max(1, (int)(((long long)q.seq + REC_TOKENS - 1) / REC_TOKENS) - q.first);
+  return q;
+}
+// the first request whose units end behind `unit`
+__device__ __forceinline__ int find(const long long* ends, int requests, long long unit) {
+  int lo = 0, hi = requests;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (ends[mid] > unit) hi = mid; else lo = mid + 1;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ unsigned pack2(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+__device__ __forceinline__ unsigned mul2(unsigned a, unsigned b) {
+  const __nv_bfloat162 h = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+__device__ __forceinline__ float low_half(unsigned w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high_half(unsigned w) { return __uint_as_float(w & 0xffff0000u); }
+// x and y as pairs of N bfloat16 terms, the largest first
+template <int N>
+__device__ __forceinline__ void split(float x, float y, unsigned (&t)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    t[i] = pack2(x, y);
+    x -= low_half(t[i]);
+    y -= high_half(t[i]);
   }
 }
+// N words from shared memory, as wide as they come
+template <int N>
+__device__ __forceinline__ void words(unsigned (&w)[N], const unsigned char* p) {
+  static_assert(N == 2 || N == 4, "");
+  if constexpr (N == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+  }
+}
+
+// T: the queries' type; NT: tiles of eight packed rows a warp; TERMS: bfloat16 terms of queries and weights
+template <typename T, int D, int NT, int TERMS>
+__global__ void __launch_bounds__(WARPS * 32, (TERMS == 1 && (NT == 1 || D == 64)) ? 2 : 1)
+kv4_attention_kernel(Kv4AttnParams p, Split sp) {
+  constexpr int G = D / GROUP, REC = rec_bytes(D), MT = 8 * NT, RING = WARPS * STAGES * REC;
+  constexpr int MERGE = WARPS * MT * (D + 2) * 4;
+  constexpr int SHARED = RING > MERGE ? RING : MERGE;
+  extern __shared__ __align__(16) unsigned char smem[];
+  long long* ends = reinterpret_cast<long long*>(smem + SHARED);
+  __shared__ long long warp_sums[WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r8 = lane >> 2, j = lane & 3;
+  const int H = p.heads, KV = p.kv_heads, HG = H / KV, per_page = p.page_tokens / REC_TOKENS;
+  pdl_wait();
+
+  // where each request's units end (a unit: one tile of 16 keys for one head and row tile)
+  long long total = 0;
+  for (int r0 = 0; r0 < p.requests; r0 += WARPS * 32) {
+    const int r = r0 + threadIdx.x;
+    long long v = 0;
+    if (r < p.requests) {
+      const Request q = request(p, sp, r, MT);
+      v = (long long)q.tiles * q.row_tiles * KV;
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    if (lane == 31) warp_sums[warp] = v;
+    __syncthreads();
+    long long before = total;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) before += warp_sums[w];
+      total += warp_sums[w];
+    }
+    if (r < p.requests) ends[r] = before + v;
+    __syncthreads();
+  }
+  const long long per_block = max((long long)MIN_UNITS, (total + gridDim.x - 1) / gridDim.x);
+  if (blockIdx.x == 0) {
+    for (int r = threadIdx.x; r < p.requests; r += WARPS * 32) sp.ends[1 + r] = ends[r];
+    if (threadIdx.x == 0) sp.ends[0] = per_block;
+  }
+  pdl_launch_dependents();
+  const float to_log2 = p.scale * 1.4426950408889634f * CODE;
+
+  unsigned char* ring = smem + warp * STAGES * REC;
+  long long unit = per_block * blockIdx.x;
+  const long long unit0 = unit, unit_end = min(unit + per_block, total);
+  while (unit < unit_end) {
+    // ---- the next item, or this block's part of it
+    const int req = find(ends, p.requests, unit);
+    const Request q = request(p, sp, req, MT);
+    const long long begin = req > 0 ? ends[req - 1] : 0;
+    const int item = (int)((unit - begin) / q.tiles);
+    const int t_begin = (int)((unit - begin) - (long long)item * q.tiles);
+    const int t_end = (int)min((long long)q.tiles, t_begin + (unit_end - unit));
+    const int kvh = item / q.row_tiles, row_tile = item - kvh * q.row_tiles;
+    const int packed = q.rows * HG, pr0 = row_tile * MT;
+    const int q0 = p.q_start[req];
+    // this lane's rows of the scores (r8, and r8 + 8 with two row tiles) and their positions
+    int pos[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) pos[n] = pr0 + n * 8 + r8 < packed ? q.pos0 + (pr0 + n * 8 + r8) / HG : -1;
+    const int pos_min = q.pos0 + pr0 / HG, pos_max = q.pos0 + (min(pr0 + MT, packed) - 1) / HG;
+    const int low_min = p.window > 0 ? pos_min - p.window + 1 : 0, low_max = p.window > 0 ? pos_max - p.window + 1 : 0;
+
+    // ---- queries: A fragments, and their sums over each group
+    unsigned qa[TERMS][G * 2][2 * NT], za[2 * NT][2];
+    float qsum[NT][G];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int pr = pr0 + n * 8 + r8;
+      const bool live = pr < packed && q0 + pr / HG < p.rows && q0 >= 0;
+      const T* src = (const T*)p.q + ((size_t)(live ? q0 + pr / HG : 0) * H + kvh * HG + pr % HG) * D + 8 * j;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        float x[8];
+        if constexpr (sizeof(T) == 2) {
+          uint4 w = make_uint4(0, 0, 0, 0);
+          if (live) w = *reinterpret_cast<const uint4*>(src + 32 * g);
+          const unsigned u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[2 * i] = low_half(u[i]), x[2 * i + 1] = high_half(u[i]);
+        } else {
+          float4 a = make_float4(0, 0, 0, 0), b = a;
+          if (live) {
+            a = *reinterpret_cast<const float4*>(src + 32 * g);
+            b = *reinterpret_cast<const float4*>(src + 32 * g + 4);
+          }
+          x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+        }
+        qsum[n][g] = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+        qsum[n][g] += __shfl_xor_sync(0xffffffffu, qsum[n][g], 1);
+        qsum[n][g] += __shfl_xor_sync(0xffffffffu, qsum[n][g], 2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {                  // pair i of the word: its codes come 16 times too large for odd i
+          const float f = i & 1 ? UP / 16.f : UP;
+          unsigned t[TERMS];
+          split<TERMS>(x[2 * i] * f, x[2 * i + 1] * f, t);
+#pragma unroll
+          for (int e = 0; e < TERMS; ++e) qa[e][2 * g + (i >> 1)][(i & 1) * NT + n] = t[e];
+        }
+      }
+      // three terms of the sums along the product's k: term * G + g
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int k = 2 * j + 8 * half, term = k / G, g0 = k % G;
+        float a = 0.f, b = 0.f;
+#pragma unroll
+        for (int g = 0; g < G; g += 2)
+          if (g == g0) a = qsum[n][g] / CODE, b = qsum[n][g + 1] / CODE;
+        unsigned t[3];
+        split<3>(a, b, t);
+        za[half * NT + n][0] = term == 0 ? t[0] : term == 1 ? t[1] : term == 2 ? t[2] : 0u;
+      }
+    }
+
+    float o[NT][2 * G][4] = {}, z[NT][4] = {}, m[NT], l[NT] = {};
+#pragma unroll
+    for (int n = 0; n < NT; ++n) m[n] = -INFINITY;
+
+    // ---- this warp's tiles: t_begin + warp, + 8, ...
+    const int mine = t_end - t_begin > warp ? (t_end - t_begin - warp + WARPS - 1) / WARPS : 0;
+    const int32_t* table = p.block_table + (long long)req * p.bt_stride;
+    auto record = [&](int i) {                         // the record of this warp's tile i, -1: none to be seen
+      if (i >= mine) return -1;
+      const int t = q.first + t_begin + warp + i * WARPS, blk = t / per_page;
+      if (blk >= p.table_pages || t * REC_TOKENS > pos_max || t * REC_TOKENS + REC_TOKENS <= low_min) return -1;
+      const int page = table[blk];
+      return page >= 0 && page < p.num_pages ? (page * KV + kvh) * per_page + (t - blk * per_page) : -1;
+    };
+    int recs = record(lane), recs_next = record(32 + lane);
+    unsigned there = 0;                                // bit i: the tile issued i tiles ago has a record
+    auto issue = [&](int i) {
+      if (i > 0 && (i & 31) == 0) {
+        recs = recs_next;
+        recs_next = record(i + 32 + lane);
+      }
+      const int rec = __shfl_sync(0xffffffffu, recs, i & 31);
+      there = there << 1 | (rec >= 0 ? 1u : 0u);
+      if (rec >= 0) {
+        const unsigned char* src = p.pages + (long long)rec * REC;
+        unsigned char* dst = ring + (i % STAGES) * REC;
+#pragma unroll
+        for (int c = 0; c < (REC + 511) / 512; ++c) {
+          const int at = (c * 32 + lane) * 16;
+          if (REC % 512 == 0 || at < REC) cp16(dst + at, src + at, true);
+        }
+      }
+      cp_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) issue(i);
+    for (int i = 0; i < mine; ++i) {
+      cp_wait<STAGES - 2>();
+      __syncwarp();                                    // the tile has landed, and the one before is read
+      const bool seen = there >> (STAGES - 2) & 1;
+      const unsigned char* rec = ring + (i % STAGES) * REC;
+      issue(i + STAGES - 1);
+      if (!seen) continue;
+      const int key0 = (q.first + t_begin + warp + i * WARPS) * REC_TOKENS;
+      const unsigned char* num = rec + numbers(D);
+
+      // ---- scores of 16 keys: two tiles of eight
+      float s[2][2 * NT][2];                           // [key tile][.][key 2j, 2j + 1]
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        unsigned w[G], ks[G], lo2[2];
+        words<G>(w, rec + (n * 8 + r8) * (D / 2) + j * (4 * G));
+        words<G>(ks, num + K_S * D + (n * 4 + j) * (4 * G));
+        words<2>(lo2, num + K_LO * D + (n * 4 + (r8 >> 1)) * (4 * G) + (G == 4 ? (j & 1) * 8 : 0));
+        const unsigned lo = __byte_perm(lo2[0], lo2[1], r8 & 1 ? 0x7632 : 0x5410);
+        float acc[4] = {};
+        {
+          unsigned a[4] = {za[0][0], NT == 2 ? za[NT - 1][0] : 0u, za[NT][0], NT == 2 ? za[2 * NT - 1][0] : 0u};
+          mma(acc, a, lo, lo);
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          float c[4] = {};
+#pragma unroll
+          for (int e = 0; e < TERMS; ++e) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const unsigned u = h ? w[g] >> 8 : w[g];
+              const unsigned(&f)[2 * NT] = qa[e][2 * g + h];
+              unsigned a[4] = {f[0], NT == 2 ? f[NT - 1] : 0u, f[NT], NT == 2 ? f[2 * NT - 1] : 0u};
+              mma(c, a, u & 0x000f000fu, u & 0x00f000f0u);
+            }
+          }
+          const float s0 = low_half(ks[g]), s1 = high_half(ks[g]);
+          acc[0] = fmaf(s0, c[0], acc[0]);
+          acc[1] = fmaf(s1, c[1], acc[1]);
+          if (NT == 2) {
+            acc[2] = fmaf(s0, c[2], acc[2]);
+            acc[3] = fmaf(s1, c[3], acc[3]);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < NT; ++k) s[n][k][0] = acc[2 * k] * to_log2, s[n][k][1] = acc[2 * k + 1] * to_log2;
+      }
+      // ---- masks, on the tiles that need them
+      const bool edge = key0 + REC_TOKENS - 1 > pos_min || key0 < low_max;
+      if (edge) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int k = 0; k < NT; ++k)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int key = key0 + n * 8 + 2 * j + e;
+              if (key > pos[k] || (p.window > 0 && key <= pos[k] - p.window)) s[n][k][e] = -INFINITY;
+            }
+      }
+      // ---- the running maximum, moved only when it grew by more than 2^8
+      bool grew = false;
+      float top[NT];
+#pragma unroll
+      for (int k = 0; k < NT; ++k) {
+        top[k] = fmaxf(fmaxf(s[0][k][0], s[0][k][1]), fmaxf(s[1][k][0], s[1][k][1]));
+        grew = grew || top[k] > m[k] + 8.f;
+      }
+      if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+        for (int k = 0; k < NT; ++k) {
+          top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
+          top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2));
+          const float now = fmaxf(m[k], top[k]);
+          const float a = now == -INFINITY ? 1.f : ex2(m[k] - now);
+          m[k] = now;
+          l[k] *= a;
+          const float a0 = __shfl_sync(0xffffffffu, a, 8 * j), a1 = __shfl_sync(0xffffffffu, a, 8 * j + 4);
+#pragma unroll
+          for (int c = 0; c < 2 * G; ++c) o[k][c][0] *= a0, o[k][c][1] *= a1, o[k][c][2] *= a0, o[k][c][3] *= a1;
+          z[k][0] *= a0, z[k][1] *= a1;
+        }
+      }
+      // ---- weights, and the values they weigh
+      unsigned vs[2][G], vlo[2];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        words<G>(vs[n], num + V_S * D + (n * 4 + j) * (4 * G));
+        vlo[n] = r8 < G ? *reinterpret_cast<const unsigned*>(num + V_LO * D + (n * 4 + j) * (4 * G) + r8 * 4) : 0u;
+      }
+      if (edge) {                                      // numbers of places that hold no key of this row tile may be anything
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const int key = key0 + n * 8 + 2 * j;
+          const unsigned keep = (key <= pos_max && key >= low_min ? 0xffffu : 0u) |
+                                (key + 1 <= pos_max && key + 1 >= low_min ? 0xffff0000u : 0u);
+          vlo[n] &= keep;
+#pragma unroll
+          for (int g = 0; g < G; ++g) vs[n][g] &= keep;
+        }
+      }
+      float w[2][NT][2];
+#pragma unroll
+      for (int k = 0; k < NT; ++k) {
+        const float off = m[k] == -INFINITY ? 0.f : 64.f - m[k];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) w[n][k][e] = TERMS == 1 ? ex2(s[n][k][e] + off) : exp2f(s[n][k][e] + off);
+          l[k] += w[n][k][0] + w[n][k][1];
+        }
+      }
+      unsigned wp[NT][2][TERMS];
+#pragma unroll
+      for (int k = 0; k < NT; ++k)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) split<TERMS>(w[n][k][0], w[n][k][1], wp[k][n]);
+      {
+        const unsigned a[4] = {vlo[0], 0u, vlo[1], 0u};
+#pragma unroll
+        for (int k = 0; k < NT; ++k)
+#pragma unroll
+          for (int e = 0; e < TERMS; ++e) mma(z[k], a, wp[k][0][e], wp[k][1][e]);
+      }
+      unsigned v0[G], v1[G];
+      words<G>(v0, rec + v_codes(D) + j * D + r8 * (4 * G));
+      words<G>(v1, rec + v_codes(D) + (j + 4) * D + r8 * (4 * G));
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        unsigned b[NT][2][TERMS];
+#pragma unroll
+        for (int k = 0; k < NT; ++k)
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            if constexpr (TERMS == 1) b[k][n][0] = mul2(wp[k][n][0], vs[n][g]);     // rounded once more, as the weight was
+            else split<TERMS>(w[n][k][0] * low_half(vs[n][g]), w[n][k][1] * high_half(vs[n][g]), b[k][n]);
+          }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const unsigned x = h ? v0[g] >> 8 : v0[g], y = h ? v1[g] >> 8 : v1[g];
+          const unsigned a[4] = {x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u};
+#pragma unroll
+          for (int k = 0; k < NT; ++k)
+#pragma unroll
+            for (int e = 0; e < TERMS; ++e) mma(o[k][2 * g + h], a, b[k][0][e], b[k][1][e]);
+        }
+      }
+    }
+    cp_wait<0>();
+    __syncthreads();                                   // every warp is through with its ring
+
+    // ---- the block's warps merged
+    float* om = reinterpret_cast<float*>(smem);        // [warp][row][D]
+    float* mm = om + WARPS * MT * D;                   // [warp][row]
+    float* lm = mm + WARPS * MT;
+#pragma unroll
+    for (int k = 0; k < NT; ++k) {
+      l[k] += __shfl_xor_sync(0xffffffffu, l[k], 1);
+      l[k] += __shfl_xor_sync(0xffffffffu, l[k], 2);
+      if (j == 0) {
+        mm[warp * MT + k * 8 + r8] = m[k];
+        lm[warp * MT + k * 8 + r8] = l[k] * (1.f / UP);
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float z0 = __shfl_sync(0xffffffffu, z[k][0], g * 4 + j) * (1.f / UP);
+        const float z1 = __shfl_sync(0xffffffffu, z[k][1], g * 4 + j) * (1.f / UP);
+        const float(&a)[4] = o[k][2 * g], (&b)[4] = o[k][2 * g + 1];
+        constexpr float odd = CODE / 16.f;
+        float* dst = om + (warp * MT + k * 8 + 2 * j) * D + 32 * g + 4 * r8;
+        *reinterpret_cast<float4*>(dst) = make_float4(fmaf(a[0], CODE, z0), fmaf(a[2], odd, z0), fmaf(b[0], CODE, z0), fmaf(b[2], odd, z0));
+        *reinterpret_cast<float4*>(dst + D) = make_float4(fmaf(a[1], CODE, z1), fmaf(a[3], odd, z1), fmaf(b[1], CODE, z1), fmaf(b[3], odd, z1));
+      }
+    }
+    __syncthreads();
+    const bool whole = t_begin == 0 && t_end == q.tiles;
+    const int slot = 2 * blockIdx.x + (unit == unit0 ? 0 : 1);
+    for (int e = threadIdx.x; e < MT * (D / 4); e += WARPS * 32) {
+      const int row = e / (D / 4), c4 = (e % (D / 4)) * 4, pr = pr0 + row;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) top = fmaxf(top, mm[w * MT + row]);
+      const float base = top == -INFINITY ? 0.f : top;
+      float sum = 0.f;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float f = exp2f(mm[w * MT + row] - base);
+        const float4 y = *reinterpret_cast<const float4*>(om + (w * MT + row) * D + c4);
+        sum = fmaf(f, lm[w * MT + row], sum);
+        x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
+      }
+      if (!whole) {
+        const size_t at = (size_t)slot * MT + row;
+        *reinterpret_cast<float4*>(sp.part_o + at * D + c4) = x;
+        if (c4 == 0) sp.part_ml[at * 2] = top, sp.part_ml[at * 2 + 1] = sum;
+      } else if (pr < packed && q0 >= 0 && q0 + pr / HG < p.rows) {
+        const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;      // a row whose scores are NaN stays NaN
+        T* dst = (T*)p.out + ((size_t)(q0 + pr / HG) * H + kvh * HG + pr % HG) * D + c4;
+        if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(x.x * inv, x.y * inv), pack2(x.z * inv, x.w * inv));
+        else *reinterpret_cast<float4*>(dst) = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+      }
+    }
+    __syncthreads();                                   // the merged parts are read before the ring is filled again
+    unit += t_end - t_begin;
+  }
+}
+
+// Items that several blocks share: block b looks at the border between blocks b and b + 1 of the kernel above, and merges the
+// item that lies across it if that is the item's first border.
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(256) kv4_merge_kernel(Kv4AttnParams p, Split sp) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const long long per_block = sp.ends[0];
+  const long long* ends = sp.ends + 1;
+  const long long border = per_block * (blockIdx.x + 1);
+  if (border >= ends[p.requests - 1]) return;
+  const int req = find(ends, p.requests, border);
+  const Request q = request(p, sp, req, MT);
+  const long long begin = req > 0 ? ends[req - 1] : 0;
+  const int item = (int)((border - begin) / q.tiles);
+  const long long first = begin + (long long)item * q.tiles, last = first + q.tiles;
+  if (first == border || first < border - per_block) return;
+  const int H = p.heads, KV = p.kv_heads, HG = H / KV, kvh = item / q.row_tiles, row_tile = item - kvh * q.row_tiles;
+  const int q0 = p.q_start[req], packed = q.rows * HG;
+  const int b0 = blockIdx.x, b1 = (int)((last - 1) / per_block);
+  auto slot = [&](int b) { return 2 * b + (per_block * b >= first ? 0 : 1); };
+  for (int e = threadIdx.x; e < MT * (D / 4); e += 256) {
+    const int row = e / (D / 4), c4 = (e % (D / 4)) * 4, pr = row_tile * MT + row;
+    if (pr >= packed || q0 < 0 || q0 + pr / HG >= p.rows) continue;
+    float top = -INFINITY;
+    for (int b = b0; b <= b1; ++b) top = fmaxf(top, sp.part_ml[((size_t)slot(b) * MT + row) * 2]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int b = b0; b <= b1; ++b) {
+      const size_t at = (size_t)slot(b) * MT + row;
+      const float f = exp2f(sp.part_ml[at * 2] - base);
+      const float4 y = *reinterpret_cast<const float4*>(sp.part_o + at * D + c4);
+      sum = fmaf(f, sp.part_ml[at * 2 + 1], sum);
+      x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
+    }
+    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+    T* dst = (T*)p.out + ((size_t)(q0 + pr / HG) * H + kvh * HG + pr % HG) * D + c4;
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(x.x * inv, x.y * inv), pack2(x.z * inv, x.w * inv));
+    else *reinterpret_cast<float4*>(dst) = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+  }
+}
+
+template <typename T, int D, int NT, int TERMS>
+int launch(const Kv4AttnParams& p, const Split& sp, int blocks, cudaStream_t stream) {
+  constexpr int MT = 8 * NT, ring = WARPS * STAGES * rec_bytes(D), merge = WARPS * MT * (D + 2) * 4;
+  const size_t smem = (ring > merge ? ring : merge) + (size_t)p.requests * sizeof(long long);
+  static OptIn opt_in;
+  if (const cudaError_t e = opt_in(smem, kv4_attention_kernel<T, D, NT, TERMS>)) return (int)e;
+  launch_k(kv4_attention_kernel<T, D, NT, TERMS>, blocks, WARPS * 32, smem, stream, p, sp);
+  if (blocks > 1) launch_k(kv4_merge_kernel<T, D, MT>, blocks - 1, 256, 0, stream, p, sp);
+  return launch_status();
+}
+
 }  // namespace
 
-PBE_EXPORT int pbe_kv4_attention(const Kv4AttnParams* params, int head_dim, int most_rows, int dtype, cudaStream_t stream) {
+// workspace: 2 (1 + requests) floats, rounded up to four, then 2 blocks * tile rows * (head_dim + 2).  tile_rows: 8, or 16
+// (bfloat16); requests of more than most_packed packed rows are left out.
+PBE_EXPORT int pbe_kv4_attention(const Kv4AttnParams* params, float* workspace, int blocks, int head_dim, int tile_rows,
+                                 int most_packed, int dtype, cudaStream_t stream) {
   const Kv4AttnParams p = *params;
   if (p.requests <= 0 || p.rows <= 0) return 0;
-  const dim3 grid(p.requests, p.heads, most_rows > 128 ? 32 : most_rows > 1 ? 4 : 1);
-  if (dtype == PBE_F32) {
-    if (head_dim == 64) launch_k(kv4_attention_kernel<float, 64>, grid, 128, 0, stream, p);
-    else launch_k(kv4_attention_kernel<float, 128>, grid, 128, 0, stream, p);
-  } else {
-    if (head_dim == 64) launch_k(kv4_attention_kernel<__nv_bfloat16, 64>, grid, 128, 0, stream, p);
-    else launch_k(kv4_attention_kernel<__nv_bfloat16, 128>, grid, 128, 0, stream, p);
-  }
-  return launch_status();
+  if (p.requests > MOST_REQUESTS || blocks < 1 || (head_dim != 64 && head_dim != 128) ||
+      !(tile_rows == 8 || (tile_rows == 16 && dtype == PBE_BF16)))
+    return (int)cudaErrorInvalidValue;
+  Split sp;
+  sp.ends = reinterpret_cast<long long*>(workspace);
+  sp.part_o = workspace + ((2 * (1 + p.requests) + 3) & ~3);
+  sp.part_ml = sp.part_o + (size_t)2 * blocks * tile_rows * head_dim;
+  sp.most_packed = most_packed;
+  if (dtype == PBE_F32)
+    return head_dim == 64 ? launch<float, 64, 1, 3>(p, sp, blocks, stream) : launch<float, 128, 1, 3>(p, sp, blocks, stream);
+  typedef __nv_bfloat16 B;
+  if (tile_rows == 8)
+    return head_dim == 64 ? launch<B, 64, 1, 1>(p, sp, blocks, stream) : launch<B, 128, 1, 1>(p, sp, blocks, stream);
+  return head_dim == 64 ? launch<B, 64, 2, 1>(p, sp, blocks, stream) : launch<B, 128, 2, 1>(p, sp, blocks, stream);
 }

@@ -2860,6 +2860,20 @@ class Kv4AttnParams(ctypes.Structure):
                                                       "page_tokens", "window")] + [("scale", c_float)]
 
 
+KV4_MAX_REQUESTS = 8192
+KV4_UNITS = 16              # tiles of 16 keys a block takes at least, two a warp
+
+
+def _kv4_shape(requests: int, heads: int, kv_heads: int, head_dim: int, most_rows: int, most_keys: int, wide: bool, sms: int):
+    """(packed rows of a tile, blocks) of the kernel for decoded tokens and short portions: as many blocks as the GPU holds
+    at once (one a multiprocessor where a warp's registers leave no more), fewer where there is less to do."""
+    tile_rows = 16 if wide and most_rows * (heads // kv_heads) > 8 else 8
+    resident = sms * (2 if wide and (tile_rows == 8 or head_dim == 64) else 1)
+    row_tiles = -(-max(1, most_rows) * (heads // kv_heads) // tile_rows)
+    units = requests * row_tiles * kv_heads * (-(-max(1, most_keys) // KV4_PAGE_UNIT))
+    return tile_rows, max(1, min(-(-units // KV4_UNITS), resident))
+
+
 def kv4_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor,
                   seq_len: torch.Tensor, block_table: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int,
                   scale: float, window: Optional[int], page_tokens: int, most_rows: int, most_keys: int) -> torch.Tensor:
@@ -2881,6 +2895,8 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, q_sta
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != R \
             or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
         raise KernelError("kv4_attention: block_table must be int32 [R, width] with neighbouring entries")
+    if R > KV4_MAX_REQUESTS:
+        raise KernelError(f"kv4_attention takes at most {KV4_MAX_REQUESTS} requests, got {R}")
     if window is not None and window < 0:
         raise KernelError("kv4_attention: a window is at least 1")
     dtype = _dtype_code(q)
@@ -2892,6 +2908,9 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, q_sta
         seq_len=seq_len.data_ptr(), block_table=block_table.data_ptr(), bt_stride=block_table.stride(0),
         table_pages=block_table.shape[1], num_pages=pages.shape[0], requests=R, rows=q.shape[0], heads=H, kv_heads=KV,
         page_tokens=page_tokens, window=int(window or 0), scale=float(scale))
-    fn = _fn("kv4_attention", "pbe_kv4_attention", [ctypes.POINTER(Kv4AttnParams), c_int, c_int, c_int, c_void_p])
-    _check(fn(ctypes.byref(p), head_dim, int(most_rows), dtype, _stream()), "kv4_attention")
+    tile_rows, blocks = _kv4_shape(R, H, KV, head_dim, most_rows, most_keys, q.dtype == torch.bfloat16, multiprocessors(q.device))
+    floats = (2 * (1 + R) + 3) // 4 * 4 + 2 * blocks * tile_rows * (head_dim + 2)
+    work = torch.empty(floats, dtype=torch.float32, device=q.device)
+    fn = _fn("kv4_attention", "pbe_kv4_attention", [ctypes.POINTER(Kv4AttnParams), c_void_p] + [c_int] * 5 + [c_void_p])
+    _check(fn(ctypes.byref(p), _ptr(work), blocks, head_dim, tile_rows, 0x7fffffff, dtype, _stream()), "kv4_attention")
     return out
