@@ -9,16 +9,19 @@
 // product each, Qsum in three bfloat16 terms.  Q and P carry a factor 2^64, so that the products of the tiny codes stay
 // in float32's normal range for |Q| < 2^63 and spans of values below 2^60.
 //
-// S is made with the rows (packed: query row x head of the group) as M and the keys as N, O transposed, with the channels as M
-// and the rows as N: the scores' registers are the second product's B operand as they lie, and eight rows cost it nothing in
-// vain.  A warp takes tiles of 16 keys, one record each, through a ring of its own in shared memory (cp.async, four deep), and
-// keeps a running maximum that moves only when it grew by 2^8.
+// Both products have the keys' or the channels' codes as A (16 keys, 16 channels) and the rows (packed: query row x head of the
+// group) as B, eight at a time, so eight rows leave no lane idle; the weights pass from the one's result to the other's operand
+// through movmatrix.  Sums are float32; weights times s are rounded to float16 once (2^-12; a running exponent over the
+// values' s keeps them in its range).  A warp takes tiles of 16 keys, one record each, through a ring of its own in shared
+// memory (cp.async, four deep), and keeps a running maximum that moves only when it grew by 2^8.
 //
 // Work is cut by bytes, not by requests: the tiles of all (request, head, row tile) laid end to end are shared out evenly over
 // the blocks, so one long context among short ones leaves no block idle.  A block's warps merge their parts in shared memory;
 // an item that several blocks share is merged by a second kernel, always in the blocks' order.
 //
 // Float32: queries and weights as three bfloat16 terms each, the codes are exact as they are.
+#include <cuda_fp16.h>
+
 #include "common.cuh"
 #include "kv4.cuh"
 #include "mma_sync.cuh"
@@ -54,7 +57,10 @@ constexpr int STAGES = 4;
 constexpr int MIN_UNITS = 16;  // tiles a block takes at least: two a warp
 constexpr int MOST_REQUESTS = 8192;
 constexpr float UP = 18446744073709551616.f;           // 2^64
-constexpr float CODE = 590295810358705651712.f;        // 2^69 = 2^133 / 2^64
+constexpr float CODE = 590295810358705651712.f;        // 2^69 = 2^133 / 2^64: products of bfloat16 codes
+constexpr float CODE16 = 16777216.f;                   // 2^24: products of float16 codes
+constexpr int ROOM = 6;                                // weights are kept 2^6 times too large
+constexpr int MOST_E = 60;
 
 struct Request {
   int rows, seq, pos0, first, tiles, row_tiles;        // first: the first 16-key tile, tiles: how many, at least one
@@ -91,9 +97,25 @@ __device__ __forceinline__ unsigned pack2(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const unsigned*>(&h);
 }
-__device__ __forceinline__ unsigned mul2(unsigned a, unsigned b) {
-  const __nv_bfloat162 h = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+__device__ __forceinline__ unsigned pack2_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const unsigned*>(&h);
+}
+__device__ __forceinline__ unsigned transposed(unsigned x) {
+  unsigned y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// a product alone, with nothing added to it
+__device__ __forceinline__ void mma_first(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ float low_half(unsigned w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float high_half(unsigned w) { return __uint_as_float(w & 0xffff0000u); }
@@ -107,6 +129,9 @@ __device__ __forceinline__ void split(float x, float y, unsigned (&t)[N]) {
     y -= high_half(t[i]);
   }
 }
+// the half `sel` names (HALF0 or HALF1) of a word, a bfloat16, as a float
+constexpr unsigned HALF0 = 0x1044, HALF1 = 0x3244;
+__device__ __forceinline__ float half_of(unsigned w, unsigned sel) { return __uint_as_float(__byte_perm(w, 0u, sel)); }
 // N words from shared memory, as wide as they come
 template <int N>
 __device__ __forceinline__ void words(unsigned (&w)[N], const unsigned char* p) {
@@ -181,21 +206,26 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
     const int kvh = item / q.row_tiles, row_tile = item - kvh * q.row_tiles;
     const int packed = q.rows * HG, pr0 = row_tile * MT;
     const int q0 = p.q_start[req];
-    // this lane's rows of the scores (r8, and r8 + 8 with two row tiles) and their positions
-    int pos[NT];
+    // this lane's rows of the scores, 8 k + 2 j and the next, and their positions
+    int pos[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) pos[n] = pr0 + n * 8 + r8 < packed ? q.pos0 + (pr0 + n * 8 + r8) / HG : -1;
+    for (int k = 0; k < NT; ++k)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int pr = pr0 + 8 * k + 2 * j + e;
+        pos[k][e] = pr < packed ? q.pos0 + pr / HG : -1;
+      }
     const int pos_min = q.pos0 + pr0 / HG, pos_max = q.pos0 + (min(pr0 + MT, packed) - 1) / HG;
     const int low_min = p.window > 0 ? pos_min - p.window + 1 : 0, low_max = p.window > 0 ? pos_max - p.window + 1 : 0;
 
-    // ---- queries: A fragments, and their sums over each group
-    unsigned qa[TERMS][G * 2][2 * NT], za[2 * NT][2];
-    float qsum[NT][G];
+    // ---- queries: B fragments (row 8 k + r8), and their sums over each group
+    unsigned qb[TERMS][G * 2][NT][2], zb[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int pr = pr0 + n * 8 + r8;
-      const bool live = pr < packed && q0 + pr / HG < p.rows && q0 >= 0;
+    for (int k = 0; k < NT; ++k) {
+      const int pr = pr0 + 8 * k + r8;
+      const bool live = pr < packed && q0 >= 0 && q0 + pr / HG < p.rows;
       const T* src = (const T*)p.q + ((size_t)(live ? q0 + pr / HG : 0) * H + kvh * HG + pr % HG) * D + 8 * j;
+      float qsum[G];
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         float x[8];
@@ -213,35 +243,37 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
           }
           x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
         }
-        qsum[n][g] = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-        qsum[n][g] += __shfl_xor_sync(0xffffffffu, qsum[n][g], 1);
-        qsum[n][g] += __shfl_xor_sync(0xffffffffu, qsum[n][g], 2);
+        qsum[g] = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+        qsum[g] += __shfl_xor_sync(0xffffffffu, qsum[g], 1);
+        qsum[g] += __shfl_xor_sync(0xffffffffu, qsum[g], 2);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {                  // pair i of the word: its codes come 16 times too large for odd i
           const float f = i & 1 ? UP / 16.f : UP;
           unsigned t[TERMS];
           split<TERMS>(x[2 * i] * f, x[2 * i + 1] * f, t);
 #pragma unroll
-          for (int e = 0; e < TERMS; ++e) qa[e][2 * g + (i >> 1)][(i & 1) * NT + n] = t[e];
+          for (int e = 0; e < TERMS; ++e) qb[e][2 * g + (i >> 1)][k][i & 1] = t[e];
         }
       }
       // three terms of the sums along the product's k: term * G + g
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int k = 2 * j + 8 * half, term = k / G, g0 = k % G;
+        const int at = 2 * j + 8 * half, term = at / G, g0 = at % G;
         float a = 0.f, b = 0.f;
 #pragma unroll
         for (int g = 0; g < G; g += 2)
-          if (g == g0) a = qsum[n][g] / CODE, b = qsum[n][g + 1] / CODE;
+          if (g == g0) a = qsum[g] / CODE, b = qsum[g + 1] / CODE;
         unsigned t[3];
         split<3>(a, b, t);
-        za[half * NT + n][0] = term == 0 ? t[0] : term == 1 ? t[1] : term == 2 ? t[2] : 0u;
+        zb[k][half] = term == 0 ? t[0] : term == 1 ? t[1] : term == 2 ? t[2] : 0u;
       }
     }
 
-    float o[NT][2 * G][4] = {}, z[NT][4] = {}, m[NT], l[NT] = {};
+    float o[NT][2 * G][4] = {}, z[NT][G][2] = {}, m[NT][2], l[NT][2] = {};
+    int e_run = -MOST_E;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) m[n] = -INFINITY;
+    for (int k = 0; k < NT; ++k) m[k][0] = m[k][1] = -INFINITY;
+    const unsigned mine_half = r8 & 1 ? HALF1 : HALF0, both_halves = r8 & 1 ? 0x7632 : 0x5410;
 
     // ---- this warp's tiles: t_begin + warp, + 8, ...
     const int mine = t_end - t_begin > warp ? (t_end - t_begin - warp + WARPS - 1) / WARPS : 0;
@@ -285,121 +317,128 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
       const int key0 = (q.first + t_begin + warp + i * WARPS) * REC_TOKENS;
       const unsigned char* num = rec + numbers(D);
 
-      // ---- scores of 16 keys: two tiles of eight
-      float s[2][2 * NT][2];                           // [key tile][.][key 2j, 2j + 1]
+      // ---- scores of keys r8 and r8 + 8
+      unsigned kw[2][G];
+      float ks[2][G], s[NT][4];                        // s: [key r8, rows 2j, 2j + 1, then key r8 + 8]
+      unsigned lo[2];
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        unsigned w[G], ks[G], lo2[2];
-        words<G>(w, rec + (n * 8 + r8) * (D / 2) + j * (4 * G));
-        words<G>(ks, num + K_S * D + (n * 4 + j) * (4 * G));
-        words<2>(lo2, num + K_LO * D + (n * 4 + (r8 >> 1)) * (4 * G) + (G == 4 ? (j & 1) * 8 : 0));
-        const unsigned lo = __byte_perm(lo2[0], lo2[1], r8 & 1 ? 0x7632 : 0x5410);
-        float acc[4] = {};
-        {
-          unsigned a[4] = {za[0][0], NT == 2 ? za[NT - 1][0] : 0u, za[NT][0], NT == 2 ? za[2 * NT - 1][0] : 0u};
-          mma(acc, a, lo, lo);
-        }
+        unsigned w[G], u[2];
+        words<G>(kw[n], rec + (n * 8 + r8) * (D / 2) + j * (4 * G));
+        words<G>(w, num + K_S * D + (n * 4 + (r8 >> 1)) * (4 * G));
+        words<2>(u, num + K_LO * D + (n * 4 + (r8 >> 1)) * (4 * G) + (G == 4 ? (j & 1) * 8 : 0));
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-          float c[4] = {};
-#pragma unroll
-          for (int e = 0; e < TERMS; ++e) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const unsigned u = h ? w[g] >> 8 : w[g];
-              const unsigned(&f)[2 * NT] = qa[e][2 * g + h];
-              unsigned a[4] = {f[0], NT == 2 ? f[NT - 1] : 0u, f[NT], NT == 2 ? f[2 * NT - 1] : 0u};
-              mma(c, a, u & 0x000f000fu, u & 0x00f000f0u);
-            }
-          }
-          const float s0 = low_half(ks[g]), s1 = high_half(ks[g]);
-          acc[0] = fmaf(s0, c[0], acc[0]);
-          acc[1] = fmaf(s1, c[1], acc[1]);
-          if (NT == 2) {
-            acc[2] = fmaf(s0, c[2], acc[2]);
-            acc[3] = fmaf(s1, c[3], acc[3]);
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < NT; ++k) s[n][k][0] = acc[2 * k] * to_log2, s[n][k][1] = acc[2 * k + 1] * to_log2;
+        for (int g = 0; g < G; ++g) ks[n][g] = half_of(w[g], mine_half);
+        lo[n] = __byte_perm(u[0], u[1], both_halves);
       }
-      // ---- masks, on the tiles that need them
-      const bool edge = key0 + REC_TOKENS - 1 > pos_min || key0 < low_max;
-      if (edge) {
+      {
+        const unsigned a[4] = {lo[0], lo[1], lo[0], lo[1]};
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int k = 0; k < NT; ++k) mma_first(s[k], a, zb[k][0], zb[k][1]);
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        float c[NT][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const unsigned x = h ? kw[0][g] >> 8 : kw[0][g], y = h ? kw[1][g] >> 8 : kw[1][g];
+          const unsigned a[4] = {x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u};
 #pragma unroll
           for (int k = 0; k < NT; ++k)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int key = key0 + n * 8 + 2 * j + e;
-              if (key > pos[k] || (p.window > 0 && key <= pos[k] - p.window)) s[n][k][e] = -INFINITY;
+            for (int e = 0; e < TERMS; ++e) {
+              const unsigned(&b)[2] = qb[e][2 * g + h][k];
+              if (h == 0 && e == 0) mma_first(c[k], a, b[0], b[1]);
+              else mma(c[k], a, b[0], b[1]);
             }
-      }
-      // ---- the running maximum, moved only when it grew by more than 2^8
-      bool grew = false;
-      float top[NT];
-#pragma unroll
-      for (int k = 0; k < NT; ++k) {
-        top[k] = fmaxf(fmaxf(s[0][k][0], s[0][k][1]), fmaxf(s[1][k][0], s[1][k][1]));
-        grew = grew || top[k] > m[k] + 8.f;
-      }
-      if (__any_sync(0xffffffffu, grew)) {
+        }
 #pragma unroll
         for (int k = 0; k < NT; ++k) {
-          top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
-          top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2));
-          const float now = fmaxf(m[k], top[k]);
-          const float a = now == -INFINITY ? 1.f : ex2(m[k] - now);
-          m[k] = now;
-          l[k] *= a;
-          const float a0 = __shfl_sync(0xffffffffu, a, 8 * j), a1 = __shfl_sync(0xffffffffu, a, 8 * j + 4);
-#pragma unroll
-          for (int c = 0; c < 2 * G; ++c) o[k][c][0] *= a0, o[k][c][1] *= a1, o[k][c][2] *= a0, o[k][c][3] *= a1;
-          z[k][0] *= a0, z[k][1] *= a1;
+          s[k][0] = fmaf(ks[0][g], c[k][0], s[k][0]);
+          s[k][1] = fmaf(ks[0][g], c[k][1], s[k][1]);
+          s[k][2] = fmaf(ks[1][g], c[k][2], s[k][2]);
+          s[k][3] = fmaf(ks[1][g], c[k][3], s[k][3]);
         }
       }
-      // ---- weights, and the values they weigh
-      unsigned vs[2][G], vlo[2];
+      // ---- the values' numbers of the same keys
+      float vs[2][G], vlo[2][G];
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        words<G>(vs[n], num + V_S * D + (n * 4 + j) * (4 * G));
-        vlo[n] = r8 < G ? *reinterpret_cast<const unsigned*>(num + V_LO * D + (n * 4 + j) * (4 * G) + r8 * 4) : 0u;
+        unsigned w[G], u[G];
+        words<G>(w, num + V_S * D + (n * 4 + (r8 >> 1)) * (4 * G));
+        words<G>(u, num + V_LO * D + (n * 4 + (r8 >> 1)) * (4 * G));
+#pragma unroll
+        for (int g = 0; g < G; ++g) vs[n][g] = half_of(w[g], mine_half), vlo[n][g] = half_of(u[g], mine_half);
       }
-      if (edge) {                                      // numbers of places that hold no key of this row tile may be anything
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const int key = key0 + n * 8 + 2 * j;
-          const unsigned keep = (key <= pos_max && key >= low_min ? 0xffffu : 0u) |
-                                (key + 1 <= pos_max && key + 1 >= low_min ? 0xffff0000u : 0u);
-          vlo[n] &= keep;
-#pragma unroll
-          for (int g = 0; g < G; ++g) vs[n][g] &= keep;
-        }
-      }
-      float w[2][NT][2];
-#pragma unroll
-      for (int k = 0; k < NT; ++k) {
-        const float off = m[k] == -INFINITY ? 0.f : 64.f - m[k];
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) w[n][k][e] = TERMS == 1 ? ex2(s[n][k][e] + off) : exp2f(s[n][k][e] + off);
-          l[k] += w[n][k][0] + w[n][k][1];
-        }
-      }
-      unsigned wp[NT][2][TERMS];
 #pragma unroll
       for (int k = 0; k < NT; ++k)
 #pragma unroll
-        for (int n = 0; n < 2; ++n) split<TERMS>(w[n][k][0], w[n][k][1], wp[k][n]);
-      {
-        const unsigned a[4] = {vlo[0], 0u, vlo[1], 0u};
+        for (int e = 0; e < 4; ++e) s[k][e] *= to_log2;
+      // ---- masks, on the tiles that need them
+      if (key0 + REC_TOKENS - 1 > pos_min || key0 < low_max) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const int key = key0 + n * 8 + r8;
+#pragma unroll
+          for (int k = 0; k < NT; ++k)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (key > pos[k][e] || (p.window > 0 && key <= pos[k][e] - p.window)) s[k][2 * n + e] = -INFINITY;
+          if (key > pos_max || key < low_min) {        // numbers of places that hold no key of this row tile may be anything
+#pragma unroll
+            for (int g = 0; g < G; ++g) vs[n][g] = vlo[n][g] = 0.f;
+          }
+        }
+      }
+      // ---- the running maximum, moved only when it grew by more than 2^8, or with it the largest exponent of the values' s
+      bool grew = false;
+#pragma unroll
+      for (int k = 0; k < NT; ++k)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) grew = grew || fmaxf(s[k][e], s[k][2 + e]) > m[k][e] + 8.f;
+      unsigned large = 0;
+      if constexpr (TERMS == 1) {
+        float most = 0.f;
+#pragma unroll
+        for (int g = 0; g < G; ++g) most = fmaxf(most, fmaxf(vs[0][g], vs[1][g]));
+        large = __float_as_uint(most) >> 23;
+        grew = grew || (int)large - 127 > e_run;
+      }
+      if (__any_sync(0xffffffffu, grew)) {
+        int e_now = e_run;
+        if constexpr (TERMS == 1) e_now = max(e_run, min((int)__reduce_max_sync(0xffffffffu, large) - 127, MOST_E));
 #pragma unroll
         for (int k = 0; k < NT; ++k)
 #pragma unroll
-          for (int e = 0; e < TERMS; ++e) mma(z[k], a, wp[k][0][e], wp[k][1][e]);
+          for (int e = 0; e < 2; ++e) {
+            float top = fmaxf(s[k][e], s[k][2 + e]);
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            top = fmaxf(top, m[k][e]);
+            const float a = top == -INFINITY ? 1.f : ex2(m[k][e] - top + (float)(e_run - e_now));
+            m[k][e] = top;
+            l[k][e] *= a;
+#pragma unroll
+            for (int c = 0; c < 2 * G; ++c) o[k][c][e] *= a, o[k][c][2 + e] *= a;
+#pragma unroll
+            for (int g = 0; g < G; ++g) z[k][g][e] *= a;
+          }
+        e_run = e_now;
       }
+      // ---- weights, and the values' lo that they weigh
+      float w[NT][4];
+#pragma unroll
+      for (int k = 0; k < NT; ++k)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float off = m[k][e] == -INFINITY ? 0.f : (TERMS == 1 ? (float)(ROOM - e_run) : 0.f) - m[k][e];
+#pragma unroll
+          for (int n = 0; n < 2; ++n) w[k][2 * n + e] = TERMS == 1 ? ex2(s[k][2 * n + e] + off) : exp2f(s[k][2 * n + e] + off) * UP;
+          l[k][e] += w[k][e] + w[k][2 + e];
+#pragma unroll
+          for (int g = 0; g < G; ++g) z[k][g][e] = fmaf(w[k][e], vlo[0][g], fmaf(w[k][2 + e], vlo[1][g], z[k][g][e]));
+        }
+      // ---- the codes that they weigh
       unsigned v0[G], v1[G];
       words<G>(v0, rec + v_codes(D) + j * D + r8 * (4 * G));
       words<G>(v1, rec + v_codes(D) + (j + 4) * D + r8 * (4 * G));
@@ -410,8 +449,11 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
         for (int k = 0; k < NT; ++k)
 #pragma unroll
           for (int n = 0; n < 2; ++n) {
-            if constexpr (TERMS == 1) b[k][n][0] = mul2(wp[k][n][0], vs[n][g]);     // rounded once more, as the weight was
-            else split<TERMS>(w[n][k][0] * low_half(vs[n][g]), w[n][k][1] * high_half(vs[n][g]), b[k][n]);
+            const float x = w[k][2 * n] * vs[n][g], y = w[k][2 * n + 1] * vs[n][g];
+            if constexpr (TERMS == 1) b[k][n][0] = pack2_f16(x, y);
+            else split<TERMS>(x, y, b[k][n]);
+#pragma unroll
+            for (int e = 0; e < TERMS; ++e) b[k][n][e] = transposed(b[k][n][e]);
           }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -420,7 +462,10 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
 #pragma unroll
           for (int k = 0; k < NT; ++k)
 #pragma unroll
-            for (int e = 0; e < TERMS; ++e) mma(o[k][2 * g + h], a, b[k][0][e], b[k][1][e]);
+            for (int e = 0; e < TERMS; ++e) {
+              if constexpr (TERMS == 1) mma_f16(o[k][2 * g + h], a, b[k][0][e], b[k][1][e]);
+              else mma(o[k][2 * g + h], a, b[k][0][e], b[k][1][e]);
+            }
         }
       }
     }
@@ -431,23 +476,28 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
     float* om = reinterpret_cast<float*>(smem);        // [warp][row][D]
     float* mm = om + WARPS * MT * D;                   // [warp][row]
     float* lm = mm + WARPS * MT;
+    constexpr float even = TERMS == 1 ? CODE16 : CODE, odd = even / 16.f, down = TERMS == 1 ? 1.f : 1.f / UP;
 #pragma unroll
     for (int k = 0; k < NT; ++k) {
-      l[k] += __shfl_xor_sync(0xffffffffu, l[k], 1);
-      l[k] += __shfl_xor_sync(0xffffffffu, l[k], 2);
-      if (j == 0) {
-        mm[warp * MT + k * 8 + r8] = m[k];
-        lm[warp * MT + k * 8 + r8] = l[k] * (1.f / UP);
-      }
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const float z0 = __shfl_sync(0xffffffffu, z[k][0], g * 4 + j) * (1.f / UP);
-        const float z1 = __shfl_sync(0xffffffffu, z[k][1], g * 4 + j) * (1.f / UP);
-        const float(&a)[4] = o[k][2 * g], (&b)[4] = o[k][2 * g + 1];
-        constexpr float odd = CODE / 16.f;
-        float* dst = om + (warp * MT + k * 8 + 2 * j) * D + 32 * g + 4 * r8;
-        *reinterpret_cast<float4*>(dst) = make_float4(fmaf(a[0], CODE, z0), fmaf(a[2], odd, z0), fmaf(b[0], CODE, z0), fmaf(b[2], odd, z0));
-        *reinterpret_cast<float4*>(dst + D) = make_float4(fmaf(a[1], CODE, z1), fmaf(a[3], odd, z1), fmaf(b[1], CODE, z1), fmaf(b[3], odd, z1));
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) {
+          l[k][e] += __shfl_xor_sync(0xffffffffu, l[k][e], off);
+#pragma unroll
+          for (int g = 0; g < G; ++g) z[k][g][e] += __shfl_xor_sync(0xffffffffu, z[k][g][e], off);
+        }
+        const int row = warp * MT + 8 * k + 2 * j + e;
+        if (r8 == 0) {
+          mm[row] = TERMS == 1 ? m[k][e] + (float)(e_run - ROOM) : m[k][e];
+          lm[row] = l[k][e] * down;
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const float(&a)[4] = o[k][2 * g], (&b)[4] = o[k][2 * g + 1], lean = z[k][g][e] * down;
+          *reinterpret_cast<float4*>(om + row * D + 32 * g + 4 * r8) =
+              make_float4(fmaf(a[e], even, lean), fmaf(a[2 + e], odd, lean), fmaf(b[e], even, lean), fmaf(b[2 + e], odd, lean));
+        }
       }
     }
     __syncthreads();
