@@ -65,17 +65,16 @@ constexpr int MOST_E = 60;
 struct Request {
   int rows, seq, pos0, first, tiles, row_tiles;        // first: the first 16-key tile, tiles: how many, at least one
 };
-__device__ __forceinline__ Request request(const Kv4AttnParams& p, const Split& s, int r, int tile_rows) {
+__device__ __forceinline__ Request request(const Kv4AttnParams& p, const Split& s, int rows, int seq, int tile_rows) {
   Request q;
-  q.rows = max(0, p.q_len[r]);
-  q.seq = max(0, p.seq_len[r]);
+  q.rows = max(0, rows);
+  q.seq = max(0, seq);
   q.pos0 = q.seq - q.rows;
-  const int G = p.heads / p.kv_heads;
-  const long long packed = (long long)q.rows * G;
-  q.row_tiles = packed > s.most_packed ? 0 : (int)((packed + tile_rows - 1) / tile_rows);
+  const long long packed = (long long)q.rows * (p.heads / p.kv_heads);
+  q.row_tiles = packed > s.most_packed ? 0 : (int)((packed + tile_rows - 1) / tile_rows);      // tile_rows: 8 or 16
   const int low = p.window > 0 ? max(0, q.pos0 - p.window + 1) : 0;
   q.first = low / REC_TOKENS;
-  q.tiles = max(1, (int)(((long long)q.seq + REC_TOKENS - 1) / REC_TOKENS) - q.first);
+  q.tiles = max(1, (int)(((unsigned)q.seq + REC_TOKENS - 1) / REC_TOKENS) - q.first);
   return q;
 }
 // the first request whose units end behind `unit`
@@ -86,6 +85,10 @@ __device__ __forceinline__ int find(const long long* ends, int requests, long lo
     if (ends[mid] > unit) hi = mid; else lo = mid + 1;
   }
   return lo;
+}
+// a / b, a not negative: almost always in 32 bits, where a division is a tenth of one in 64
+__device__ __forceinline__ long long quotient(long long a, int b) {
+  return a >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b);
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -157,6 +160,7 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
   __shared__ long long warp_sums[WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r8 = lane >> 2, j = lane & 3;
   const int H = p.heads, KV = p.kv_heads, HG = H / KV, per_page = p.page_tokens / REC_TOKENS;
+  const int page_shift = (per_page & (per_page - 1)) == 0 ? 31 - __clz(per_page) : -1;
   pdl_wait();
 
   // where each request's units end (a unit: one tile of 16 keys for one head and row tile)
@@ -165,7 +169,7 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
     const int r = r0 + threadIdx.x;
     long long v = 0;
     if (r < p.requests) {
-      const Request q = request(p, sp, r, MT);
+      const Request q = request(p, sp, p.q_len[r], p.seq_len[r], MT);
       v = (long long)q.tiles * q.row_tiles * KV;
     }
 #pragma unroll
@@ -184,7 +188,7 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
     if (r < p.requests) ends[r] = before + v;
     __syncthreads();
   }
-  const long long per_block = max((long long)MIN_UNITS, (total + gridDim.x - 1) / gridDim.x);
+  const long long per_block = max((long long)MIN_UNITS, quotient(total + gridDim.x - 1, gridDim.x));
   if (blockIdx.x == 0) {
     for (int r = threadIdx.x; r < p.requests; r += WARPS * 32) sp.ends[1 + r] = ends[r];
     if (threadIdx.x == 0) sp.ends[0] = per_block;
@@ -198,14 +202,49 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
   while (unit < unit_end) {
     // ---- the next item, or this block's part of it
     const int req = find(ends, p.requests, unit);
-    const Request q = request(p, sp, req, MT);
+    const Request q = request(p, sp, p.q_len[req], p.seq_len[req], MT);
     const long long begin = req > 0 ? ends[req - 1] : 0;
-    const int item = (int)((unit - begin) / q.tiles);
+    const int item = (int)quotient(unit - begin, q.tiles);
     const int t_begin = (int)((unit - begin) - (long long)item * q.tiles);
     const int t_end = (int)min((long long)q.tiles, t_begin + (unit_end - unit));
-    const int kvh = item / q.row_tiles, row_tile = item - kvh * q.row_tiles;
+    const int kvh = q.row_tiles == 1 ? item : item / q.row_tiles, row_tile = item - kvh * q.row_tiles;
     const int packed = q.rows * HG, pr0 = row_tile * MT;
     const int q0 = p.q_start[req];
+    auto row_of = [&](int pr) { return q.rows == 1 ? 0 : pr / HG; };     // the request's row of a packed one
+    const int pos_min = q.pos0 + row_of(pr0), pos_max = q.pos0 + row_of(min(pr0 + MT, packed) - 1);
+    const int low_min = p.window > 0 ? pos_min - p.window + 1 : 0, low_max = p.window > 0 ? pos_max - p.window + 1 : 0;
+
+    // ---- this warp's tiles, t_begin + warp, + 8, ...: the first are on their way before the queries are looked at
+    const int mine = t_end - t_begin > warp ? (t_end - t_begin - warp + WARPS - 1) / WARPS : 0;
+    const int32_t* table = p.block_table + (long long)req * p.bt_stride;
+    auto record = [&](int i) {                         // the record of this warp's tile i, -1: none to be seen
+      if (i >= mine) return -1;
+      const int t = q.first + t_begin + warp + i * WARPS, blk = page_shift >= 0 ? t >> page_shift : t / per_page;
+      if (blk >= p.table_pages || t * REC_TOKENS > pos_max || t * REC_TOKENS + REC_TOKENS <= low_min) return -1;
+      const int page = table[blk];
+      return page >= 0 && page < p.num_pages ? (page * KV + kvh) * per_page + (t - blk * per_page) : -1;
+    };
+    int recs = record(lane), recs_next = record(32 + lane);
+    unsigned there = 0;                                // bit i: the tile issued i tiles ago has a record
+    auto issue = [&](int i) {
+      if (i > 0 && (i & 31) == 0) {
+        recs = recs_next;
+        recs_next = record(i + 32 + lane);
+      }
+      const int rec = __shfl_sync(0xffffffffu, recs, i & 31);
+      there = there << 1 | (rec >= 0 ? 1u : 0u);
+      if (rec >= 0) {
+        const unsigned char* src = p.pages + (long long)rec * REC + lane * 16;
+        unsigned char* dst = ring + (i % STAGES) * REC + lane * 16;
+#pragma unroll
+        for (int c = 0; c < (REC + 511) / 512; ++c)
+          if (REC % 512 == 0 || c * 512 + lane * 16 < REC) cp16(dst + c * 512, src + c * 512, true);
+      }
+      cp_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) issue(i);
+
     // this lane's rows of the scores, 8 k + 2 j and the next, and their positions
     int pos[NT][2];
 #pragma unroll
@@ -213,18 +252,16 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int pr = pr0 + 8 * k + 2 * j + e;
-        pos[k][e] = pr < packed ? q.pos0 + pr / HG : -1;
+        pos[k][e] = pr < packed ? q.pos0 + row_of(pr) : -1;
       }
-    const int pos_min = q.pos0 + pr0 / HG, pos_max = q.pos0 + (min(pr0 + MT, packed) - 1) / HG;
-    const int low_min = p.window > 0 ? pos_min - p.window + 1 : 0, low_max = p.window > 0 ? pos_max - p.window + 1 : 0;
-
     // ---- queries: B fragments (row 8 k + r8), and their sums over each group
     unsigned qb[TERMS][G * 2][NT][2], zb[NT][2];
 #pragma unroll
     for (int k = 0; k < NT; ++k) {
       const int pr = pr0 + 8 * k + r8;
-      const bool live = pr < packed && q0 >= 0 && q0 + pr / HG < p.rows;
-      const T* src = (const T*)p.q + ((size_t)(live ? q0 + pr / HG : 0) * H + kvh * HG + pr % HG) * D + 8 * j;
+      const int row = row_of(pr);
+      const bool live = pr < packed && q0 >= 0 && q0 + row < p.rows;
+      const T* src = (const T*)p.q + (live ? ((size_t)(q0 + row) * H + kvh * HG + (pr - row * HG)) * D + 8 * j : 0);
       float qsum[G];
 #pragma unroll
       for (int g = 0; g < G; ++g) {
@@ -275,38 +312,6 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
     for (int k = 0; k < NT; ++k) m[k][0] = m[k][1] = -INFINITY;
     const unsigned mine_half = r8 & 1 ? HALF1 : HALF0, both_halves = r8 & 1 ? 0x7632 : 0x5410;
 
-    // ---- this warp's tiles: t_begin + warp, + 8, ...
-    const int mine = t_end - t_begin > warp ? (t_end - t_begin - warp + WARPS - 1) / WARPS : 0;
-    const int32_t* table = p.block_table + (long long)req * p.bt_stride;
-    auto record = [&](int i) {                         // the record of this warp's tile i, -1: none to be seen
-      if (i >= mine) return -1;
-      const int t = q.first + t_begin + warp + i * WARPS, blk = t / per_page;
-      if (blk >= p.table_pages || t * REC_TOKENS > pos_max || t * REC_TOKENS + REC_TOKENS <= low_min) return -1;
-      const int page = table[blk];
-      return page >= 0 && page < p.num_pages ? (page * KV + kvh) * per_page + (t - blk * per_page) : -1;
-    };
-    int recs = record(lane), recs_next = record(32 + lane);
-    unsigned there = 0;                                // bit i: the tile issued i tiles ago has a record
-    auto issue = [&](int i) {
-      if (i > 0 && (i & 31) == 0) {
-        recs = recs_next;
-        recs_next = record(i + 32 + lane);
-      }
-      const int rec = __shfl_sync(0xffffffffu, recs, i & 31);
-      there = there << 1 | (rec >= 0 ? 1u : 0u);
-      if (rec >= 0) {
-        const unsigned char* src = p.pages + (long long)rec * REC;
-        unsigned char* dst = ring + (i % STAGES) * REC;
-#pragma unroll
-        for (int c = 0; c < (REC + 511) / 512; ++c) {
-          const int at = (c * 32 + lane) * 16;
-          if (REC % 512 == 0 || at < REC) cp16(dst + at, src + at, true);
-        }
-      }
-      cp_commit();
-    };
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) issue(i);
     for (int i = 0; i < mine; ++i) {
       cp_wait<STAGES - 2>();
       __syncwarp();                                    // the tile has landed, and the one before is read
@@ -522,9 +527,9 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
         const size_t at = (size_t)slot * MT + row;
         *reinterpret_cast<float4*>(sp.part_o + at * D + c4) = x;
         if (c4 == 0) sp.part_ml[at * 2] = top, sp.part_ml[at * 2 + 1] = sum;
-      } else if (pr < packed && q0 >= 0 && q0 + pr / HG < p.rows) {
+      } else if (const int at = row_of(pr); pr < packed && q0 >= 0 && q0 + at < p.rows) {
         const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;      // a row whose scores are NaN stays NaN
-        T* dst = (T*)p.out + ((size_t)(q0 + pr / HG) * H + kvh * HG + pr % HG) * D + c4;
+        T* dst = (T*)p.out + ((size_t)(q0 + at) * H + kvh * HG + (pr - at * HG)) * D + c4;
         if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(x.x * inv, x.y * inv), pack2(x.z * inv, x.w * inv));
         else *reinterpret_cast<float4*>(dst) = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
       }
@@ -535,9 +540,14 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
 }
 
 // Items that several blocks share: block b looks at the border between blocks b and b + 1 of the kernel above, and merges the
-// item that lies across it if that is the item's first border.
+// item that lies across it if that is the item's first border.  A warp takes one row and every PARTS-th of the item's parts
+// (one request of 32,768 keys has 74, whose loads one warp a row would wait for in turn: 53 us), eight loads on their way.
+constexpr int MERGE_WARPS = 16;
+
 template <typename T, int D, int MT>
-__global__ void __launch_bounds__(256) kv4_merge_kernel(Kv4AttnParams p, Split sp) {
+__global__ void __launch_bounds__(MERGE_WARPS * 32) kv4_merge_kernel(Kv4AttnParams p, Split sp) {
+  constexpr int PARTS = MERGE_WARPS / MT, C = D / 32;  // C: columns a lane
+  __shared__ float held[PARTS > 1 ? PARTS : 1][MT][D], held_m[MERGE_WARPS], held_l[MERGE_WARPS];
   pdl_launch_dependents();
   pdl_wait();
   const long long per_block = sp.ends[0];
@@ -545,34 +555,70 @@ __global__ void __launch_bounds__(256) kv4_merge_kernel(Kv4AttnParams p, Split s
   const long long border = per_block * (blockIdx.x + 1);
   if (border >= ends[p.requests - 1]) return;
   const int req = find(ends, p.requests, border);
-  const Request q = request(p, sp, req, MT);
+  const Request q = request(p, sp, p.q_len[req], p.seq_len[req], MT);
   const long long begin = req > 0 ? ends[req - 1] : 0;
-  const int item = (int)((border - begin) / q.tiles);
+  const int item = (int)quotient(border - begin, q.tiles);
   const long long first = begin + (long long)item * q.tiles, last = first + q.tiles;
   if (first == border || first < border - per_block) return;
   const int H = p.heads, KV = p.kv_heads, HG = H / KV, kvh = item / q.row_tiles, row_tile = item - kvh * q.row_tiles;
   const int q0 = p.q_start[req], packed = q.rows * HG;
   const int b0 = blockIdx.x, b1 = (int)((last - 1) / per_block);
-  auto slot = [&](int b) { return 2 * b + (per_block * b >= first ? 0 : 1); };
-  for (int e = threadIdx.x; e < MT * (D / 4); e += 256) {
-    const int row = e / (D / 4), c4 = (e % (D / 4)) * 4, pr = row_tile * MT + row;
-    if (pr >= packed || q0 < 0 || q0 + pr / HG >= p.rows) continue;
-    float top = -INFINITY;
-    for (int b = b0; b <= b1; ++b) top = fmaxf(top, sp.part_ml[((size_t)slot(b) * MT + row) * 2]);
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int b = b0; b <= b1; ++b) {
-      const size_t at = (size_t)slot(b) * MT + row;
-      const float f = exp2f(sp.part_ml[at * 2] - base);
-      const float4 y = *reinterpret_cast<const float4*>(sp.part_o + at * D + c4);
-      sum = fmaf(f, sp.part_ml[at * 2 + 1], sum);
-      x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = warp % MT, part = warp / MT;
+  // a block's first segment is in its slot 0: every block's but perhaps the first one's
+  const int slot0 = 2 * b0 + (per_block * b0 >= first ? 0 : 1);
+  auto slot = [&](int b) { return (size_t)(b == b0 ? slot0 : 2 * b) * MT + row; };
+  float top = -INFINITY, sum = 0.f, x[C] = {};
+  for (int b = b0 + part; b <= b1; b += PARTS * 32) {              // 32 of the warp's parts at a time
+    const int n = min(32, (b1 - b) / PARTS + 1);
+    const float m = lane < n ? sp.part_ml[slot(b + lane * PARTS) * 2] : -INFINITY;
+    const float l = lane < n ? sp.part_ml[slot(b + lane * PARTS) * 2 + 1] : 0.f;
+    const float now = fmaxf(top, warp_max(m)), base = now == -INFINITY ? 0.f : now;
+    const float old = exp2f(top - base), f = exp2f(m - base);
+    top = now;
+    sum = fmaf(sum, old, warp_sum(f * l));
+#pragma unroll
+    for (int c = 0; c < C; ++c) x[c] *= old;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      const float w = __shfl_sync(0xffffffffu, f, i);
+      const float* src = sp.part_o + slot(b + i * PARTS) * D + C * lane;
+#pragma unroll
+      for (int c = 0; c < C; c += 2) {
+        const float2 y = *reinterpret_cast<const float2*>(src + c);
+        x[c] = fmaf(w, y.x, x[c]);
+        x[c + 1] = fmaf(w, y.y, x[c + 1]);
+      }
     }
-    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-    T* dst = (T*)p.out + ((size_t)(q0 + pr / HG) * H + kvh * HG + pr % HG) * D + c4;
-    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(x.x * inv, x.y * inv), pack2(x.z * inv, x.w * inv));
-    else *reinterpret_cast<float4*>(dst) = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+  }
+  if (PARTS > 1) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) held[part][row][C * lane + c] = x[c];
+    if (lane == 0) held_m[warp] = top, held_l[warp] = sum;
+    __syncthreads();
+    if (part > 0) return;
+    float most = top;
+#pragma unroll
+    for (int o = 1; o < PARTS; ++o) most = fmaxf(most, held_m[o * MT + row]);
+    const float base = most == -INFINITY ? 0.f : most, own = exp2f(top - base);
+    sum *= own;
+#pragma unroll
+    for (int c = 0; c < C; ++c) x[c] *= own;
+#pragma unroll
+    for (int o = 1; o < PARTS; ++o) {
+      const float f = exp2f(held_m[o * MT + row] - base);
+      sum = fmaf(f, held_l[o * MT + row], sum);
+#pragma unroll
+      for (int c = 0; c < C; ++c) x[c] = fmaf(f, held[o][row][C * lane + c], x[c]);
+    }
+  }
+  const int pr = row_tile * MT + row, at = q.rows == 1 ? 0 : pr / HG;
+  if (pr >= packed || q0 < 0 || q0 + at >= p.rows) return;
+  const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+  T* dst = (T*)p.out + ((size_t)(q0 + at) * H + kvh * HG + (pr - at * HG)) * D + C * lane;
+#pragma unroll
+  for (int c = 0; c < C; c += 2) {
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<unsigned*>(dst + c) = pack2(x[c] * inv, x[c + 1] * inv);
+    else *reinterpret_cast<float2*>(dst + c) = make_float2(x[c] * inv, x[c + 1] * inv);
   }
 }
 
@@ -583,7 +629,7 @@ int launch(const Kv4AttnParams& p, const Split& sp, int blocks, cudaStream_t str
   static OptIn opt_in;
   if (const cudaError_t e = opt_in(smem, kv4_attention_kernel<T, D, NT, TERMS>)) return (int)e;
   launch_k(kv4_attention_kernel<T, D, NT, TERMS>, blocks, WARPS * 32, smem, stream, p, sp);
-  if (blocks > 1) launch_k(kv4_merge_kernel<T, D, MT>, blocks - 1, 256, 0, stream, p, sp);
+  if (blocks > 1) launch_k(kv4_merge_kernel<T, D, MT>, blocks - 1, MERGE_WARPS * 32, 0, stream, p, sp);
   return launch_status();
 }
 
