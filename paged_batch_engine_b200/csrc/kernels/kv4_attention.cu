@@ -24,6 +24,7 @@
 
 #include "common.cuh"
 #include "kv4.cuh"
+#include "kv4_params.cuh"
 #include "mma_sync.cuh"
 #include "opt_in.cuh"
 #include "pdl.cuh"
@@ -33,18 +34,6 @@ using namespace pbe::kv4;
 using namespace pbe::mma_sync;
 
 namespace {
-struct Kv4AttnParams {
-  const void* q;
-  const unsigned char* pages;
-  void* out;
-  const int32_t* q_start;
-  const int32_t* q_len;
-  const int32_t* seq_len;
-  const int32_t* block_table;
-  long long bt_stride;
-  int table_pages, num_pages, requests, rows, heads, kv_heads, page_tokens, window;
-  float scale;
-};
 struct Split {
   float* part_o;               // [2 blocks][rows of a tile][D]
   float* part_ml;              // [2 blocks][rows of a tile][2]

@@ -2861,6 +2861,9 @@ class Kv4AttnParams(ctypes.Structure):
 
 
 KV4_MAX_REQUESTS = 8192
+KV4_FEW_PACKED = 64         # packed rows (rows x heads of a key/value head) up to which a request is the mma.sync kernel's
+KV4_SPLIT_KEYS = 512        # keys of a split of the tcgen05 kernel at least
+KV4_MOST_SPLITS = 32
 KV4_UNITS = 16              # tiles of 16 keys a block takes at least, two a warp
 
 
@@ -2878,7 +2881,7 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, q_sta
                   seq_len: torch.Tensor, block_table: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int,
                   scale: float, window: Optional[int], page_tokens: int, most_rows: int, most_keys: int) -> torch.Tensor:
     """Causal attention of every row over 4-bit pages, ``paged_attention`` for a cache in four bits: row i of request r (row
-    ``q_start[r] + i`` of q and out, both [T, H * head_dim]) sees the request's first ``seq_len[r] - q_len[r] + i + 1`` keys, or the last ``window`` of
+    ``q_start[r] + i`` of q and out, both [T, H * head_dim], no row of two requests) sees the request's first ``seq_len[r] - q_len[r] + i + 1`` keys, or the last ``window`` of
     them, at ``block_table[r]`` (int32 [R, width], rows may be strided).  A row that sees no key is 0; rows of no request are left as
     they are.  A key whose block-table entry is no page, or lies behind the table, is not seen.  ``most_rows`` and ``most_keys`` are the
     largest of q_len and seq_len as far as the host knows them: they choose the shape of the launch, not the result."""
@@ -2908,9 +2911,26 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, q_sta
         seq_len=seq_len.data_ptr(), block_table=block_table.data_ptr(), bt_stride=block_table.stride(0),
         table_pages=block_table.shape[1], num_pages=pages.shape[0], requests=R, rows=q.shape[0], heads=H, kv_heads=KV,
         page_tokens=page_tokens, window=int(window or 0), scale=float(scale))
-    tile_rows, blocks = _kv4_shape(R, H, KV, head_dim, most_rows, most_keys, q.dtype == torch.bfloat16, multiprocessors(q.device))
-    floats = (2 * (1 + R) + 3) // 4 * 4 + 2 * blocks * tile_rows * (head_dim + 2)
-    work = torch.empty(floats, dtype=torch.float32, device=q.device)
-    fn = _fn("kv4_attention", "pbe_kv4_attention", [ctypes.POINTER(Kv4AttnParams), c_void_p] + [c_int] * 5 + [c_void_p])
-    _check(fn(ctypes.byref(p), _ptr(work), blocks, head_dim, tile_rows, 0x7fffffff, dtype, _stream()), "kv4_attention")
+    bf16, group, T = q.dtype == torch.bfloat16, H // KV, q.shape[0]
+    # requests of many packed rows go to the tcgen05 kernel, where the hint says that there may be some (a request alone in
+    # its step then goes there whatever its rows); both kernels read from the lengths on the device which are theirs
+    most_packed = 0x7fffffff
+    if bf16 and scale > 0 and most_rows * group > KV4_FEW_PACKED:
+        most_packed = 0 if R == 1 else KV4_FEW_PACKED
+    params, stream = ctypes.byref(p), _stream()
+    if most_packed:
+        rows = min(most_rows, max(1, most_packed // group))
+        tile_rows, blocks = _kv4_shape(R, H, KV, head_dim, rows, most_keys, bf16, multiprocessors(q.device))
+        floats = (2 * (1 + R) + 3) // 4 * 4 + 2 * blocks * tile_rows * (head_dim + 2)
+        work = torch.empty(floats, dtype=torch.float32, device=q.device)
+        fn = _fn("kv4_attention", "pbe_kv4_attention", [ctypes.POINTER(Kv4AttnParams), c_void_p] + [c_int] * 5 + [c_void_p])
+        _check(fn(params, _ptr(work), blocks, head_dim, tile_rows, most_packed, dtype, stream), "kv4_attention")
+    if most_packed != 0x7fffffff:
+        # row tiles of 128: at most one of each request is not full
+        tiles = T * group // 128 + min(R, T * group // (most_packed + 1))
+        splits = max(1, min(2 * multiprocessors(q.device) // (tiles * KV), -(-most_keys // KV4_SPLIT_KEYS), KV4_MOST_SPLITS))
+        work = torch.empty(tiles * KV * splits * 128 * (head_dim + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
+        fn = _fn("kv4_attention_tc5", "pbe_kv4_attention_tc5", [ctypes.POINTER(Kv4AttnParams), c_void_p] + [c_int] * 4 + [c_void_p] * 2)
+        _check(fn(params, _ptr(work), tiles, splits, head_dim, most_packed, _ptr(tc5_attention_error_buffer(q.device)), stream),
+               "kv4_attention (tcgen05)")
     return out
