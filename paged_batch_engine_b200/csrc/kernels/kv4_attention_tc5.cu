@@ -1,25 +1,27 @@
 // Causal attention over 4-bit pages (kv4.cuh) for prompt portions, on the fifth-generation tensor cores.
 //
-// One block owns a row tile of 128 packed rows (query row x head of the group) of one key/value head and walks over its keys in
-// tiles of 64, four records:
-//   S = Q K^T     tcgen05.mma, 128 x 64 x D, into two alternating score buffers in tensor memory;
-//   softmax       warps 0-3, one thread a row: tcgen05.ld, maximum, exponentials, sum; the running maximum moves only after it
-//                 grew by 2^8, so the output accumulator is rarely rescaled;
+// One block owns a row tile of 256 packed rows (query row x head of the group) of one key/value head, two halves of 128, and
+// walks over its keys in tiles of 64, four records, which both halves read once they are operands:
+//   S = Q K^T     tcgen05.mma, 128 x 64 x D, into two alternating score buffers in tensor memory for each half;
+//   softmax       warps 0-3 and 4-7, one thread a row: tcgen05.ld, maximum, exponentials, sum; the running maximum moves only
+//                 after it grew by 2^8, so the output accumulator is rarely rescaled, and only then waited for;
 //   O += P V      P goes back into the columns of its scores and is the A operand from tensor memory.
-// Warps 4-7 turn records into operands, a record of each tile a warp: words are loaded a tile ahead into registers, and
-// lo + s * code is one float16 multiply-add a pair of channels, since a code in the low bits of a float16 is already a number
-// (code * 2^-24).  Keys become 64 rows of D channels, values D rows of 64 keys (their words hold pairs of keys, so that is
-// how they lie), both K-major under the 128-byte swizzle; the rows of the values are ordered (group, i, r), so that eight
-// lanes write eight different banks, and the epilogue puts the channels back in order.  Warp 8 issues the products.
+// Warps 8-14 turn records into operands, record after record in turn: a record's words are loaded into registers while the
+// one before is converted, and lo + s * code is one float16 multiply-add a pair of channels, since a code in the low bits of
+// a float16 is already a number (code * 2^-24).  Keys become 64 rows of D channels, values D rows of 64 keys (their words
+// hold pairs of keys, so that is how they lie), both K-major under the 128-byte swizzle, three tiles of each in flight; the
+// rows of the values are ordered (group, i, r), so that eight lanes write eight different banks, and the epilogue puts the
+// channels back in order.  Warp 15 issues the products.  (With one half a block and two blocks a multiprocessor each record
+// was converted twice as often, and four converting warps were what the rest waited for: 4,096 tokens 269 us.)
 //
 // All operands are float16, with sums in float32: eleven bits where bfloat16 keeps eight, so the rounding of keys, values and
 // weights stays below the output's.  Ranges are kept by exponents: a row's queries, and a record's keys and values, are scaled
 // by powers of two that the softmax takes out again (keys in the factor before the exponential, values as an offset within
 // it, with a running reference for the output's unit).  Spans of keys and values from 2^-60 to 2^60 are held.
 //
-// Two blocks share a multiprocessor (256 columns of tensor memory and 100 KB each).  Few row tiles with many keys are split
-// along the keys and merged by a second kernel.  Every mbarrier wait is bounded; one that runs out sets *err, and the roles run
-// to their end.
+// A block takes all of tensor memory (two halves of two score buffers of 64 columns and an output of up to 128).  Few row
+// tiles with many keys are split along the keys and merged by a second kernel.  Every mbarrier wait is bounded; one that runs
+// out sets *err, and the roles run to their end.
 #include <cuda.h>
 #include <cuda_fp16.h>
 
@@ -35,17 +37,20 @@ using namespace pbe::kv4;
 using namespace pbe::tc5;
 
 namespace {
-constexpr int BM = 128, BN = 64;        // packed rows of a block, keys of a tile
-constexpr int RECS = BN / REC_TOKENS;   // records of a tile, one a dequantising warp
-constexpr int THREADS = 288;
-constexpr int TMEM_COLS = 256;
-constexpr int S_COL = 0, O_COL = 128;
+constexpr int HALF = 128, BM = 2 * HALF, BN = 64;     // packed rows of a block, keys of a tile
+constexpr int RECS = BN / REC_TOKENS;   // records of a tile
+constexpr int SOFT = 8, CONV = 7, MMA_WARP = SOFT + CONV;
+constexpr int THREADS = 32 * (MMA_WARP + 1);
+constexpr int STAGES = 3;               // tiles of keys and of values that are operands
+constexpr int UNITS = 8;                // tiles whose records' exponents are kept
+constexpr int TMEM_COLS = 512;
+constexpr int S_COL = 0, O_COL = 256;   // of half h: two score buffers at 128 h, the output at 256 + 128 h
 constexpr int ROOM = 6;                 // weights are kept 2^6 times too large: float16 reaches further down
 constexpr int MOST_E = 60;
 
 struct Tc5Split {
-  float* part_o;               // [tiles * KV * splits][128][D]
-  float* part_ml;              // [tiles * KV * splits][128][2]: maximum (log2), sum
+  float* part_o;               // [tiles * KV * splits][256][D]
+  float* part_ml;              // [tiles * KV * splits][256][2]: maximum (log2), sum
   int most_packed;             // requests of at most as many packed rows are another kernel's
   int splits;
 };
@@ -118,20 +123,35 @@ __device__ __forceinline__ Tile tile_of(const Kv4AttnParams& p, int most_packed,
   return {-1, 0, target};
 }
 
+// N words from shared memory, as wide as they come
+template <int N>
+__device__ __forceinline__ void words(unsigned (&w)[N], const unsigned* p) {
+  if constexpr (N == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+    w[0] = *p;
+  }
+}
+
 template <int D>
-__global__ void __launch_bounds__(THREADS, 2)
+__global__ void __launch_bounds__(THREADS, 1)
 kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
   constexpr int G = D / GROUP, REC = rec_bytes(D);
   constexpr int Q_BYTES = BM * D * 2, T_BYTES = BN * D * 2;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* base = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  unsigned char* Qs = base;                            // [D / 64][128 rows][128 B]
-  unsigned char* Ks = Qs + Q_BYTES;                    // [2][D / 64][64 keys][128 B]
-  unsigned char* Vs = Ks + 2 * T_BYTES;                // [2][D rows][64 keys: 128 B]
-  unsigned* nums = reinterpret_cast<unsigned*>(Vs + 2 * T_BYTES);   // [4 warps][keys s, lo: 16 tokens x G; values s, lo: 8 pairs x G]
-  __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], e_full[4], p_full, o_ready, q_full;
-  __shared__ float key_unit[4][RECS];                  // 2^exponent of a record's keys, negative: no key of it is seen
-  __shared__ int value_exp[4][RECS];
+  unsigned char* Qs = base;                            // [2 halves][D / 64][128 rows][128 B]
+  unsigned char* Ks = Qs + Q_BYTES;                    // [STAGES][D / 64][64 keys][128 B]
+  unsigned char* Vs = Ks + STAGES * T_BYTES;           // [STAGES][D rows][64 keys: 128 B]
+  unsigned* nums = reinterpret_cast<unsigned*>(Vs + STAGES * T_BYTES);   // [CONV][keys s, lo: 16 tokens x G; values s, lo: 8 pairs x G]
+  __shared__ __align__(8) uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2][2], e_full[UNITS],
+      p_full[2][2], o_ready[2], o_done[2], q_full[2];
+  __shared__ float key_unit[UNITS][RECS];              // 2^exponent of a record's keys, negative: no key of it is seen
+  __shared__ int value_exp[UNITS][RECS];
   __shared__ uint32_t tmem_base_smem;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
@@ -151,21 +171,26 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
   const int n_tiles = tile_lo + (int)((long long)all_tiles * (split + 1) / sp.splits) - t_begin;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < STAGES; ++i) {
       mbar_init(&k_full[i], RECS);
       mbar_init(&k_empty[i], 1);
       mbar_init(&v_full[i], RECS);
       mbar_init(&v_empty[i], 1);
-      mbar_init(&s_full[i], 1);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(&e_full[i], RECS);
-    mbar_init(&p_full, 4);
-    mbar_init(&o_ready, 1);
-    mbar_init(&q_full, 4);
+    for (int i = 0; i < UNITS; ++i) mbar_init(&e_full[i], RECS);
+    for (int h = 0; h < 2; ++h) {
+      mbar_init(&s_full[h][0], 1);
+      mbar_init(&s_full[h][1], 1);
+      mbar_init(&p_full[h][0], 4);
+      mbar_init(&p_full[h][1], 4);
+      mbar_init(&o_ready[h], 1);
+      mbar_init(&o_done[h], 1);
+      mbar_init(&q_full[h], 4);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  if (warp == 8) {
+  if (warp == MMA_WARP) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                  ::"r"(smem_u32(&tmem_base_smem)), "r"(TMEM_COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -175,16 +200,19 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = tmem_base_smem;
 
-  if (warp >= 4 && warp < 8) {
+  const int halves = rows_here > HALF ? 2 : 1;
+  if (warp >= SOFT && warp < MMA_WARP) {
     // ------------------------------------------------------------ records to operands
-    const int rec = warp - 4;
-    unsigned* kn = nums + rec * (48 * G);              // keys: [16 tokens][G] s twice, then lo twice
+    // records q = 4 tile + r of the block's tiles, q = own, own + CONV, ...
+    const int own = warp - SOFT, records = n_tiles * RECS;
+    unsigned* kn = nums + own * (48 * G);              // keys: [16 tokens][G] s twice, then lo twice
     unsigned* vn = kn + 32 * G;                        // values: [8 pairs][G] s, then lo
     const int32_t* table = p.block_table + (long long)r * p.bt_stride;
-    auto record = [&](int j) -> long long {            // where tile j's record of this warp lies, -1: nothing to be seen
-      const int t = (t_begin + j) * RECS + rec;
-      if (j >= n_tiles || t * REC_TOKENS > pos_max || t * REC_TOKENS + REC_TOKENS <= low_min) return -1;
-      const int blk = t / per_page;
+    const int page_shift = (per_page & (per_page - 1)) == 0 ? 31 - __clz(per_page) : -1;
+    auto record = [&](int n) -> long long {            // where record n lies, -1: nothing to be seen
+      const int t = t_begin * RECS + n;
+      if (n >= records || t * REC_TOKENS > pos_max || t * REC_TOKENS + REC_TOKENS <= low_min) return -1;
+      const int blk = page_shift >= 0 ? t >> page_shift : t / per_page;
       const int page = blk < p.table_pages ? table[blk] : -1;
       return page >= 0 && page < p.num_pages ? ((long long)(page * KV + kvh) * per_page + (t - blk * per_page)) * REC : -1;
     };
@@ -227,13 +255,13 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
         nw[0] = x.x, nw[1] = x.y;
       }
     };
-    long long at = record(0), at_next = record(1);
+    long long at = record(own), at_next = record(own + CONV);
     load(at);
     bool ok = true;
-    for (int j = 0; j < n_tiles; ++j) {
-      const int st = j & 1;
+    for (int n = own; n < records; n += CONV) {
+      const int j = n / RECS, rec = n % RECS, st = j % STAGES, round = j / STAGES;
       const bool seen = at >= 0;
-      const int key = ((t_begin + j) * RECS + rec) * REC_TOKENS + 2 * np;     // the numbers' two tokens
+      const int key = (t_begin * RECS + n) * REC_TOKENS + 2 * np;            // the numbers' two tokens
       // places that hold no key of this row tile may hold anything: their numbers count as zero
       const unsigned keep = !seen ? 0u : (key <= pos_max && key >= low_min ? 0xffffu : 0u) |
                                              (key + 1 <= pos_max && key + 1 >= low_min ? 0xffff0000u : 0u);
@@ -268,21 +296,24 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
 #pragma unroll
         for (int g = 0; g < G; ++g) dst[g] = half[g];
       }
-      if (lane == 0) key_unit[j & 3][rec] = seen ? pow2(e) : -1.f;
-      if (lane == 16) value_exp[j & 3][rec] = e;
+      if (lane == 0) key_unit[j % UNITS][rec] = seen ? pow2(e) : -1.f;
+      if (lane == 16) value_exp[j % UNITS][rec] = e;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&e_full[j & 3]);
+      if (lane == 0) mbar_arrive(&e_full[j % UNITS]);
       // ---- keys
-      if (lane == 0) ok = ok && mbar_wait(&k_empty[st], ((j >> 1) & 1) ^ 1, err);
+      if (lane == 0) ok = ok && mbar_wait(&k_empty[st], (round & 1) ^ 1, err);
       __syncwarp();
       unsigned char* kd = Ks + st * T_BYTES;
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const int t = kt + 8 * n, row = rec * REC_TOKENS + t;
+      for (int i = 0; i < 2; ++i) {
+        const int t = kt + 8 * i, row = rec * REC_TOKENS + t;
+        unsigned sc[G], lo[G];
+        words<G>(sc, kn + t * G);
+        words<G>(lo, kn + 16 * G + t * G);
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           unsigned x[4] = {};
-          if (seen) four_pairs(kw[n][g], kn[t * G + g], kn[16 * G + t * G + g], x);
+          if (seen) four_pairs(kw[i][g], sc[g], lo[g], x);
           *reinterpret_cast<uint4*>(kd + (g >> 1) * (BN * 128) + swizzled(row, 4 * (g & 1) + kj)) = make_uint4(x[0], x[1], x[2], x[3]);
         }
       }
@@ -290,75 +321,91 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&k_full[st]);
-        ok = ok && mbar_wait(&v_empty[st], ((j >> 1) & 1) ^ 1, err);
+        ok = ok && mbar_wait(&v_empty[st], (round & 1) ^ 1, err);
       }
       __syncwarp();
       // ---- values
       unsigned char* vd = Vs + st * T_BYTES;
+      unsigned sc[4][G / 2], lo[4][G / 2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        words<G / 2>(sc[i], vn + (4 * vc + i) * G + vg);
+        words<G / 2>(lo[i], vn + 8 * G + (4 * vc + i) * G + vg);
+      }
 #pragma unroll
       for (int g = 0; g < G / 2; ++g) {
         unsigned x[4][4] = {};                         // [pair][i]
         if (seen) {
 #pragma unroll
-          for (int n = 0; n < 4; ++n) four_pairs(vw[n][g], vn[(4 * vc + n) * G + vg + g], vn[8 * G + (4 * vc + n) * G + vg + g], x[n]);
+          for (int i = 0; i < 4; ++i) four_pairs(vw[i][g], sc[i][g], lo[i][g], x[i]);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           *reinterpret_cast<uint4*>(vd + swizzled(32 * (vg + g) + 8 * i + vr, 2 * rec + vc)) = make_uint4(x[0][i], x[1][i], x[2][i], x[3][i]);
       }
       at = at_next;
-      load(at);                                        // the next tile's words, while this one is multiplied
-      at_next = record(j + 2);
+      load(at);                                        // the next record's words, while this one is multiplied
+      at_next = record(n + 2 * CONV);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&v_full[st]);
     }
     // the commits that release the last tiles arrive whenever the tensor core gets there: not after the block is gone
-    if (lane == 0) {
-      for (int j = max(0, n_tiles - 2); j < n_tiles && ok; ++j) {
-        ok = mbar_wait(&k_empty[j & 1], (j >> 1) & 1, err);
-        ok = ok && mbar_wait(&v_empty[j & 1], (j >> 1) & 1, err);
+    if (own == 0 && lane == 0) {
+      for (int j = max(0, n_tiles - STAGES); j < n_tiles && ok; ++j) {
+        ok = mbar_wait(&k_empty[j % STAGES], (j / STAGES) & 1, err);
+        ok = ok && mbar_wait(&v_empty[j % STAGES], (j / STAGES) & 1, err);
       }
     }
-  } else if (warp == 8) {
+  } else if (warp == MMA_WARP) {
     if (lane == 0 && n_tiles > 0) {
       // ------------------------------------------------------------ MMA issuer
-      const uint32_t idesc_s = idesc_f16(BM, BN), idesc_o = idesc_f16(BM, D);
-      const uint32_t q_addr = smem_u32(Qs);
+      const uint32_t idesc_s = idesc_f16(HALF, BN), idesc_o = idesc_f16(HALF, D);
       bool ok = true;
-      auto issue_qk = [&](int j) {
-        const int st = j & 1;
-        ok = ok && mbar_wait(&k_full[st], (j >> 1) & 1, err);
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t k_addr = smem_u32(Ks + st * T_BYTES);
+      auto issue_qk = [&](int j, int h) {
+        const int st = j % STAGES;
+        const uint32_t q_addr = smem_u32(Qs) + h * (HALF * D * 2), k_addr = smem_u32(Ks + st * T_BYTES);
+        const uint32_t d = tmem_base + S_COL + h * 128 + (j & 1) * BN;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks)
-          umma(tmem_base + S_COL + st * BN, make_desc(q_addr + (ks >> 2) * (BM * 128) + (ks & 3) * 32),
+          umma(d, make_desc(q_addr + (ks >> 2) * (HALF * 128) + (ks & 3) * 32),
                make_desc(k_addr + (ks >> 2) * (BN * 128) + (ks & 3) * 32), idesc_s, ks > 0 ? 1u : 0u);
-        umma_commit(&k_empty[st]);
-        umma_commit(&s_full[st]);
+        umma_commit(&s_full[h][j & 1]);
+        if (h + 1 == halves) umma_commit(&k_empty[st]);
       };
-      ok = ok && mbar_wait(&q_full, 0, err);
-      issue_qk(0);
-      if (n_tiles > 1) issue_qk(1);
-      for (int j = 0; j < n_tiles && ok; ++j) {
-        const int st = j & 1;
-        ok = ok && mbar_wait(&v_full[st], (j >> 1) & 1, err);
-        ok = ok && mbar_wait(&p_full, j & 1, err);     // P_j written, O rescaled
+      for (int h = 0; h < halves; ++h) ok = ok && mbar_wait(&q_full[h], 0, err);
+      for (int j = 0; j < min(2, n_tiles); ++j) {
+        ok = ok && mbar_wait(&k_full[j], 0, err);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t v_addr = smem_u32(Vs + st * T_BYTES);
+        for (int h = 0; h < halves; ++h) issue_qk(j, h);
+      }
+      for (int j = 0; j < n_tiles && ok; ++j) {
+        const int st = j % STAGES, next = j + 2;
+        ok = ok && mbar_wait(&v_full[st], (j / STAGES) & 1, err);
+        for (int h = 0; h < halves; ++h) {
+          ok = ok && mbar_wait(&p_full[h][j & 1], (j >> 1) & 1, err);          // P_j written, O rescaled
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t v_addr = smem_u32(Vs + st * T_BYTES);
 #pragma unroll
-        for (int ks = 0; ks < BN / 16; ++ks)
-          umma_ts(tmem_base + O_COL, tmem_base + S_COL + st * BN + ks * 8, make_desc(v_addr + ks * 32), idesc_o,
-                  (j > 0 || ks > 0) ? 1u : 0u);
-        umma_commit(&v_empty[st]);
-        umma_commit(&o_ready);
-        if (j + 2 < n_tiles) issue_qk(j + 2);          // into the buffer that P_j has left: the tensor pipe runs in order
+          for (int ks = 0; ks < BN / 16; ++ks)
+            umma_ts(tmem_base + O_COL + h * 128, tmem_base + S_COL + h * 128 + (j & 1) * BN + ks * 8, make_desc(v_addr + ks * 32),
+                    idesc_o, (j > 0 || ks > 0) ? 1u : 0u);
+          umma_commit(&o_ready[h]);
+          if (j + 1 == n_tiles) umma_commit(&o_done[h]);
+          if (h + 1 == halves) umma_commit(&v_empty[st]);
+          if (next < n_tiles) {                        // into the buffer that P_j has left: the tensor pipe runs in order
+            if (h == 0) {
+              ok = ok && mbar_wait(&k_full[next % STAGES], (next / STAGES) & 1, err);
+              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            }
+            issue_qk(next, h);
+          }
+        }
       }
     }
-  } else {
+  } else if (warp < 4 * halves) {
     // ---------------------------------------------------------------- softmax, correction, epilogue
-    const int row = warp * 32 + lane, pr = pr0 + row;
+    const int h = warp >> 2, row = warp * 32 + lane, pr = pr0 + row;
     const bool row_valid = row < rows_here;
     const int q_row = row_valid ? pr / HG : 0, head = kvh * HG + (row_valid ? pr - q_row * HG : 0);
     const bool held = row_valid && q0 >= 0 && q0 + q_row < p.rows;
@@ -385,39 +432,40 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
         unsigned x[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = h2(__uint_as_float(u[i] << 16) * by, __uint_as_float(u[i] & 0xffff0000u) * by);
-        *reinterpret_cast<uint4*>(Qs + (c >> 3) * (BM * 128) + swizzled(row, c & 7)) = make_uint4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<uint4*>(Qs + h * (HALF * D * 2) + (c >> 3) * (HALF * 128) + swizzled(row & (HALF - 1), c & 7)) = make_uint4(x[0], x[1], x[2], x[3]);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full);
+      if (lane == 0) mbar_arrive(&q_full[h]);
     }
-    const uint32_t lane_addr = tmem_base + ((uint32_t)(warp * 32) << 16);
+    const uint32_t lane_addr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t s_addr = lane_addr + S_COL + h * 128, o_addr = lane_addr + O_COL + h * 128;
     float m_run = -INFINITY, l_run = 0.f;              // maximum in units of log2
     int e_run = -2 * MOST_E;                           // the output's unit: 2^(e_run - ROOM + m_run)
     bool ok = true;
     for (int j = 0; j < n_tiles; ++j) {
       const int st = j & 1, ts = (t_begin + j) * BN;
-      ok = ok && mbar_wait(&s_full[st], (j >> 1) & 1, err);
-      ok = ok && mbar_wait(&e_full[j & 3], (j >> 2) & 1, err);
+      ok = ok && mbar_wait(&s_full[h][st], (j >> 1) & 1, err);
+      ok = ok && mbar_wait(&e_full[j % UNITS], (j / UNITS) & 1, err);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       float s[BN];
 #pragma unroll
-      for (int c = 0; c < BN / 32; ++c) tmem_ld32_nowait(lane_addr + S_COL + st * BN + c * 32, &s[c * 32]);
+      for (int c = 0; c < BN / 32; ++c) tmem_ld32_nowait(s_addr + st * BN + c * 32, &s[c * 32]);
       float unit[RECS];
       int ev[RECS];
       bool whole = ts + BN - 1 <= pos_min && ts >= low_max;
 #pragma unroll
       for (int g = 0; g < RECS; ++g) {
-        unit[g] = key_unit[j & 3][g] * row_unit;
-        ev[g] = value_exp[j & 3][g];
-        whole = whole && key_unit[j & 3][g] > 0.f;
+        unit[g] = key_unit[j % UNITS][g] * row_unit;
+        ev[g] = value_exp[j % UNITS][g];
+        whole = whole && key_unit[j % UNITS][g] > 0.f;
       }
       asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
       if (!whole) {
 #pragma unroll
         for (int i = 0; i < BN; ++i) {
           const int key = ts + i;
-          if (key > pos || key < lo || !(key_unit[j & 3][i / REC_TOKENS] > 0.f)) s[i] = -INFINITY;
+          if (key > pos || key < lo || !(key_unit[j % UNITS][i / REC_TOKENS] > 0.f)) s[i] = -INFINITY;
         }
 #pragma unroll
         for (int g = 0; g < RECS; ++g) unit[g] = fabsf(unit[g]);
@@ -458,21 +506,20 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
         uint32_t w[BN / 2];
 #pragma unroll
         for (int i = 0; i < BN / 2; ++i) w[i] = h2(s[2 * i], s[2 * i + 1]);
-        tmem_st32_nowait(lane_addr + S_COL + st * BN, &w[0]);
+        tmem_st32_nowait(s_addr + st * BN, &w[0]);
       }
-      if (j > 0) {
-        ok = ok && mbar_wait(&o_ready, (j - 1) & 1, err);
+      // only a rescaled output has to wait for the product before (the scores of tile j came after that of tile j - 2)
+      if (j > 0 && __any_sync(0xffffffffu, m_new > m_run || e_new > e_run)) {
+        ok = ok && mbar_wait(&o_ready[h], (j - 1) & 1, err);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (__any_sync(0xffffffffu, m_new > m_run || e_new > e_run)) {
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            float v[32];
-            tmem_ld32(lane_addr + O_COL + c * 32, v);
-            uint32_t w[32];
+        for (int c = 0; c < D / 32; ++c) {
+          float v[32];
+          tmem_ld32(o_addr + c * 32, v);
+          uint32_t w[32];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i] * alpha);
-            tmem_st32_nowait(lane_addr + O_COL + c * 32, w);
-          }
+          for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i] * alpha);
+          tmem_st32_nowait(o_addr + c * 32, w);
         }
       }
       m_run = m_new;
@@ -480,11 +527,11 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full);
+      if (lane == 0) mbar_arrive(&p_full[h][st]);      // by turns: the next tile's may come before this one is waited for
     }
     pdl_launch_dependents();
     if (n_tiles > 0) {
-      ok = ok && mbar_wait(&o_ready, (n_tiles - 1) & 1, err);
+      ok = ok && mbar_wait(&o_done[h], 0, err);        // o_ready may be two products behind: its parity would not tell
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     }
     // l is in units of 2^(m_run - ROOM), the output in units of 2^e_run more
@@ -495,7 +542,7 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
     for (int g = 0; g < G; ++g) {
       float v[32];
       if (n_tiles > 0) {                               // block-uniform: every lane takes part in the load
-        tmem_ld32(lane_addr + O_COL + g * 32, v);
+        tmem_ld32(o_addr + g * 32, v);
       } else {
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = 0.f;
@@ -529,7 +576,7 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   }
   __syncthreads();
-  if (warp == 8) {
+  if (warp == MMA_WARP) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
   }
@@ -574,17 +621,17 @@ __global__ void __launch_bounds__(256) kv4_tc5_merge_kernel(Kv4AttnParams p, Tc5
 
 template <int D>
 int launch(const Kv4AttnParams& p, const Tc5Split& sp, int tiles, int* err, cudaStream_t stream) {
-  const size_t smem = (size_t)BM * D * 2 + 4 * (size_t)BN * D * 2 + RECS * 48 * (D / GROUP) * 4 + 1024;
+  const size_t smem = (size_t)BM * D * 2 + 2 * STAGES * (size_t)BN * D * 2 + CONV * 48 * (D / GROUP) * 4 + 1024;
   static OptIn opt_in;
   if (const cudaError_t e = opt_in(smem, kv4_attention_tc5_kernel<D>)) return (int)e;
   launch_k(kv4_attention_tc5_kernel<D>, (unsigned)(tiles * p.kv_heads * sp.splits), THREADS, smem, stream, p, sp, err);
-  if (sp.splits > 1) launch_k(kv4_tc5_merge_kernel<D>, dim3(tiles * p.kv_heads, 4), 256, 0, stream, p, sp);
+  if (sp.splits > 1) launch_k(kv4_tc5_merge_kernel<D>, dim3(tiles * p.kv_heads, 8), 256, 0, stream, p, sp);
   return launch_status();
 }
 }  // namespace
 
-// Requests of more than most_packed packed rows.  tiles: row tiles of 128 packed rows, at least as many as there are.
-// workspace (splits > 1): tiles * kv_heads * splits * 128 * (head_dim + 2) floats.
+// Requests of more than most_packed packed rows.  tiles: row tiles of 256 packed rows, at least as many as there are.
+// workspace (splits > 1): tiles * kv_heads * splits * 256 * (head_dim + 2) floats.
 PBE_EXPORT int pbe_kv4_attention_tc5(const Kv4AttnParams* params, float* workspace, int tiles, int splits, int head_dim,
                                      int most_packed, int* err, cudaStream_t stream) {
   const Kv4AttnParams p = *params;
