@@ -90,6 +90,27 @@ __device__ __forceinline__ uint32_t idesc_f16(int m, int n) {
   return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
+// The products' instructions, executed by a whole warp and issued by one elected lane of it.  Code that all lanes run alike
+// keeps descriptors and addresses in uniform registers, where the instruction takes them from; issued from a branch of one
+// lane, each product waited some 100 cycles for them to be moved there, three times what the tensor core takes for it.
+__device__ __forceinline__ void mma_elected(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p, q;\nelect.sync _|q, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_ts_elected(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p, q;\nelect.sync _|q, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void commit_elected(uint64_t* bar) {
+  asm volatile(
+      "{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\n"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)) : "memory");
+}
+
 struct Tile {
   int req, row_tile, index;    // index: among all row tiles; req < 0: none
 };
@@ -209,12 +230,15 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
     unsigned* vn = kn + 32 * G;                        // values: [8 pairs][G] s, then lo
     const int32_t* table = p.block_table + (long long)r * p.bt_stride;
     const int page_shift = (per_page & (per_page - 1)) == 0 ? 31 - __clz(per_page) : -1;
-    auto record = [&](int n) -> long long {            // where record n lies, -1: nothing to be seen
+    auto page_of = [&](int n) {                        // the page of record n, -1: nothing to be seen
       const int t = t_begin * RECS + n;
       if (n >= records || t * REC_TOKENS > pos_max || t * REC_TOKENS + REC_TOKENS <= low_min) return -1;
       const int blk = page_shift >= 0 ? t >> page_shift : t / per_page;
-      const int page = blk < p.table_pages ? table[blk] : -1;
-      return page >= 0 && page < p.num_pages ? ((long long)(page * KV + kvh) * per_page + (t - blk * per_page)) * REC : -1;
+      return blk < p.table_pages ? table[blk] : -1;
+    };
+    auto record = [&](int n, int page) -> long long {  // and where it lies
+      const int t = t_begin * RECS + n, in_page = page_shift >= 0 ? t & (per_page - 1) : t % per_page;
+      return page >= 0 && page < p.num_pages ? ((long long)(page * KV + kvh) * per_page + in_page) * REC : -1;
     };
     // lane's tasks: keys: tokens kt and kt + 8, words j of all groups; values: pairs 4 vc .. 4 vc + 3, r8, half the groups;
     // numbers: four words of one kind and pair
@@ -255,7 +279,9 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
         nw[0] = x.x, nw[1] = x.y;
       }
     };
-    long long at = record(own), at_next = record(own + CONV);
+    // pages are asked for two records ahead, words one: neither is waited for where it is asked for
+    int page_1 = page_of(own + CONV), page_2 = page_of(own + 2 * CONV);
+    long long at = record(own, page_of(own));
     load(at);
     bool ok = true;
     for (int n = own; n < records; n += CONV) {
@@ -343,9 +369,10 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
         for (int i = 0; i < 4; ++i)
           *reinterpret_cast<uint4*>(vd + swizzled(32 * (vg + g) + 8 * i + vr, 2 * rec + vc)) = make_uint4(x[0][i], x[1][i], x[2][i], x[3][i]);
       }
-      at = at_next;
+      at = record(n + CONV, page_1);
       load(at);                                        // the next record's words, while this one is multiplied
-      at_next = record(n + 2 * CONV);
+      page_1 = page_2;
+      page_2 = page_of(n + 3 * CONV);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&v_full[st]);
@@ -358,44 +385,47 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
       }
     }
   } else if (warp == MMA_WARP) {
-    if (lane == 0 && n_tiles > 0) {
+    if (n_tiles > 0) {
       // ------------------------------------------------------------ MMA issuer
       const uint32_t idesc_s = idesc_f16(HALF, BN), idesc_o = idesc_f16(HALF, D);
+      const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
       bool ok = true;
+      // an operand further on is an addition to its descriptor's address field (in units of 16 bytes)
+      const uint64_t q_desc = make_desc(smem_u32(Qs)), k_desc = make_desc(smem_u32(Ks)), v_desc = make_desc(smem_u32(Vs));
       auto issue_qk = [&](int j, int h) {
         const int st = j % STAGES;
-        const uint32_t q_addr = smem_u32(Qs) + h * (HALF * D * 2), k_addr = smem_u32(Ks + st * T_BYTES);
-        const uint32_t d = tmem_base + S_COL + h * 128 + (j & 1) * BN;
+        const uint64_t a = q_desc + (uint32_t)(h * (HALF * D * 2 / 16)), b = k_desc + (uint32_t)(st * (T_BYTES / 16));
+        const uint32_t d = tmem + S_COL + h * 128 + (j & 1) * BN;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks)
-          umma(d, make_desc(q_addr + (ks >> 2) * (HALF * 128) + (ks & 3) * 32),
-               make_desc(k_addr + (ks >> 2) * (BN * 128) + (ks & 3) * 32), idesc_s, ks > 0 ? 1u : 0u);
-        umma_commit(&s_full[h][j & 1]);
-        if (h + 1 == halves) umma_commit(&k_empty[st]);
+          mma_elected(d, a + ((ks >> 2) * (HALF * 128 / 16) + (ks & 3) * 2), b + ((ks >> 2) * (BN * 128 / 16) + (ks & 3) * 2), idesc_s,
+               ks > 0 ? 1u : 0u);
+        commit_elected(&s_full[h][j & 1]);
+        if (h + 1 == halves) commit_elected(&k_empty[st]);
       };
-      for (int h = 0; h < halves; ++h) ok = ok && mbar_wait(&q_full[h], 0, err);
+      for (int h = 0; h < halves; ++h) ok = ok && mbar_wait_warp(&q_full[h], 0, err);
       for (int j = 0; j < min(2, n_tiles); ++j) {
-        ok = ok && mbar_wait(&k_full[j], 0, err);
+        ok = ok && mbar_wait_warp(&k_full[j], 0, err);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         for (int h = 0; h < halves; ++h) issue_qk(j, h);
       }
       for (int j = 0; j < n_tiles && ok; ++j) {
         const int st = j % STAGES, next = j + 2;
-        ok = ok && mbar_wait(&v_full[st], (j / STAGES) & 1, err);
+        ok = ok && mbar_wait_warp(&v_full[st], (j / STAGES) & 1, err);
         for (int h = 0; h < halves; ++h) {
-          ok = ok && mbar_wait(&p_full[h][j & 1], (j >> 1) & 1, err);          // P_j written, O rescaled
+          ok = ok && mbar_wait_warp(&p_full[h][j & 1], (j >> 1) & 1, err);          // P_j written, O rescaled
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t v_addr = smem_u32(Vs + st * T_BYTES);
+          const uint64_t b = v_desc + (uint32_t)(st * (T_BYTES / 16));
 #pragma unroll
           for (int ks = 0; ks < BN / 16; ++ks)
-            umma_ts(tmem_base + O_COL + h * 128, tmem_base + S_COL + h * 128 + (j & 1) * BN + ks * 8, make_desc(v_addr + ks * 32),
-                    idesc_o, (j > 0 || ks > 0) ? 1u : 0u);
-          umma_commit(&o_ready[h]);
-          if (j + 1 == n_tiles) umma_commit(&o_done[h]);
-          if (h + 1 == halves) umma_commit(&v_empty[st]);
+            mma_ts_elected(tmem + O_COL + h * 128, tmem + S_COL + h * 128 + (j & 1) * BN + ks * 8, b + ks * 2, idesc_o,
+                    (j > 0 || ks > 0) ? 1u : 0u);
+          commit_elected(&o_ready[h]);
+          if (j + 1 == n_tiles) commit_elected(&o_done[h]);
+          if (h + 1 == halves) commit_elected(&v_empty[st]);
           if (next < n_tiles) {                        // into the buffer that P_j has left: the tensor pipe runs in order
             if (h == 0) {
-              ok = ok && mbar_wait(&k_full[next % STAGES], (next / STAGES) & 1, err);
+              ok = ok && mbar_wait_warp(&k_full[next % STAGES], (next / STAGES) & 1, err);
               asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             }
             issue_qk(next, h);
