@@ -6,12 +6,12 @@
 //   softmax       warps 0-3 and 4-7, one thread a row: tcgen05.ld, maximum, exponentials, sum; the running maximum moves only
 //                 after it grew by 2^8, so the output accumulator is rarely rescaled, and only then waited for;
 //   O += P V      P goes back into the columns of its scores and is the A operand from tensor memory.
-// Warps 8-14 turn records into operands, record after record in turn: a record's words are loaded into registers while the
+// Warps 8-13 turn records into operands, record after record in turn: a record's words are loaded into registers while the
 // one before is converted, and lo + s * code is one float16 multiply-add a pair of channels, since a code in the low bits of
 // a float16 is already a number (code * 2^-24).  Keys become 64 rows of D channels, values D rows of 64 keys (their words
 // hold pairs of keys, so that is how they lie), both K-major under the 128-byte swizzle, three tiles of each in flight; the
 // rows of the values are ordered (group, i, r), so that eight lanes write eight different banks, and the epilogue puts the
-// channels back in order.  Warp 15 issues the products.  (With one half a block and two blocks a multiprocessor each record
+// channels back in order.  Warps 14 and 15 issue the products, each those of its half.  (With one half a block and two blocks a multiprocessor each record
 // was converted twice as often, and four converting warps were what the rest waited for: 4,096 tokens 269 us.)
 //
 // All operands are float16, with sums in float32: eleven bits where bfloat16 keeps eight, so the rounding of keys, values and
@@ -39,8 +39,8 @@ using namespace pbe::tc5;
 namespace {
 constexpr int HALF = 128, BM = 2 * HALF, BN = 64;     // packed rows of a block, keys of a tile
 constexpr int RECS = BN / REC_TOKENS;   // records of a tile
-constexpr int SOFT = 8, CONV = 7, MMA_WARP = SOFT + CONV;
-constexpr int THREADS = 32 * (MMA_WARP + 1);
+constexpr int SOFT = 8, CONV = 6, MMA_WARP = SOFT + CONV;    // and one issuing warp a half
+constexpr int THREADS = 32 * (MMA_WARP + 2);
 constexpr int STAGES = 3;               // tiles of keys and of values that are operands
 constexpr int UNITS = 8;                // tiles whose records' exponents are kept
 constexpr int TMEM_COLS = 512;
@@ -191,12 +191,13 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
   const int t_begin = tile_lo + (int)((long long)all_tiles * split / sp.splits);
   const int n_tiles = tile_lo + (int)((long long)all_tiles * (split + 1) / sp.splits) - t_begin;
 
+  const int halves = rows_here > HALF ? 2 : 1;
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&k_full[i], RECS);
-      mbar_init(&k_empty[i], 1);
+      mbar_init(&k_empty[i], halves);
       mbar_init(&v_full[i], RECS);
-      mbar_init(&v_empty[i], 1);
+      mbar_init(&v_empty[i], halves);
     }
     for (int i = 0; i < UNITS; ++i) mbar_init(&e_full[i], RECS);
     for (int h = 0; h < 2; ++h) {
@@ -221,7 +222,6 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = tmem_base_smem;
 
-  const int halves = rows_here > HALF ? 2 : 1;
   if (warp >= SOFT && warp < MMA_WARP) {
     // ------------------------------------------------------------ records to operands
     // records q = 4 tile + r of the block's tiles, q = own, own + CONV, ...
@@ -245,9 +245,14 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
     const int kj = lane & 3, kt = (lane >> 3) + 4 * ((lane >> 2) & 1);
     const int vr = lane & 7, vc = (lane >> 3) & 1, vg = (lane >> 4) * (G / 2);
     const int kind = lane >> 3, np = lane & 7;
-    unsigned kw[2][G], vw[4][G / 2], nw[G];
-    auto load = [&](long long at) {
+    struct Words {
+      unsigned k[2][G], v[4][G / 2], n[G];
+    };
+    auto load = [&](Words& to, long long at) {
       if (at < 0) return;
+      auto &kw = to.k;
+      auto &vw = to.v;
+      auto &nw = to.n;
       const unsigned char* src = p.pages + at;
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
@@ -282,10 +287,18 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
     // pages are asked for two records ahead, words one: neither is waited for where it is asked for
     int page_1 = page_of(own + CONV), page_2 = page_of(own + 2 * CONV);
     long long at = record(own, page_of(own));
-    load(at);
+    Words now, then;
+    load(now, at);
     bool ok = true;
     for (int n = own; n < records; n += CONV) {
       const int j = n / RECS, rec = n % RECS, st = j % STAGES, round = j / STAGES;
+      const long long at_then = record(n + CONV, page_1);
+      load(then, at_then);
+      page_1 = page_2;
+      page_2 = page_of(n + 3 * CONV);
+      auto &kw = now.k;
+      auto &vw = now.v;
+      auto &nw = now.n;
       const bool seen = at >= 0;
       const int key = (t_begin * RECS + n) * REC_TOKENS + 2 * np;            // the numbers' two tokens
       // places that hold no key of this row tile may hold anything: their numbers count as zero
@@ -369,13 +382,11 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
         for (int i = 0; i < 4; ++i)
           *reinterpret_cast<uint4*>(vd + swizzled(32 * (vg + g) + 8 * i + vr, 2 * rec + vc)) = make_uint4(x[0][i], x[1][i], x[2][i], x[3][i]);
       }
-      at = record(n + CONV, page_1);
-      load(at);                                        // the next record's words, while this one is multiplied
-      page_1 = page_2;
-      page_2 = page_of(n + 3 * CONV);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&v_full[st]);
+      now = then;
+      at = at_then;
     }
     // the commits that release the last tiles arrive whenever the tensor core gets there: not after the block is gone
     if (own == 0 && lane == 0) {
@@ -384,53 +395,43 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
         ok = ok && mbar_wait(&v_empty[j % STAGES], (j / STAGES) & 1, err);
       }
     }
-  } else if (warp == MMA_WARP) {
-    if (n_tiles > 0) {
-      // ------------------------------------------------------------ MMA issuer
+  } else if (warp >= MMA_WARP) {
+    const int h = warp - MMA_WARP;
+    if (h < halves && n_tiles > 0) {
+      // ------------------------------------------------------------ MMA issuer of half h
       const uint32_t idesc_s = idesc_f16(HALF, BN), idesc_o = idesc_f16(HALF, D);
-      const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+      const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0) + h * 128;
       bool ok = true;
       // an operand further on is an addition to its descriptor's address field (in units of 16 bytes)
-      const uint64_t q_desc = make_desc(smem_u32(Qs)), k_desc = make_desc(smem_u32(Ks)), v_desc = make_desc(smem_u32(Vs));
-      auto issue_qk = [&](int j, int h) {
+      const uint64_t q_desc = make_desc(smem_u32(Qs) + h * (HALF * D * 2)), k_desc = make_desc(smem_u32(Ks)), v_desc = make_desc(smem_u32(Vs));
+      auto scores = [&](int j) {
         const int st = j % STAGES;
-        const uint64_t a = q_desc + (uint32_t)(h * (HALF * D * 2 / 16)), b = k_desc + (uint32_t)(st * (T_BYTES / 16));
-        const uint32_t d = tmem + S_COL + h * 128 + (j & 1) * BN;
+        ok = ok && mbar_wait_warp(&k_full[st], (j / STAGES) & 1, err);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint64_t b = k_desc + (uint32_t)(st * (T_BYTES / 16));
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks)
-          mma_elected(d, a + ((ks >> 2) * (HALF * 128 / 16) + (ks & 3) * 2), b + ((ks >> 2) * (BN * 128 / 16) + (ks & 3) * 2), idesc_s,
-               ks > 0 ? 1u : 0u);
+          mma_elected(tmem + S_COL + (j & 1) * BN, q_desc + ((ks >> 2) * (HALF * 128 / 16) + (ks & 3) * 2),
+                      b + ((ks >> 2) * (BN * 128 / 16) + (ks & 3) * 2), idesc_s, ks > 0 ? 1u : 0u);
         commit_elected(&s_full[h][j & 1]);
-        if (h + 1 == halves) commit_elected(&k_empty[st]);
+        commit_elected(&k_empty[st]);
       };
-      for (int h = 0; h < halves; ++h) ok = ok && mbar_wait_warp(&q_full[h], 0, err);
-      for (int j = 0; j < min(2, n_tiles); ++j) {
-        ok = ok && mbar_wait_warp(&k_full[j], 0, err);
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        for (int h = 0; h < halves; ++h) issue_qk(j, h);
-      }
+      ok = ok && mbar_wait_warp(&q_full[h], 0, err);
+      scores(0);
+      if (n_tiles > 1) scores(1);
       for (int j = 0; j < n_tiles && ok; ++j) {
-        const int st = j % STAGES, next = j + 2;
+        const int st = j % STAGES;
         ok = ok && mbar_wait_warp(&v_full[st], (j / STAGES) & 1, err);
-        for (int h = 0; h < halves; ++h) {
-          ok = ok && mbar_wait_warp(&p_full[h][j & 1], (j >> 1) & 1, err);          // P_j written, O rescaled
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint64_t b = v_desc + (uint32_t)(st * (T_BYTES / 16));
+        ok = ok && mbar_wait_warp(&p_full[h][j & 1], (j >> 1) & 1, err);     // P_j written, O rescaled
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint64_t b = v_desc + (uint32_t)(st * (T_BYTES / 16));
 #pragma unroll
-          for (int ks = 0; ks < BN / 16; ++ks)
-            mma_ts_elected(tmem + O_COL + h * 128, tmem + S_COL + h * 128 + (j & 1) * BN + ks * 8, b + ks * 2, idesc_o,
-                    (j > 0 || ks > 0) ? 1u : 0u);
-          commit_elected(&o_ready[h]);
-          if (j + 1 == n_tiles) commit_elected(&o_done[h]);
-          if (h + 1 == halves) commit_elected(&v_empty[st]);
-          if (next < n_tiles) {                        // into the buffer that P_j has left: the tensor pipe runs in order
-            if (h == 0) {
-              ok = ok && mbar_wait_warp(&k_full[next % STAGES], (next / STAGES) & 1, err);
-              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            }
-            issue_qk(next, h);
-          }
-        }
+        for (int ks = 0; ks < BN / 16; ++ks)
+          mma_ts_elected(tmem + O_COL, tmem + S_COL + (j & 1) * BN + ks * 8, b + ks * 2, idesc_o, (j > 0 || ks > 0) ? 1u : 0u);
+        commit_elected(&o_ready[h]);
+        commit_elected(&v_empty[st]);
+        if (j + 1 == n_tiles) commit_elected(&o_done[h]);
+        if (j + 2 < n_tiles) scores(j + 2);            // into the buffer that P_j has left: the tensor pipe runs in order
       }
     }
   } else if (warp < 4 * halves) {
