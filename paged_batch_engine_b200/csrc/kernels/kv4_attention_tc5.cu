@@ -9,7 +9,7 @@
 // Warps 8-13 turn records into operands, record after record in turn: a record's words are loaded into registers while the
 // one before is converted, and lo + s * code is one float16 multiply-add a pair of channels, since a code in the low bits of
 // a float16 is already a number (code * 2^-24).  Keys become 64 rows of D channels, values D rows of 64 keys (their words
-// hold pairs of keys, so that is how they lie), both K-major under the 128-byte swizzle, three tiles of each in flight; the
+// hold pairs of keys, so that is how they lie), both K-major under the 128-byte swizzle, four tiles of each in flight; the
 // rows of the values are ordered (group, i, r), so that eight lanes write eight different banks, and the epilogue puts the
 // channels back in order.  Warps 14 and 15 issue the products, each those of its half.  (With one half a block and two blocks a multiprocessor each record
 // was converted twice as often, and four converting warps were what the rest waited for: 4,096 tokens 269 us.)
@@ -41,8 +41,7 @@ constexpr int HALF = 128, BM = 2 * HALF, BN = 64;     // packed rows of a block,
 constexpr int RECS = BN / REC_TOKENS;   // records of a tile
 constexpr int SOFT = 8, CONV = 6, MMA_WARP = SOFT + CONV;    // and one issuing warp a half
 constexpr int THREADS = 32 * (MMA_WARP + 2);
-constexpr int STAGES = 3;               // tiles of keys and of values that are operands
-constexpr int UNITS = 8;                // tiles whose records' exponents are kept
+constexpr int STAGES = 4;               // tiles of keys and of values that are operands
 constexpr int TMEM_COLS = 512;
 constexpr int S_COL = 0, O_COL = 256;   // of half h: two score buffers at 128 h, the output at 256 + 128 h
 constexpr int ROOM = 6;                 // weights are kept 2^6 times too large: float16 reaches further down
@@ -74,6 +73,26 @@ __device__ __forceinline__ unsigned hmul(unsigned a, unsigned b) {
   unsigned d;
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
+}
+// two float32 operations an instruction
+struct f32x2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ f32x2 both(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void apart(f32x2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
 }
 constexpr unsigned SIXTEENTH = 0x2c002c00u;            // 1/16 twice
 // the four pairs of a word: lo + s * code each
@@ -169,10 +188,9 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
   unsigned char* Ks = Qs + Q_BYTES;                    // [STAGES][D / 64][64 keys][128 B]
   unsigned char* Vs = Ks + STAGES * T_BYTES;           // [STAGES][D rows][64 keys: 128 B]
   unsigned* nums = reinterpret_cast<unsigned*>(Vs + STAGES * T_BYTES);   // [CONV][keys s, lo: 16 tokens x G; values s, lo: 8 pairs x G]
-  __shared__ __align__(8) uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2][2], e_full[UNITS],
-      p_full[2][2], o_ready[2], o_done[2], q_full[2];
-  __shared__ float key_unit[UNITS][RECS];              // 2^exponent of a record's keys, negative: no key of it is seen
-  __shared__ int value_exp[UNITS][RECS];
+  __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], s_full[2][2], p_full[2][2], o_ready[2], o_done[2], q_full[2];
+  __shared__ float key_unit[STAGES][RECS];              // 2^exponent of a record's keys, negative: no key of it is seen
+  __shared__ int value_exp[STAGES][RECS];
   __shared__ uint32_t tmem_base_smem;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
@@ -194,12 +212,9 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
   const int halves = rows_here > HALF ? 2 : 1;
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
-      mbar_init(&k_full[i], RECS);
-      mbar_init(&k_empty[i], halves);
-      mbar_init(&v_full[i], RECS);
-      mbar_init(&v_empty[i], halves);
+      mbar_init(&full[i], RECS);
+      mbar_init(&empty[i], halves);
     }
-    for (int i = 0; i < UNITS; ++i) mbar_init(&e_full[i], RECS);
     for (int h = 0; h < 2; ++h) {
       mbar_init(&s_full[h][0], 1);
       mbar_init(&s_full[h][1], 1);
@@ -310,13 +325,10 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
         nw[g] &= keep;
         most = max(most, max(nw[g] & 0x7fffu, (nw[g] >> 16) & 0x7fffu));
       }
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
       // kinds by eights of lanes: lo and s of keys, lo and s of values.  The unit is such that s reaches up to 2^-8 and lo
       // stays within float16
-      const int e_own = (int)(most >> 7) - 127, e_other = __shfl_xor_sync(0xffffffffu, e_own, 8);
-      const int e_s = kind & 1 ? e_own : e_other, e_lo = kind & 1 ? e_other : e_own;
-      const int e = max(-MOST_E, min(MOST_E + 9, max(e_s + 9, e_lo - 14)));
+      const int e_own = (int)(most >> 7) - 127 + (kind & 1 ? 9 : -14);
+      const int e = max(-MOST_E, min(MOST_E + 9, lane < 16 ? __reduce_max_sync(0x0000ffffu, e_own) : __reduce_max_sync(0xffff0000u, e_own)));
       const float by = pow2((kind & 1 ? 24 : 0) - e);
       unsigned half[G];
 #pragma unroll
@@ -335,13 +347,11 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
 #pragma unroll
         for (int g = 0; g < G; ++g) dst[g] = half[g];
       }
-      if (lane == 0) key_unit[j % UNITS][rec] = seen ? pow2(e) : -1.f;
-      if (lane == 16) value_exp[j % UNITS][rec] = e;
+      if (lane == 0) ok = ok && mbar_wait(&empty[st], (round & 1) ^ 1, err);
       __syncwarp();
-      if (lane == 0) mbar_arrive(&e_full[j % UNITS]);
+      if (lane == 0) key_unit[st][rec] = seen ? pow2(e) : -1.f;
+      if (lane == 16) value_exp[st][rec] = e;
       // ---- keys
-      if (lane == 0) ok = ok && mbar_wait(&k_empty[st], (round & 1) ^ 1, err);
-      __syncwarp();
       unsigned char* kd = Ks + st * T_BYTES;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -356,13 +366,6 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
           *reinterpret_cast<uint4*>(kd + (g >> 1) * (BN * 128) + swizzled(row, 4 * (g & 1) + kj)) = make_uint4(x[0], x[1], x[2], x[3]);
         }
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&k_full[st]);
-        ok = ok && mbar_wait(&v_empty[st], (round & 1) ^ 1, err);
-      }
-      __syncwarp();
       // ---- values
       unsigned char* vd = Vs + st * T_BYTES;
       unsigned sc[4][G / 2], lo[4][G / 2];
@@ -384,15 +387,14 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(&v_full[st]);
+      if (lane == 0) mbar_arrive(&full[st]);
       now = then;
       at = at_then;
     }
     // the commits that release the last tiles arrive whenever the tensor core gets there: not after the block is gone
     if (own == 0 && lane == 0) {
       for (int j = max(0, n_tiles - STAGES); j < n_tiles && ok; ++j) {
-        ok = mbar_wait(&k_empty[j % STAGES], (j / STAGES) & 1, err);
-        ok = ok && mbar_wait(&v_empty[j % STAGES], (j / STAGES) & 1, err);
+        ok = mbar_wait(&empty[j % STAGES], (j / STAGES) & 1, err);
       }
     }
   } else if (warp >= MMA_WARP) {
@@ -406,7 +408,7 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
       const uint64_t q_desc = make_desc(smem_u32(Qs) + h * (HALF * D * 2)), k_desc = make_desc(smem_u32(Ks)), v_desc = make_desc(smem_u32(Vs));
       auto scores = [&](int j) {
         const int st = j % STAGES;
-        ok = ok && mbar_wait_warp(&k_full[st], (j / STAGES) & 1, err);
+        ok = ok && mbar_wait_warp(&full[st], (j / STAGES) & 1, err);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint64_t b = k_desc + (uint32_t)(st * (T_BYTES / 16));
 #pragma unroll
@@ -414,14 +416,12 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
           mma_elected(tmem + S_COL + (j & 1) * BN, q_desc + ((ks >> 2) * (HALF * 128 / 16) + (ks & 3) * 2),
                       b + ((ks >> 2) * (BN * 128 / 16) + (ks & 3) * 2), idesc_s, ks > 0 ? 1u : 0u);
         commit_elected(&s_full[h][j & 1]);
-        commit_elected(&k_empty[st]);
       };
       ok = ok && mbar_wait_warp(&q_full[h], 0, err);
       scores(0);
       if (n_tiles > 1) scores(1);
       for (int j = 0; j < n_tiles && ok; ++j) {
         const int st = j % STAGES;
-        ok = ok && mbar_wait_warp(&v_full[st], (j / STAGES) & 1, err);
         ok = ok && mbar_wait_warp(&p_full[h][j & 1], (j >> 1) & 1, err);     // P_j written, O rescaled
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint64_t b = v_desc + (uint32_t)(st * (T_BYTES / 16));
@@ -429,7 +429,7 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
         for (int ks = 0; ks < BN / 16; ++ks)
           mma_ts_elected(tmem + O_COL, tmem + S_COL + (j & 1) * BN + ks * 8, b + ks * 2, idesc_o, (j > 0 || ks > 0) ? 1u : 0u);
         commit_elected(&o_ready[h]);
-        commit_elected(&v_empty[st]);
+        commit_elected(&empty[st]);                    // the keys were multiplied before
         if (j + 1 == n_tiles) commit_elected(&o_done[h]);
         if (j + 2 < n_tiles) scores(j + 2);            // into the buffer that P_j has left: the tensor pipe runs in order
       }
@@ -475,9 +475,9 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
     int e_run = -2 * MOST_E;                           // the output's unit: 2^(e_run - ROOM + m_run)
     bool ok = true;
     for (int j = 0; j < n_tiles; ++j) {
-      const int st = j & 1, ts = (t_begin + j) * BN;
+      const int st = j & 1, kst = j % STAGES, ts = (t_begin + j) * BN;
       ok = ok && mbar_wait(&s_full[h][st], (j >> 1) & 1, err);
-      ok = ok && mbar_wait(&e_full[j % UNITS], (j / UNITS) & 1, err);
+      ok = ok && mbar_wait(&full[kst], (j / STAGES) & 1, err);              // complete, but for the exponents beside it
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       float s[BN];
 #pragma unroll
@@ -487,16 +487,16 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
       bool whole = ts + BN - 1 <= pos_min && ts >= low_max;
 #pragma unroll
       for (int g = 0; g < RECS; ++g) {
-        unit[g] = key_unit[j % UNITS][g] * row_unit;
-        ev[g] = value_exp[j % UNITS][g];
-        whole = whole && key_unit[j % UNITS][g] > 0.f;
+        unit[g] = key_unit[kst][g] * row_unit;
+        ev[g] = value_exp[kst][g];
+        whole = whole && key_unit[kst][g] > 0.f;
       }
       asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
       if (!whole) {
 #pragma unroll
         for (int i = 0; i < BN; ++i) {
           const int key = ts + i;
-          if (key > pos || key < lo || !(key_unit[j % UNITS][i / REC_TOKENS] > 0.f)) s[i] = -INFINITY;
+          if (key > pos || key < lo || !(key_unit[kst][i / REC_TOKENS] > 0.f)) s[i] = -INFINITY;
         }
 #pragma unroll
         for (int g = 0; g < RECS; ++g) unit[g] = fabsf(unit[g]);
@@ -522,14 +522,17 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
 #pragma unroll
       for (int g = 0; g < RECS; ++g) {
         const float off = (float)(ROOM + ev[g] - e_new) - m_use;
-        float a = 0.f, b = 0.f;
+        const f32x2 unit2 = both(unit[g], unit[g]), off2 = both(off, off);
+        f32x2 part = both(0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          s[g * 16 + i] = ex2(fmaf(s[g * 16 + i], unit[g], off));
-          s[g * 16 + i + 1] = ex2(fmaf(s[g * 16 + i + 1], unit[g], off));
-          a += s[g * 16 + i];
-          b += s[g * 16 + i + 1];
+        for (int i = g * 16; i < g * 16 + 16; i += 2) {
+          apart(fma2(both(s[i], s[i + 1]), unit2, off2), s[i], s[i + 1]);
+          s[i] = ex2(s[i]);
+          s[i + 1] = ex2(s[i + 1]);
+          part = add2(part, both(s[i], s[i + 1]));
         }
+        float a, b;
+        apart(part, a, b);
         sum = fmaf(a + b, ex2((float)min(e_new - ev[g], 126)), sum);
       }
       l_run = fmaf(l_run, shrink, sum);
