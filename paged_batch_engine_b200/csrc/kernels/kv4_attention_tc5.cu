@@ -3,8 +3,8 @@
 // One block owns a row tile of 256 packed rows (query row x head of the group) of one key/value head, two halves of 128, and
 // walks over its keys in tiles of 64, four records, which both halves read once they are operands:
 //   S = Q K^T     tcgen05.mma, 128 x 64 x D, into two alternating score buffers in tensor memory for each half;
-//   softmax       warps 0-3 and 4-7, one thread a row: tcgen05.ld, maximum, exponentials, sum; the running maximum moves only
-//                 after it grew by 2^8, so the output accumulator is rarely rescaled, and only then waited for;
+//   softmax       warps 0-3 and 4-7, one thread a row: tcgen05.ld, maximum, exponentials, sum; weights are made against the maximum so far, which
+//                 moves only when they grow too large for it, so the output is rarely rescaled, and only then waited for;
 //   O += P V      P goes back into the columns of its scores and is the A operand from tensor memory.
 // Warps 8-13 turn records into operands, record after record in turn: a record's words are loaded into registers while the
 // one before is converted, and lo + s * code is one float16 multiply-add a pair of channels, since a code in the low bits of
@@ -128,6 +128,23 @@ __device__ __forceinline__ void commit_elected(uint64_t* bar) {
   asm volatile(
       "{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\n"
       "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// the wait for loads from tensor memory, which these registers' uses stay behind
+__device__ __forceinline__ void tmem_landed(float (&x)[BN]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(x[0]), "+f"(x[1]), "+f"(x[2]), "+f"(x[3]), "+f"(x[4]), "+f"(x[5]), "+f"(x[6]), "+f"(x[7]),
+                 "+f"(x[8]), "+f"(x[9]), "+f"(x[10]), "+f"(x[11]), "+f"(x[12]), "+f"(x[13]), "+f"(x[14]), "+f"(x[15]),
+                 "+f"(x[16]), "+f"(x[17]), "+f"(x[18]), "+f"(x[19]), "+f"(x[20]), "+f"(x[21]), "+f"(x[22]),
+                 "+f"(x[23]), "+f"(x[24]), "+f"(x[25]), "+f"(x[26]), "+f"(x[27]), "+f"(x[28]), "+f"(x[29]),
+                 "+f"(x[30]), "+f"(x[31])
+               :: "memory");
+  asm volatile(""
+               : "+f"(x[32]), "+f"(x[33]), "+f"(x[34]), "+f"(x[35]), "+f"(x[36]), "+f"(x[37]), "+f"(x[38]), "+f"(x[39]),
+                 "+f"(x[40]), "+f"(x[41]), "+f"(x[42]), "+f"(x[43]), "+f"(x[44]), "+f"(x[45]), "+f"(x[46]),
+                 "+f"(x[47]), "+f"(x[48]), "+f"(x[49]), "+f"(x[50]), "+f"(x[51]), "+f"(x[52]), "+f"(x[53]),
+                 "+f"(x[54]), "+f"(x[55]), "+f"(x[56]), "+f"(x[57]), "+f"(x[58]), "+f"(x[59]), "+f"(x[60]),
+                 "+f"(x[61]), "+f"(x[62]), "+f"(x[63]));
 }
 
 struct Tile {
@@ -260,6 +277,7 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
     const int kj = lane & 3, kt = (lane >> 3) + 4 * ((lane >> 2) & 1);
     const int vr = lane & 7, vc = (lane >> 3) & 1, vg = (lane >> 4) * (G / 2);
     const int kind = lane >> 3, np = lane & 7;
+    const unsigned k_chunk[2] = {(unsigned)((kj ^ kt) << 4), (unsigned)(((4 + kj) ^ kt) << 4)};     // of 128 swizzled bytes
     struct Words {
       unsigned k[2][G], v[4][G / 2], n[G];
     };
@@ -305,6 +323,7 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
     Words now, then;
     load(now, at);
     bool ok = true;
+#pragma unroll 2
     for (int n = own; n < records; n += CONV) {
       const int j = n / RECS, rec = n % RECS, st = j % STAGES, round = j / STAGES;
       const long long at_then = record(n + CONV, page_1);
@@ -347,27 +366,26 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
 #pragma unroll
         for (int g = 0; g < G; ++g) dst[g] = half[g];
       }
-      if (lane == 0) ok = ok && mbar_wait(&empty[st], (round & 1) ^ 1, err);
-      __syncwarp();
+      ok = ok && mbar_wait(&empty[st], (round & 1) ^ 1, err);
       if (lane == 0) key_unit[st][rec] = seen ? pow2(e) : -1.f;
       if (lane == 16) value_exp[st][rec] = e;
       // ---- keys
-      unsigned char* kd = Ks + st * T_BYTES;
+      // (a record that is not seen, or a place without a key, has numbers that are zero, whatever its codes)
+      unsigned char* kd = Ks + st * T_BYTES + rec * (REC_TOKENS * 128) + kt * 128;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int t = kt + 8 * i, row = rec * REC_TOKENS + t;
         unsigned sc[G], lo[G];
-        words<G>(sc, kn + t * G);
-        words<G>(lo, kn + 16 * G + t * G);
+        words<G>(sc, kn + (kt + 8 * i) * G);
+        words<G>(lo, kn + 16 * G + (kt + 8 * i) * G);
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          unsigned x[4] = {};
-          if (seen) four_pairs(kw[i][g], sc[g], lo[g], x);
-          *reinterpret_cast<uint4*>(kd + (g >> 1) * (BN * 128) + swizzled(row, 4 * (g & 1) + kj)) = make_uint4(x[0], x[1], x[2], x[3]);
+          unsigned x[4];
+          four_pairs(kw[i][g], sc[g], lo[g], x);
+          *reinterpret_cast<uint4*>(kd + (g >> 1) * (BN * 128) + i * 1024 + k_chunk[g & 1]) = make_uint4(x[0], x[1], x[2], x[3]);
         }
       }
       // ---- values
-      unsigned char* vd = Vs + st * T_BYTES;
+      unsigned char* vd = Vs + st * T_BYTES + (32 * vg + vr) * 128 + (((2 * rec + vc) ^ vr) << 4);
       unsigned sc[4][G / 2], lo[4][G / 2];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -376,14 +394,12 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
       }
 #pragma unroll
       for (int g = 0; g < G / 2; ++g) {
-        unsigned x[4][4] = {};                         // [pair][i]
-        if (seen) {
+        unsigned x[4][4];                              // [pair][i]
 #pragma unroll
-          for (int i = 0; i < 4; ++i) four_pairs(vw[i][g], sc[i][g], lo[i][g], x[i]);
-        }
+        for (int i = 0; i < 4; ++i) four_pairs(vw[i][g], sc[i][g], lo[i][g], x[i]);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<uint4*>(vd + swizzled(32 * (vg + g) + 8 * i + vr, 2 * rec + vc)) = make_uint4(x[0][i], x[1][i], x[2][i], x[3][i]);
+          *reinterpret_cast<uint4*>(vd + (32 * g + 8 * i) * 128) = make_uint4(x[0][i], x[1][i], x[2][i], x[3][i]);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
@@ -480,8 +496,11 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
       ok = ok && mbar_wait(&full[kst], (j / STAGES) & 1, err);              // complete, but for the exponents beside it
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       float s[BN];
+      auto fetch = [&]() {
 #pragma unroll
-      for (int c = 0; c < BN / 32; ++c) tmem_ld32_nowait(s_addr + st * BN + c * 32, &s[c * 32]);
+        for (int c = 0; c < BN / 32; ++c) tmem_ld32_nowait(s_addr + st * BN + c * 32, &s[c * 32]);
+      };
+      fetch();
       float unit[RECS];
       int ev[RECS];
       bool whole = ts + BN - 1 <= pos_min && ts >= low_max;
@@ -489,10 +508,36 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
       for (int g = 0; g < RECS; ++g) {
         unit[g] = key_unit[kst][g] * row_unit;
         ev[g] = value_exp[kst][g];
-        whole = whole && key_unit[kst][g] > 0.f;
+        whole = whole && unit[g] > 0.f;
       }
-      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-      if (!whole) {
+      int e_new = max(e_run, max(max(ev[0], ev[1]), max(ev[2], ev[3])));
+      float m_new = m_run, sum, most;
+      uint32_t w[BN / 2];
+      // weights from the scores, against the maximum so far; their sum, in units of 2^(m_new - ROOM), and the largest part of it
+      auto weigh = [&]() {
+        const float m_use = m_new == -INFINITY ? 0.f : m_new;
+        sum = most = 0.f;
+#pragma unroll
+        for (int g = 0; g < RECS; ++g) {
+          const float off = (float)(ROOM + ev[g] - e_new) - m_use;
+          const f32x2 unit2 = both(unit[g], unit[g]), off2 = both(off, off);
+          f32x2 part = both(0.f, 0.f);
+#pragma unroll
+          for (int i = g * 16; i < g * 16 + 16; i += 2) {
+            float x, y;
+            apart(fma2(both(s[i], s[i + 1]), unit2, off2), x, y);
+            x = ex2(x);
+            y = ex2(y);
+            part = add2(part, both(x, y));
+            w[i / 2] = h2(x, y);
+          }
+          float x, y;
+          apart(part, x, y);
+          most = fmaxf(most, x + y);
+          sum = fmaf(x + y, ex2((float)min(e_new - ev[g], 126)), sum);
+        }
+      };
+      auto masked = [&]() {
 #pragma unroll
         for (int i = 0; i < BN; ++i) {
           const int key = ts + i;
@@ -500,48 +545,38 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
         }
 #pragma unroll
         for (int g = 0; g < RECS; ++g) unit[g] = fabsf(unit[g]);
-      }
-      float mx = -INFINITY;
+      };
+      tmem_landed(s);
+      if (!whole) masked();
+      // Weights first, without a look at this tile's maximum: while no sum of 16 passes 2^15 none of them is too large for
+      // float16.  Where one does, or none was seen before, or larger values come, the maximum is found and moved (to no more
+      // than 2^8 below it) and the weights are made again: a few tiles of a row.
+      weigh();
+      float alpha = 1.f, shrink = 1.f;
+      const bool again = !(most <= 32768.f) || m_run == -INFINITY || e_new > e_run;
+      if (__any_sync(0xffffffffu, again)) {
+        fetch();
+        tmem_landed(s);
+        if (!whole) masked();
+        float mx = -INFINITY;
 #pragma unroll
-      for (int g = 0; g < RECS; ++g) {
-        float a = s[g * 16], b = s[g * 16 + 1];
+        for (int g = 0; g < RECS; ++g) {
+          float a = s[g * 16], b = s[g * 16 + 1];
 #pragma unroll
-        for (int i = 2; i < 16; i += 2) {
-          a = fmaxf(a, s[g * 16 + i]);
-          b = fmaxf(b, s[g * 16 + i + 1]);
+          for (int i = 2; i < 16; i += 2) {
+            a = fmaxf(a, s[g * 16 + i]);
+            b = fmaxf(b, s[g * 16 + i + 1]);
+          }
+          mx = fmaxf(mx, fmaxf(a, b) * unit[g]);
         }
-        mx = fmaxf(mx, fmaxf(a, b) * unit[g]);
-      }
-      // the maximum moves only when it has grown by more than 2^8; the values' unit when a larger one comes
-      const int e_new = max(e_run, max(max(ev[0], ev[1]), max(ev[2], ev[3])));
-      float m_new = fmaxf(m_run, mx);
-      if (m_run != -INFINITY && m_new - m_run <= 8.0f) m_new = m_run;
-      const float m_use = m_new == -INFINITY ? 0.f : m_new;
-      const float shrink = ex2(m_run - m_use), alpha = shrink * ex2((float)(e_run - e_new));
-      float sum = 0.f;
-#pragma unroll
-      for (int g = 0; g < RECS; ++g) {
-        const float off = (float)(ROOM + ev[g] - e_new) - m_use;
-        const f32x2 unit2 = both(unit[g], unit[g]), off2 = both(off, off);
-        f32x2 part = both(0.f, 0.f);
-#pragma unroll
-        for (int i = g * 16; i < g * 16 + 16; i += 2) {
-          apart(fma2(both(s[i], s[i + 1]), unit2, off2), s[i], s[i + 1]);
-          s[i] = ex2(s[i]);
-          s[i + 1] = ex2(s[i + 1]);
-          part = add2(part, both(s[i], s[i + 1]));
-        }
-        float a, b;
-        apart(part, a, b);
-        sum = fmaf(a + b, ex2((float)min(e_new - ev[g], 126)), sum);
+        m_new = fmaxf(m_run, mx);
+        if (m_run != -INFINITY && m_new - m_run <= 8.0f) m_new = m_run;
+        shrink = ex2(m_run - (m_new == -INFINITY ? 0.f : m_new));
+        alpha = shrink * ex2((float)(e_run - e_new));
+        weigh();
       }
       l_run = fmaf(l_run, shrink, sum);
-      {
-        uint32_t w[BN / 2];
-#pragma unroll
-        for (int i = 0; i < BN / 2; ++i) w[i] = h2(s[2 * i], s[2 * i + 1]);
-        tmem_st32_nowait(s_addr + st * BN, &w[0]);
-      }
+      tmem_st32_nowait(s_addr + st * BN, &w[0]);
       // only a rescaled output has to wait for the product before (the scores of tile j came after that of tile j - 2)
       if (j > 0 && __any_sync(0xffffffffu, m_new > m_run || e_new > e_run)) {
         ok = ok && mbar_wait(&o_ready[h], (j - 1) & 1, err);
@@ -550,10 +585,10 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
         for (int c = 0; c < D / 32; ++c) {
           float v[32];
           tmem_ld32(o_addr + c * 32, v);
-          uint32_t w[32];
+          uint32_t x[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i] * alpha);
-          tmem_st32_nowait(o_addr + c * 32, w);
+          for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(v[i] * alpha);
+          tmem_st32_nowait(o_addr + c * 32, x);
         }
       }
       m_run = m_new;
