@@ -149,6 +149,7 @@ __device__ __forceinline__ void tmem_landed(float (&x)[BN]) {
 
 struct Tile {
   int req, row_tile, index;    // index: among all row tiles; req < 0: none
+  int rows, start, seq;        // the request's
 };
 // the row tile that a block works on, found by every warp for itself
 __device__ __forceinline__ Tile tile_of(const Kv4AttnParams& p, int most_packed, int target) {
@@ -156,9 +157,12 @@ __device__ __forceinline__ Tile tile_of(const Kv4AttnParams& p, int most_packed,
   int before = 0;
   for (int r0 = 0; r0 < p.requests; r0 += 32) {
     const int r = r0 + lane;
-    int n = 0;
+    int n = 0, rows = 0, start = 0, seq = 0;
     if (r < p.requests) {
-      const long long packed = (long long)max(0, p.q_len[r]) * G;
+      rows = max(0, p.q_len[r]);
+      start = p.q_start[r];
+      seq = max(0, p.seq_len[r]);
+      const long long packed = (long long)rows * G;
       n = packed > most_packed ? (int)((packed + BM - 1) / BM) : 0;
     }
     int end = n;
@@ -173,11 +177,12 @@ __device__ __forceinline__ Tile tile_of(const Kv4AttnParams& p, int most_packed,
       const int who = __ffs(past) - 1;
       const int n_who = __shfl_sync(0xffffffffu, n, who), end_who = __shfl_sync(0xffffffffu, end, who);
       // the last tiles of a request see the most keys: they come first
-      return {r0 + who, before + end_who - 1 - target, target};
+      return {r0 + who, before + end_who - 1 - target, target, __shfl_sync(0xffffffffu, rows, who),
+              __shfl_sync(0xffffffffu, start, who), __shfl_sync(0xffffffffu, seq, who)};
     }
     before += all;
   }
-  return {-1, 0, target};
+  return {-1, 0, target, 0, 0, 0};
 }
 
 // N words from shared memory, as wide as they come
@@ -216,7 +221,7 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
   const Tile tile = tile_of(p, sp.most_packed, blockIdx.x / sp.splits / KV);
   if (tile.req < 0) return;
   const int r = tile.req;
-  const int nq = p.q_len[r], q0 = p.q_start[r], seq = max(0, p.seq_len[r]);
+  const int nq = tile.rows, q0 = tile.start, seq = tile.seq;
   const int packed = nq * HG, pr0 = tile.row_tile * BM, rows_here = min(BM, packed - pr0);
   const int pos0 = seq - nq;
   const int pos_min = pos0 + pr0 / HG, pos_max = pos0 + (pr0 + rows_here - 1) / HG;
@@ -458,29 +463,39 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
     const bool held = row_valid && q0 >= 0 && q0 + q_row < p.rows;
     const int pos = row_valid ? pos0 + q_row : -1;
     const int lo = p.window > 0 ? pos - p.window + 1 : 0;
-    // ---- the row's queries as float16, scaled by a power of two so that the largest lies in [1, 2)
+    // ---- the warp's 32 rows of queries as float16, each scaled by a power of two so that its largest lies in [1, 2); the lanes
+    // load whole rows (a thread loading its own asks for 32 lines an instruction, and the first records wait behind them)
     float row_unit;
+    constexpr int LANES = D / 8, ROWS = 32 / LANES;    // lanes a row takes, rows an instruction
     {
-      const __nv_bfloat16* src = (const __nv_bfloat16*)p.q + ((size_t)(held ? q0 + q_row : 0) * H + head) * D;
-      uint4 w[D / 8];
-      unsigned most = 0;
+      const unsigned own = held ? (unsigned)(((size_t)(q0 + q_row) * H + head) * LANES) : 0xffffffffu;   // in 16 bytes
+      const uint4* src = (const uint4*)p.q + lane % LANES;
+      uint4 w[32 / ROWS];
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        w[c] = held ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0, 0, 0, 0);
-        most = max(most, max(max(w[c].x & 0x7fffu, (w[c].x >> 16) & 0x7fffu), max(w[c].y & 0x7fffu, (w[c].y >> 16) & 0x7fffu)));
-        most = max(most, max(max(w[c].z & 0x7fffu, (w[c].z >> 16) & 0x7fffu), max(w[c].w & 0x7fffu, (w[c].w >> 16) & 0x7fffu)));
+      for (int i = 0; i < 32 / ROWS; ++i) {
+        const unsigned from = __shfl_sync(0xffffffffu, own, i * ROWS + lane / LANES);
+        w[i] = from != 0xffffffffu ? src[from] : make_uint4(0, 0, 0, 0);
       }
-      const int e = max(-MOST_E, min(MOST_E, (int)(most >> 7) - 127));
-      const float by = pow2(-e);
-      row_unit = pow2(e) * p.scale * 1.4426950408889634f;
+      int e_row = 0;
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        const unsigned u[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
+      for (int i = 0; i < 32 / ROWS; ++i) {
+        const unsigned u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+        unsigned most = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) most = max(most, max(u[k] & 0x7fffu, (u[k] >> 16) & 0x7fffu));
+#pragma unroll
+        for (int o = 1; o < LANES; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+        const int e = max(-MOST_E, min(MOST_E, (int)(most >> 7) - 127));
+        const int e_there = __shfl_sync(0xffffffffu, e, lane % ROWS * LANES);
+        if (lane / ROWS == i) e_row = e_there;
+        const float by = pow2(-e);
         unsigned x[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = h2(__uint_as_float(u[i] << 16) * by, __uint_as_float(u[i] & 0xffff0000u) * by);
-        *reinterpret_cast<uint4*>(Qs + h * (HALF * D * 2) + (c >> 3) * (HALF * 128) + swizzled(row & (HALF - 1), c & 7)) = make_uint4(x[0], x[1], x[2], x[3]);
+        for (int k = 0; k < 4; ++k) x[k] = h2(__uint_as_float(u[k] << 16) * by, __uint_as_float(u[k] & 0xffff0000u) * by);
+        const int to = (warp & 3) * 32 + i * ROWS + lane / LANES, c = lane % LANES;
+        *reinterpret_cast<uint4*>(Qs + h * (HALF * D * 2) + (c >> 3) * (HALF * 128) + swizzled(to, c & 7)) = make_uint4(x[0], x[1], x[2], x[3]);
       }
+      row_unit = pow2(e_row) * p.scale * 1.4426950408889634f;
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full[h]);
@@ -607,6 +622,21 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
     const float back = n_tiles > 0 ? pow2(e_run) : 0.f;
     const float inv = sp.splits > 1 ? back : l_run > 0.f ? back / l_run : l_run == 0.f ? 0.f : l_run;
     const size_t part = ((size_t)tile.index * KV + kvh) * sp.splits + split;
+    // rows are stored whole too, through shared memory that held queries (no product of this half reads them any more)
+    unsigned char* stage = Qs + h * (HALF * D * 2) + (warp & 3) * (32 * D * 2);        // [32 rows][LANES chunks of 16 bytes]
+    auto place = [&](int to, int c) { return stage + (to * LANES + (c ^ (to & 7))) * 16; };
+    const unsigned own = held ? (unsigned)(((size_t)(q0 + q_row) * H + head) * LANES) : 0xffffffffu;
+    auto flush = [&](auto store) {
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 32 / ROWS; ++i) {
+        const int to = i * ROWS + lane / LANES, c = lane % LANES;
+        const unsigned at = __shfl_sync(0xffffffffu, own, to);
+        const uint4 x = *reinterpret_cast<const uint4*>(place(to, c));
+        if (at != 0xffffffffu) store(to, c, at, x);
+      }
+      __syncwarp();
+    };
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       float v[32];
@@ -617,30 +647,36 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
         for (int i = 0; i < 32; ++i) v[i] = 0.f;
       }
       // column 8 i + r is channel 4 r + i
-      if (held && sp.splits == 1) {
-        __nv_bfloat16* dst = (__nv_bfloat16*)p.out + ((size_t)(q0 + q_row) * H + head) * D + g * 32;
+      if (sp.splits == 1) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           unsigned w[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int r8 = 2 * c + (k >> 1), i = 2 * (k & 1);
-            const __nv_bfloat162 h = __floats2bfloat162_rn(v[8 * i + r8] * inv, v[8 * (i + 1) + r8] * inv);
-            w[k] = *reinterpret_cast<const unsigned*>(&h);
+            const __nv_bfloat162 x = __floats2bfloat162_rn(v[8 * i + r8] * inv, v[8 * (i + 1) + r8] * inv);
+            w[k] = *reinterpret_cast<const unsigned*>(&x);
           }
-          reinterpret_cast<uint4*>(dst)[c] = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4*>(place(lane, 4 * g + c)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
-      } else if (held) {
-        float* dst = sp.part_o + (part * BM + row) * D + g * 32;
+      } else {
 #pragma unroll
         for (int r8 = 0; r8 < 8; ++r8)
-          reinterpret_cast<float4*>(dst)[r8] = make_float4(v[r8] * inv, v[8 + r8] * inv, v[16 + r8] * inv, v[24 + r8] * inv);
-        if (g == 0) {
-          sp.part_ml[(part * BM + row) * 2] = m_run;
-          sp.part_ml[(part * BM + row) * 2 + 1] = l_run;
+          *reinterpret_cast<float4*>(place(lane, (8 * g + r8) % LANES)) =
+              make_float4(v[r8] * inv, v[8 + r8] * inv, v[16 + r8] * inv, v[24 + r8] * inv);
+        if (g % (G / 2) == G / 2 - 1) {                // half of the channels are there
+          const int first = g / (G / 2) * LANES;
+          flush([&](int to, int c, unsigned, uint4 x) {
+            reinterpret_cast<uint4*>(sp.part_o + (part * BM + (row - lane) + to) * D)[first + c] = x;
+          });
         }
       }
-      __syncwarp();
+    }
+    if (sp.splits == 1) {
+      flush([&](int, int c, unsigned at, uint4 x) { ((uint4*)p.out)[(size_t)at + c] = x; });
+    } else if (held) {
+      sp.part_ml[(part * BM + row) * 2] = m_run;
+      sp.part_ml[(part * BM + row) * 2 + 1] = l_run;
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   }
@@ -660,7 +696,7 @@ __global__ void __launch_bounds__(256) kv4_tc5_merge_kernel(Kv4AttnParams p, Tc5
   const int KV = p.kv_heads, H = p.heads, HG = H / KV, kvh = blockIdx.x % KV;
   const Tile tile = tile_of(p, sp.most_packed, blockIdx.x / KV);
   if (tile.req < 0) return;
-  const int packed = p.q_len[tile.req] * HG, q0 = p.q_start[tile.req], lane = threadIdx.x & 31;
+  const int packed = tile.rows * HG, q0 = tile.start, lane = threadIdx.x & 31;
   for (int row = blockIdx.y * 8 + (threadIdx.x >> 5); row < BM; row += gridDim.y * 8) {
     const int pr = tile.row_tile * BM + row, q_row = pr / HG;
     if (pr >= packed || q0 < 0 || q0 + q_row >= p.rows) return;

@@ -2928,7 +2928,8 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, q_sta
     if most_packed != 0x7fffffff:
         # row tiles of 256: at most one of each request is not full
         tiles = T * group // 256 + min(R, T * group // (most_packed + 1))
-        splits = max(1, min(multiprocessors(q.device) // (tiles * KV), -(-most_keys // KV4_SPLIT_KEYS), KV4_MOST_SPLITS))
+        busy = -(-T * group // 256) * KV
+        splits = max(1, min(multiprocessors(q.device) // busy, -(-most_keys // KV4_SPLIT_KEYS), KV4_MOST_SPLITS))
         work = torch.empty(tiles * KV * splits * 256 * (head_dim + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
         fn = _fn("kv4_attention_tc5", "pbe_kv4_attention_tc5", [ctypes.POINTER(Kv4AttnParams), c_void_p] + [c_int] * 4 + [c_void_p] * 2)
         _check(fn(params, _ptr(work), tiles, splits, head_dim, most_packed, _ptr(tc5_attention_error_buffer(q.device)), stream),
