@@ -34,10 +34,16 @@ using namespace pbe::kv4;
 using namespace pbe::mma_sync;
 
 namespace {
+struct Shared {                // an item that several blocks share, as the block that begins it notes it
+  int parts, slot;             // parts: 0: none.  The first part's slot; the others' are 2 (block + 1), 2 (block + 2), ...
+  int rows, q_start;           // its packed rows (at most a tile's) and the query row of the first
+  int head, first;             // first head of its key/value head; packed row of the first, within the request
+  int pad[2];
+};
 struct Split {
   float* part_o;               // [2 blocks][rows of a tile][D]
   float* part_ml;              // [2 blocks][rows of a tile][2]
-  long long* ends;             // [1 + requests]: units a block, then where each request's units end
+  Shared* shared;              // [blocks]
   int most_packed;             // requests of more packed rows are another kernel's
 };
 
@@ -65,15 +71,6 @@ __device__ __forceinline__ Request request(const Kv4AttnParams& p, const Split& 
   q.first = low / REC_TOKENS;
   q.tiles = max(1, (int)(((unsigned)q.seq + REC_TOKENS - 1) / REC_TOKENS) - q.first);
   return q;
-}
-// the first request whose units end behind `unit`
-__device__ __forceinline__ int find(const long long* ends, int requests, long long unit) {
-  int lo = 0, hi = requests;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (ends[mid] > unit) hi = mid; else lo = mid + 1;
-  }
-  return lo;
 }
 // a / b, a not negative: almost always in 32 bits, where a division is a tenth of one in 64
 __device__ __forceinline__ long long quotient(long long a, int b) {
@@ -142,23 +139,26 @@ template <typename T, int D, int NT, int TERMS>
 __global__ void __launch_bounds__(WARPS * 32, (TERMS == 1 && (NT == 1 || D == 64)) ? 2 : 1)
 kv4_attention_kernel(Kv4AttnParams p, Split sp) {
   constexpr int G = D / GROUP, REC = rec_bytes(D), MT = 8 * NT, RING = WARPS * STAGES * REC;
-  constexpr int MERGE = WARPS * MT * (D + 2) * 4;
+  constexpr int MERGE = WARPS * MT * (D + 2 + G) * 4;
   constexpr int SHARED = RING > MERGE ? RING : MERGE;
   extern __shared__ __align__(16) unsigned char smem[];
-  long long* ends = reinterpret_cast<long long*>(smem + SHARED);
+  long long* ends = reinterpret_cast<long long*>(smem + SHARED);     // where each request's units end
+  int4* known = reinterpret_cast<int4*>(ends + (p.requests + 1) / 2 * 2);      // its q_len, seq_len, q_start
   __shared__ long long warp_sums[WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r8 = lane >> 2, j = lane & 3;
   const int H = p.heads, KV = p.kv_heads, HG = H / KV, per_page = p.page_tokens / REC_TOKENS;
   const int page_shift = (per_page & (per_page - 1)) == 0 ? 31 - __clz(per_page) : -1;
   pdl_wait();
 
-  // where each request's units end (a unit: one tile of 16 keys for one head and row tile)
+  // a unit: one tile of 16 keys for one head and row tile
   long long total = 0;
   for (int r0 = 0; r0 < p.requests; r0 += WARPS * 32) {
     const int r = r0 + threadIdx.x;
     long long v = 0;
     if (r < p.requests) {
-      const Request q = request(p, sp, p.q_len[r], p.seq_len[r], MT);
+      const int4 x = make_int4(p.q_len[r], p.seq_len[r], p.q_start[r], 0);
+      known[r] = x;
+      const Request q = request(p, sp, x.x, x.y, MT);
       v = (long long)q.tiles * q.row_tiles * KV;
     }
 #pragma unroll
@@ -178,27 +178,32 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
     __syncthreads();
   }
   const long long per_block = max((long long)MIN_UNITS, quotient(total + gridDim.x - 1, gridDim.x));
-  if (blockIdx.x == 0) {
-    for (int r = threadIdx.x; r < p.requests; r += WARPS * 32) sp.ends[1 + r] = ends[r];
-    if (threadIdx.x == 0) sp.ends[0] = per_block;
-  }
   pdl_launch_dependents();
   const float to_log2 = p.scale * 1.4426950408889634f * CODE;
 
   unsigned char* ring = smem + warp * STAGES * REC;
   long long unit = per_block * blockIdx.x;
   const long long unit0 = unit, unit_end = min(unit + per_block, total);
+  Shared note = {};
   while (unit < unit_end) {
     // ---- the next item, or this block's part of it
-    const int req = find(ends, p.requests, unit);
-    const Request q = request(p, sp, p.q_len[req], p.seq_len[req], MT);
+    int req = 0;                                       // the first request whose units end behind this one
+    for (;; req += 32) {
+      const unsigned past = __ballot_sync(0xffffffffu, req + lane < p.requests && ends[req + lane] > unit);
+      if (past != 0) {
+        req += __ffs(past) - 1;
+        break;
+      }
+    }
+    const int4 given = known[req];
+    const Request q = request(p, sp, given.x, given.y, MT);
     const long long begin = req > 0 ? ends[req - 1] : 0;
     const int item = (int)quotient(unit - begin, q.tiles);
     const int t_begin = (int)((unit - begin) - (long long)item * q.tiles);
     const int t_end = (int)min((long long)q.tiles, t_begin + (unit_end - unit));
     const int kvh = q.row_tiles == 1 ? item : item / q.row_tiles, row_tile = item - kvh * q.row_tiles;
     const int packed = q.rows * HG, pr0 = row_tile * MT;
-    const int q0 = p.q_start[req];
+    const int q0 = given.z;
     auto row_of = [&](int pr) { return q.rows == 1 ? 0 : pr / HG; };     // the request's row of a packed one
     const int pos_min = q.pos0 + row_of(pr0), pos_max = q.pos0 + row_of(min(pr0 + MT, packed) - 1);
     const int low_min = p.window > 0 ? pos_min - p.window + 1 : 0, low_max = p.window > 0 ? pos_max - p.window + 1 : 0;
@@ -471,16 +476,30 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
     float* mm = om + WARPS * MT * D;                   // [warp][row]
     float* lm = mm + WARPS * MT;
     constexpr float even = TERMS == 1 ? CODE16 : CODE, odd = even / 16.f, down = TERMS == 1 ? 1.f : 1.f / UP;
+    float* zm = lm + WARPS * MT;                       // [warp][row][G]
 #pragma unroll
     for (int k = 0; k < NT; ++k) {
+      // the sums over the keys' lanes of the values' lo: by halves, so that lane r8 is left with one of the 2 G sums (two
+      // lanes with the same one where there are four)
+      float v[2 * G];
+#pragma unroll
+      for (int i = 0; i < 2 * G; ++i) v[i] = z[k][i >> 1][i & 1];
+#pragma unroll
+      for (int n = G, off = 16; n > 0; n >>= 1, off >>= 1) {
+        const bool up = lane & off;
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+          const float other = __shfl_xor_sync(0xffffffffu, up ? v[i] : v[n + i], off);
+          v[i] = (up ? v[n + i] : v[i]) + other;
+        }
+      }
+      if (G == 2) v[0] += __shfl_xor_sync(0xffffffffu, v[0], 4);
+      const int which = G == 4 ? r8 : r8 >> 1;
+      zm[(warp * MT + 8 * k + 2 * j + (which & 1)) * G + (which >> 1)] = v[0] * down;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
-        for (int off = 4; off < 32; off <<= 1) {
-          l[k][e] += __shfl_xor_sync(0xffffffffu, l[k][e], off);
-#pragma unroll
-          for (int g = 0; g < G; ++g) z[k][g][e] += __shfl_xor_sync(0xffffffffu, z[k][g][e], off);
-        }
+        for (int off = 4; off < 32; off <<= 1) l[k][e] += __shfl_xor_sync(0xffffffffu, l[k][e], off);
         const int row = warp * MT + 8 * k + 2 * j + e;
         if (r8 == 0) {
           mm[row] = TERMS == 1 ? m[k][e] + (float)(e_run - ROOM) : m[k][e];
@@ -488,15 +507,18 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          const float(&a)[4] = o[k][2 * g], (&b)[4] = o[k][2 * g + 1], lean = z[k][g][e] * down;
-          *reinterpret_cast<float4*>(om + row * D + 32 * g + 4 * r8) =
-              make_float4(fmaf(a[e], even, lean), fmaf(a[2 + e], odd, lean), fmaf(b[e], even, lean), fmaf(b[2 + e], odd, lean));
+          const float(&a)[4] = o[k][2 * g], (&b)[4] = o[k][2 * g + 1];
+          *reinterpret_cast<float4*>(om + row * D + 32 * g + 4 * r8) = make_float4(a[e] * even, a[2 + e] * odd, b[e] * even, b[2 + e] * odd);
         }
       }
     }
     __syncthreads();
     const bool whole = t_begin == 0 && t_end == q.tiles;
     const int slot = 2 * blockIdx.x + (unit == unit0 ? 0 : 1);
+    if (t_begin == 0 && !whole) {
+      const int last = (int)quotient(unit + q.tiles - 1, (int)per_block);
+      note = {last - (int)blockIdx.x + 1, slot, min(MT, packed - pr0), q0, kvh * HG, pr0, {0, 0}};
+    }
     for (int e = threadIdx.x; e < MT * (D / 4); e += WARPS * 32) {
       const int row = e / (D / 4), c4 = (e % (D / 4)) * 4, pr = pr0 + row;
       float top = -INFINITY;
@@ -507,10 +529,12 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
-        const float f = exp2f(mm[w * MT + row] - base);
+        const float f = TERMS == 1 ? ex2(mm[w * MT + row] - base) : exp2f(mm[w * MT + row] - base);
         const float4 y = *reinterpret_cast<const float4*>(om + (w * MT + row) * D + c4);
+        const float lean = zm[(w * MT + row) * G + c4 / GROUP];
         sum = fmaf(f, lm[w * MT + row], sum);
-        x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
+        x.x = fmaf(f, y.x + lean, x.x), x.y = fmaf(f, y.y + lean, x.y);
+        x.z = fmaf(f, y.z + lean, x.z), x.w = fmaf(f, y.w + lean, x.w);
       }
       if (!whole) {
         const size_t at = (size_t)slot * MT + row;
@@ -526,11 +550,12 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
     __syncthreads();                                   // the merged parts are read before the ring is filled again
     unit += t_end - t_begin;
   }
+  if (threadIdx.x == 0) sp.shared[blockIdx.x] = note;
 }
 
-// Items that several blocks share: block b looks at the border between blocks b and b + 1 of the kernel above, and merges the
-// item that lies across it if that is the item's first border.  A warp takes one row and every PARTS-th of the item's parts
-// (one request of 32,768 keys has 74, whose loads one warp a row would wait for in turn: 53 us), eight loads on their way.
+// Items that several blocks share: block b merges the one that block b of the kernel above began and did not end.  A warp
+// takes one row and every PARTS-th of the item's parts (one request of 32,768 keys has 74, whose loads one warp a row would
+// wait for in turn: 53 us), eight loads on their way.
 constexpr int MERGE_WARPS = 16;
 
 template <typename T, int D, int MT>
@@ -539,26 +564,14 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) kv4_merge_kernel(Kv4AttnPara
   __shared__ float held[PARTS > 1 ? PARTS : 1][MT][D], held_m[MERGE_WARPS], held_l[MERGE_WARPS];
   pdl_launch_dependents();
   pdl_wait();
-  const long long per_block = sp.ends[0];
-  const long long* ends = sp.ends + 1;
-  const long long border = per_block * (blockIdx.x + 1);
-  if (border >= ends[p.requests - 1]) return;
-  const int req = find(ends, p.requests, border);
-  const Request q = request(p, sp, p.q_len[req], p.seq_len[req], MT);
-  const long long begin = req > 0 ? ends[req - 1] : 0;
-  const int item = (int)quotient(border - begin, q.tiles);
-  const long long first = begin + (long long)item * q.tiles, last = first + q.tiles;
-  if (first == border || first < border - per_block) return;
-  const int H = p.heads, KV = p.kv_heads, HG = H / KV, kvh = item / q.row_tiles, row_tile = item - kvh * q.row_tiles;
-  const int q0 = p.q_start[req], packed = q.rows * HG;
-  const int b0 = blockIdx.x, b1 = (int)((last - 1) / per_block);
+  const Shared item = sp.shared[blockIdx.x];
+  if (item.parts == 0) return;
+  const int H = p.heads, HG = H / p.kv_heads, last = item.parts - 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = warp % MT, part = warp / MT;
-  // a block's first segment is in its slot 0: every block's but perhaps the first one's
-  const int slot0 = 2 * b0 + (per_block * b0 >= first ? 0 : 1);
-  auto slot = [&](int b) { return (size_t)(b == b0 ? slot0 : 2 * b) * MT + row; };
+  auto slot = [&](int i) { return (size_t)(i == 0 ? item.slot : 2 * ((int)blockIdx.x + i)) * MT + row; };
   float top = -INFINITY, sum = 0.f, x[C] = {};
-  for (int b = b0 + part; b <= b1; b += PARTS * 32) {              // 32 of the warp's parts at a time
-    const int n = min(32, (b1 - b) / PARTS + 1);
+  for (int b = part; b <= last; b += PARTS * 32) {                 // 32 of the warp's parts at a time
+    const int n = min(32, (last - b) / PARTS + 1);
     const float m = lane < n ? sp.part_ml[slot(b + lane * PARTS) * 2] : -INFINITY;
     const float l = lane < n ? sp.part_ml[slot(b + lane * PARTS) * 2 + 1] : 0.f;
     const float now = fmaxf(top, warp_max(m)), base = now == -INFINITY ? 0.f : now;
@@ -600,10 +613,10 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) kv4_merge_kernel(Kv4AttnPara
       for (int c = 0; c < C; ++c) x[c] = fmaf(f, held[o][row][C * lane + c], x[c]);
     }
   }
-  const int pr = row_tile * MT + row, at = q.rows == 1 ? 0 : pr / HG;
-  if (pr >= packed || q0 < 0 || q0 + at >= p.rows) return;
+  const int pr = item.first + row, at = pr / HG, q0 = item.q_start;
+  if (row >= item.rows || q0 < 0 || q0 + at >= p.rows) return;
   const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-  T* dst = (T*)p.out + ((size_t)(q0 + at) * H + kvh * HG + (pr - at * HG)) * D + C * lane;
+  T* dst = (T*)p.out + ((size_t)(q0 + at) * H + item.head + (pr - at * HG)) * D + C * lane;
 #pragma unroll
   for (int c = 0; c < C; c += 2) {
     if constexpr (sizeof(T) == 2) *reinterpret_cast<unsigned*>(dst + c) = pack2(x[c] * inv, x[c + 1] * inv);
@@ -613,8 +626,8 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) kv4_merge_kernel(Kv4AttnPara
 
 template <typename T, int D, int NT, int TERMS>
 int launch(const Kv4AttnParams& p, const Split& sp, int blocks, cudaStream_t stream) {
-  constexpr int MT = 8 * NT, ring = WARPS * STAGES * rec_bytes(D), merge = WARPS * MT * (D + 2) * 4;
-  const size_t smem = (ring > merge ? ring : merge) + (size_t)p.requests * sizeof(long long);
+  constexpr int MT = 8 * NT, ring = WARPS * STAGES * rec_bytes(D), merge = WARPS * MT * (D + 2 + D / GROUP) * 4;
+  const size_t smem = (ring > merge ? ring : merge) + (size_t)(p.requests + 1) / 2 * 2 * sizeof(long long) + (size_t)p.requests * sizeof(int4);
   static OptIn opt_in;
   if (const cudaError_t e = opt_in(smem, kv4_attention_kernel<T, D, NT, TERMS>)) return (int)e;
   launch_k(kv4_attention_kernel<T, D, NT, TERMS>, blocks, WARPS * 32, smem, stream, p, sp);
@@ -624,7 +637,7 @@ int launch(const Kv4AttnParams& p, const Split& sp, int blocks, cudaStream_t str
 
 }  // namespace
 
-// workspace: 2 (1 + requests) floats, rounded up to four, then 2 blocks * tile rows * (head_dim + 2).  tile_rows: 8, or 16
+// workspace: 8 floats a block, then 2 blocks * tile rows * (head_dim + 2).  tile_rows: 8, or 16
 // (bfloat16); requests of more than most_packed packed rows are left out.
 PBE_EXPORT int pbe_kv4_attention(const Kv4AttnParams* params, float* workspace, int blocks, int head_dim, int tile_rows,
                                  int most_packed, int dtype, cudaStream_t stream) {
@@ -634,8 +647,8 @@ PBE_EXPORT int pbe_kv4_attention(const Kv4AttnParams* params, float* workspace, 
       !(tile_rows == 8 || (tile_rows == 16 && dtype == PBE_BF16)))
     return (int)cudaErrorInvalidValue;
   Split sp;
-  sp.ends = reinterpret_cast<long long*>(workspace);
-  sp.part_o = workspace + ((2 * (1 + p.requests) + 3) & ~3);
+  sp.shared = reinterpret_cast<Shared*>(workspace);
+  sp.part_o = workspace + (size_t)blocks * (sizeof(Shared) / sizeof(float));
   sp.part_ml = sp.part_o + (size_t)2 * blocks * tile_rows * head_dim;
   sp.most_packed = most_packed;
   if (dtype == PBE_F32)

@@ -2921,7 +2921,7 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, q_sta
     if most_packed:
         rows = min(most_rows, max(1, most_packed // group))
         tile_rows, blocks = _kv4_shape(R, H, KV, head_dim, rows, most_keys, bf16, multiprocessors(q.device))
-        floats = (2 * (1 + R) + 3) // 4 * 4 + 2 * blocks * tile_rows * (head_dim + 2)
+        floats = 8 * blocks + 2 * blocks * tile_rows * (head_dim + 2)
         work = torch.empty(floats, dtype=torch.float32, device=q.device)
         fn = _fn("kv4_attention", "pbe_kv4_attention", [ctypes.POINTER(Kv4AttnParams), c_void_p] + [c_int] * 5 + [c_void_p])
         _check(fn(params, _ptr(work), blocks, head_dim, tile_rows, most_packed, dtype, stream), "kv4_attention")
