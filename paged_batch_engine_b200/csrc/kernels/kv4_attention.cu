@@ -558,16 +558,17 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
 // wait for in turn: 53 us), eight loads on their way.
 constexpr int MERGE_WARPS = 16;
 
-template <typename T, int D, int MT>
+template <typename T, int D, int MT, int ROWS>         // MT rows a tile, ROWS of them a block
 __global__ void __launch_bounds__(MERGE_WARPS * 32) kv4_merge_kernel(Kv4AttnParams p, Split sp) {
-  constexpr int PARTS = MERGE_WARPS / MT, C = D / 32;  // C: columns a lane
-  __shared__ float held[PARTS > 1 ? PARTS : 1][MT][D], held_m[MERGE_WARPS], held_l[MERGE_WARPS];
+  constexpr int PARTS = MERGE_WARPS / ROWS, C = D / 32;  // C: columns a lane
+  __shared__ float held[PARTS > 1 ? PARTS : 1][ROWS][D], held_m[MERGE_WARPS], held_l[MERGE_WARPS];
   pdl_launch_dependents();
   pdl_wait();
   const Shared item = sp.shared[blockIdx.x];
   if (item.parts == 0) return;
   const int H = p.heads, HG = H / p.kv_heads, last = item.parts - 1;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = warp % MT, part = warp / MT;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, in_block = warp % ROWS, part = warp / ROWS;
+  const int row = blockIdx.y * ROWS + in_block;
   auto slot = [&](int i) { return (size_t)(i == 0 ? item.slot : 2 * ((int)blockIdx.x + i)) * MT + row; };
   float top = -INFINITY, sum = 0.f, x[C] = {};
   for (int b = part; b <= last; b += PARTS * 32) {                 // 32 of the warp's parts at a time
@@ -594,23 +595,23 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) kv4_merge_kernel(Kv4AttnPara
   }
   if (PARTS > 1) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) held[part][row][C * lane + c] = x[c];
+    for (int c = 0; c < C; ++c) held[part][in_block][C * lane + c] = x[c];
     if (lane == 0) held_m[warp] = top, held_l[warp] = sum;
     __syncthreads();
     if (part > 0) return;
     float most = top;
 #pragma unroll
-    for (int o = 1; o < PARTS; ++o) most = fmaxf(most, held_m[o * MT + row]);
+    for (int o = 1; o < PARTS; ++o) most = fmaxf(most, held_m[o * ROWS + in_block]);
     const float base = most == -INFINITY ? 0.f : most, own = exp2f(top - base);
     sum *= own;
 #pragma unroll
     for (int c = 0; c < C; ++c) x[c] *= own;
 #pragma unroll
     for (int o = 1; o < PARTS; ++o) {
-      const float f = exp2f(held_m[o * MT + row] - base);
-      sum = fmaf(f, held_l[o * MT + row], sum);
+      const float f = exp2f(held_m[o * ROWS + in_block] - base);
+      sum = fmaf(f, held_l[o * ROWS + in_block], sum);
 #pragma unroll
-      for (int c = 0; c < C; ++c) x[c] = fmaf(f, held[o][row][C * lane + c], x[c]);
+      for (int c = 0; c < C; ++c) x[c] = fmaf(f, held[o][in_block][C * lane + c], x[c]);
     }
   }
   const int pr = item.first + row, at = pr / HG, q0 = item.q_start;
@@ -625,13 +626,15 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) kv4_merge_kernel(Kv4AttnPara
 }
 
 template <typename T, int D, int NT, int TERMS>
-int launch(const Kv4AttnParams& p, const Split& sp, int blocks, cudaStream_t stream) {
+int launch(const Kv4AttnParams& p, const Split& sp, int blocks, bool few_items, cudaStream_t stream) {
   constexpr int MT = 8 * NT, ring = WARPS * STAGES * rec_bytes(D), merge = WARPS * MT * (D + 2 + D / GROUP) * 4;
   const size_t smem = (ring > merge ? ring : merge) + (size_t)(p.requests + 1) / 2 * 2 * sizeof(long long) + (size_t)p.requests * sizeof(int4);
   static OptIn opt_in;
   if (const cudaError_t e = opt_in(smem, kv4_attention_kernel<T, D, NT, TERMS>)) return (int)e;
   launch_k(kv4_attention_kernel<T, D, NT, TERMS>, blocks, WARPS * 32, smem, stream, p, sp);
-  if (blocks > 1) launch_k(kv4_merge_kernel<T, D, MT>, blocks - 1, MERGE_WARPS * 32, 0, stream, p, sp);
+  // few items in many parts (a long context alone in its step): a quarter of an item's rows a block, four times the warps a row
+  if (blocks > 1 && few_items) launch_k(kv4_merge_kernel<T, D, MT, MT / 4>, dim3(blocks - 1, 4), MERGE_WARPS * 32, 0, stream, p, sp);
+  else if (blocks > 1) launch_k(kv4_merge_kernel<T, D, MT, MT>, blocks - 1, MERGE_WARPS * 32, 0, stream, p, sp);
   return launch_status();
 }
 
@@ -651,10 +654,11 @@ PBE_EXPORT int pbe_kv4_attention(const Kv4AttnParams* params, float* workspace, 
   sp.part_o = workspace + (size_t)blocks * (sizeof(Shared) / sizeof(float));
   sp.part_ml = sp.part_o + (size_t)2 * blocks * tile_rows * head_dim;
   sp.most_packed = most_packed;
+  const bool few_items = (long long)p.requests * p.kv_heads * 8 <= blocks;
   if (dtype == PBE_F32)
-    return head_dim == 64 ? launch<float, 64, 1, 3>(p, sp, blocks, stream) : launch<float, 128, 1, 3>(p, sp, blocks, stream);
+    return head_dim == 64 ? launch<float, 64, 1, 3>(p, sp, blocks, few_items, stream) : launch<float, 128, 1, 3>(p, sp, blocks, few_items, stream);
   typedef __nv_bfloat16 B;
   if (tile_rows == 8)
-    return head_dim == 64 ? launch<B, 64, 1, 1>(p, sp, blocks, stream) : launch<B, 128, 1, 1>(p, sp, blocks, stream);
-  return head_dim == 64 ? launch<B, 64, 2, 1>(p, sp, blocks, stream) : launch<B, 128, 2, 1>(p, sp, blocks, stream);
+    return head_dim == 64 ? launch<B, 64, 1, 1>(p, sp, blocks, few_items, stream) : launch<B, 128, 1, 1>(p, sp, blocks, few_items, stream);
+  return head_dim == 64 ? launch<B, 64, 2, 1>(p, sp, blocks, few_items, stream) : launch<B, 128, 2, 1>(p, sp, blocks, few_items, stream);
 }
