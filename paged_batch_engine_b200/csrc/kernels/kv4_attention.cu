@@ -47,9 +47,9 @@ struct Split {
   int most_packed;             // requests of more packed rows are another kernel's
 };
 
-constexpr int WARPS = 8;
+constexpr int WARPS = 4;
 constexpr int STAGES = 4;
-constexpr int MIN_UNITS = 16;  // tiles a block takes at least: two a warp
+constexpr int MIN_UNITS = 8;   // tiles a block takes at least: two a warp
 constexpr int MOST_REQUESTS = 8192;
 constexpr float UP = 18446744073709551616.f;           // 2^64
 constexpr float CODE = 590295810358705651712.f;        // 2^69 = 2^133 / 2^64: products of bfloat16 codes
@@ -136,7 +136,7 @@ __device__ __forceinline__ void words(unsigned (&w)[N], const unsigned char* p) 
 
 // T: the queries' type; NT: tiles of eight packed rows a warp; TERMS: bfloat16 terms of queries and weights
 template <typename T, int D, int NT, int TERMS>
-__global__ void __launch_bounds__(WARPS * 32, (TERMS == 1 && (NT == 1 || D == 64)) ? 2 : 1)
+__global__ void __launch_bounds__(WARPS * 32, (TERMS == 1 && (NT == 1 || D == 64)) ? 4 : 2)
 kv4_attention_kernel(Kv4AttnParams p, Split sp) {
   constexpr int G = D / GROUP, REC = rec_bytes(D), MT = 8 * NT, RING = WARPS * STAGES * REC;
   constexpr int MERGE = WARPS * MT * (D + 2 + G) * 4;

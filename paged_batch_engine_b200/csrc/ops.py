@@ -2864,14 +2864,14 @@ KV4_MAX_REQUESTS = 8192
 KV4_FEW_PACKED = 64         # packed rows (rows x heads of a key/value head) up to which a request is the mma.sync kernel's
 KV4_SPLIT_KEYS = 512        # keys of a split of the tcgen05 kernel at least
 KV4_MOST_SPLITS = 32
-KV4_UNITS = 16              # tiles of 16 keys a block takes at least, two a warp
+KV4_UNITS = 8               # tiles of 16 keys a block takes at least, two a warp
 
 
 def _kv4_shape(requests: int, heads: int, kv_heads: int, head_dim: int, most_rows: int, most_keys: int, wide: bool, sms: int):
     """(packed rows of a tile, blocks) of the kernel for decoded tokens and short portions: as many blocks as the GPU holds
-    at once (one a multiprocessor where a warp's registers leave no more), fewer where there is less to do."""
+    at once (two a multiprocessor where a warp's registers leave no more), fewer where there is less to do."""
     tile_rows = 16 if wide and most_rows * (heads // kv_heads) > 8 else 8
-    resident = sms * (2 if wide and (tile_rows == 8 or head_dim == 64) else 1)
+    resident = sms * (4 if wide and (tile_rows == 8 or head_dim == 64) else 2)
     row_tiles = -(-max(1, most_rows) * (heads // kv_heads) // tile_rows)
     units = requests * row_tiles * kv_heads * (-(-max(1, most_keys) // KV4_PAGE_UNIT))
     return tile_rows, max(1, min(-(-units // KV4_UNITS), resident))
