@@ -119,13 +119,15 @@ __global__ void __launch_bounds__(THREADS) page_maps_kernel(MapsParams p) {
 
 PBE_EXPORT int pbe_page_maps_most_requests() { return MOST_REQUESTS; }
 
+// out: q_start [requests], seq_len [requests], positions [rows], request_of_row [rows], slots [rows], table [requests, width],
+// each on the next multiple of four integers.
 PBE_EXPORT int pbe_page_maps(const int32_t* q_len, const int32_t* context, const int32_t* pages, long long num_pages,
-                             int32_t* q_start, int32_t* seq_len, int32_t* positions, int32_t* request_of_row, int32_t* slots,
-                             int32_t* table, int requests, int rows, int width, int page_tokens, int stride,
+                             int32_t* out, int requests, int rows, int width, int page_tokens, int stride,
                              cudaStream_t stream) {
   if (requests <= 0 || requests > MOST_REQUESTS || rows < 0 || width < 0 || page_tokens <= 0 || stride <= 0)
     return (int)cudaErrorInvalidValue;
-  MapsParams p{q_len, context, pages, q_start, seq_len, positions, request_of_row, slots, table,
+  const size_t r = ((size_t)requests + 3) / 4 * 4, n = ((size_t)rows + 3) / 4 * 4;
+  MapsParams p{q_len, context, pages, out, out + r, out + 2 * r, out + 2 * r + n, out + 2 * r + 2 * n, out + 2 * r + 3 * n,
                requests, rows, width, page_tokens, stride, num_pages};
   const size_t smem = (size_t)requests * 2 * sizeof(long long);
   static OptIn opt_in;

@@ -7,7 +7,7 @@ a CUDA device is an error, and so is a failed build of the kernel library.
 from __future__ import annotations
 
 import ctypes
-import itertools
+import functools
 import math
 import os
 from typing import NamedTuple, Optional
@@ -37,6 +37,11 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else c_void_p(t.data_ptr())
 
 
+def _at(t: Optional[torch.Tensor]):
+    """The address as a plain integer, as ctypes takes it for a pointer argument."""
+    return None if t is None else t.data_ptr()
+
+
 def _stream():
     # the raw handle of the current stream, without building a torch.cuda.Stream object per launch
     return c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
@@ -54,18 +59,24 @@ def _need_contiguous(*tensors):
             raise KernelError("kernel operands must be contiguous")
 
 
-def _need_here(what: str, *tensors):
-    """Launches go to the current device's current stream: operands of another device are refused."""
-    here = torch._C._cuda_getDevice()
+def _ready(what: str, aligned, others=()):
+    """Operands of a launch on the current stream: contiguous, on the current device, the first ones on 16-byte boundaries
+    (None stands for no operand)."""
+    tensors = [t for t in (*aligned, *others) if t is not None]
     for t in tensors:
-        if t is not None and t.device.index != here:
-            raise KernelError(f"{what}: the operands must lie on the current device (cuda:{here}), got {t.device}")
-
-
-def _need_aligned(what: str, *tensors):
-    for t in tensors:
-        if t is not None and t.data_ptr() % 16:
+        if not t.is_contiguous():
+            raise KernelError("kernel operands must be contiguous")
+    for t in aligned:
+        if t is not None and t.data_ptr() & 15:
             raise KernelError(f"{what}: operands must begin on a 16-byte boundary")
+    here = None
+    for t in tensors:
+        at = t.get_device()
+        if at != here:
+            _need_cuda(t)
+            here = torch._C._cuda_getDevice()
+            if at != here:
+                raise KernelError(f"{what}: the operands must lie on the current device (cuda:{here}), got {t.device}")
 
 
 _launches = 0
@@ -2740,6 +2751,20 @@ class PageMaps(NamedTuple):
 MAPS_MAX_REQUESTS = 8192
 
 
+@functools.lru_cache(maxsize=None)
+def _page_maps_fn():
+    return _fn("page_maps", "pbe_page_maps", [c_void_p] * 3 + [c_ll, c_void_p] + [c_int] * 5 + [c_void_p])
+
+
+@functools.lru_cache(maxsize=256)
+def _maps_pieces(requests: int, rows: int, width: int):
+    """Sizes of the arrays of ``PageMaps`` in one buffer, each with what is left to a 16-byte boundary behind it."""
+    sizes = []
+    for n in (requests, requests, rows, rows, rows, requests * width):
+        sizes += [n, -n % 4]
+    return tuple(sizes), sum(sizes)
+
+
 def page_maps(q_len: torch.Tensor, context: torch.Tensor, pages: Optional[torch.Tensor], page_tokens: int, rows: int,
               width: int, stride: int = 1) -> PageMaps:
     """Row maps and block tables of a step from its requests' lengths.  Request r brings ``q_len[r]`` rows behind
@@ -2749,8 +2774,7 @@ def page_maps(q_len: torch.Tensor, context: torch.Tensor, pages: Optional[torch.
     and the slot (page * page_tokens + place) of its entry, one entry for every ``stride`` tokens.  ``block_table`` has
     ``width`` entries a request, -1 behind its last page.  Of ``rows`` rows those behind the last request have request and
     slot -1 and position 0.  A row whose page is negative or lies behind the end of ``pages`` has slot -1.  At most
-    ``MAPS_MAX_REQUESTS`` requests."""
-    _need_contiguous(q_len, context, pages)
+    ``MAPS_MAX_REQUESTS`` requests; the arrays are views of one buffer."""
     R = q_len.numel()
     if q_len.dtype != torch.int32 or context.dtype != torch.int32 or q_len.dim() != 1 or context.shape != q_len.shape:
         raise KernelError("page_maps: q_len and context must be int32 [R]")
@@ -2760,18 +2784,16 @@ def page_maps(q_len: torch.Tensor, context: torch.Tensor, pages: Optional[torch.
         raise KernelError("page_maps: page_tokens and stride are at least 1, rows and width not negative")
     if not 1 <= R <= MAPS_MAX_REQUESTS:
         raise KernelError(f"page_maps takes 1 to {MAPS_MAX_REQUESTS} requests, got {R}")
-    sizes = [R, R, rows, rows, rows, R * width]
-    ends = list(itertools.accumulate((n + 3) // 4 * 4 for n in sizes))        # each on a 16-byte boundary
-    if ends[-1] > 0x7fffffff:
+    sizes, total = _maps_pieces(R, int(rows), int(width))
+    if total > 0x7fffffff:
         raise KernelError("page_maps: more rows or table entries than int32 counts")
-    _need_cuda(q_len, context, pages)
-    _need_here("page_maps", q_len, context, pages)
-    held = torch.empty(ends[-1], dtype=torch.int32, device=q_len.device)
-    out = [held[e - (n + 3) // 4 * 4:][:n] for e, n in zip(ends, sizes)]
-    fn = _fn("page_maps", "pbe_page_maps", [c_void_p] * 3 + [c_ll] + [c_void_p] * 6 + [c_int] * 5 + [c_void_p])
-    _check(fn(_ptr(q_len), _ptr(context), _ptr(pages), pages.numel() if pages is not None else 1 << 31,
-              *[_ptr(t) for t in out], R, int(rows), int(width), int(page_tokens), int(stride), _stream()), "page_maps")
-    return PageMaps(*out[:5], out[5].view(R, width))
+    _ready("page_maps", (), (q_len, context, pages))
+    held = q_len.new_empty(total)
+    _check(_page_maps_fn()(q_len.data_ptr(), context.data_ptr(), _at(pages),
+                           pages.numel() if pages is not None else 1 << 31, held.data_ptr(), R, rows, width, page_tokens, stride,
+                           _stream()), "page_maps")
+    parts = held.split_with_sizes(sizes)
+    return PageMaps(parts[0], parts[2], parts[4], parts[6], parts[8], parts[10].view(R, width))
 
 
 # ------------------------------------------------------------------ key/value cache in four bits
@@ -2788,12 +2810,10 @@ def kv4_width(head_dim: int) -> int:
 
 
 def _kv4_pages(what: str, pages: torch.Tensor, kv_heads: int, page_tokens: int, head_dim: int) -> None:
-    _need_contiguous(pages)
     if page_tokens < 1 or page_tokens % KV4_PAGE_UNIT:
         raise KernelError(f"{what}: a page holds a multiple of {KV4_PAGE_UNIT} tokens, got {page_tokens}")
-    if pages.dtype != torch.uint8 or tuple(pages.shape[1:]) != (kv_heads, page_tokens, kv4_width(head_dim)):
+    if pages.dtype != torch.uint8 or pages.dim() != 4 or pages.shape[1:] != (kv_heads, page_tokens, kv4_width(head_dim)):
         raise KernelError(f"{what}: pages must be uint8 [page, kv_head, page_tokens, {kv4_width(head_dim)}]")
-    _need_aligned(what, pages)
 
 
 def kv4_write(qkv: torch.Tensor, bias: Optional[torch.Tensor], q_out: torch.Tensor, pages: Optional[torch.Tensor],
@@ -2803,7 +2823,6 @@ def kv4_write(qkv: torch.Tensor, bias: Optional[torch.Tensor], q_out: torch.Tens
     is one layer's, uint8 [page, kv_head, page_tokens, kv4_width(head_dim)] (None: nothing is written); a row whose slot is
     negative or behind the last page writes nothing.  Two rows of one call must not share a slot.  Groups of 32 channels are kept as lo + s * code, code 0..15, each off by at most s / 2 (s: a
     fifteenth of the group's span, rounded up to bfloat16); NaN is kept as 0, what lies beyond 2^120 as 2^120."""
-    _need_contiguous(qkv, bias, q_out, positions, slots, inv_freq)
     T, H, KV = qkv.shape[0], num_heads, num_kv_heads
     width = (H + 2 * KV) * head_dim
     kv4_width(head_dim)
@@ -2825,32 +2844,26 @@ def kv4_write(qkv: torch.Tensor, bias: Optional[torch.Tensor], q_out: torch.Tens
         raise KernelError("kv4_write: inv_freq must be float32 [rotary_dim / 2], rotary_dim even and at most head_dim")
     if 2 * KV * head_dim * 4 + rotary_dim * 4 > 48 * 1024:
         raise KernelError(f"kv4_write: {KV} key/value heads of {head_dim} do not fit in shared memory")
-    _need_aligned("kv4_write", qkv, bias, q_out)
-    _need_cuda(qkv, bias, q_out, pages, positions, slots, inv_freq)
-    _need_here("kv4_write", qkv, bias, q_out, pages, positions, slots, inv_freq)
-    fn = _fn("kv4_write", "pbe_kv4_write", [c_void_p] * 7 + [c_int] * 7 + [c_ll, c_int, c_void_p])
-    _check(fn(_ptr(qkv), _ptr(bias), _ptr(q_out), _ptr(pages), _ptr(positions), _ptr(slots), _ptr(inv_freq), T, H, KV, head_dim,
-              rotary_dim, page_tokens, 1 if interleaved else 0, pages.shape[0] if pages is not None else 0, dtype, _stream()),
-           "kv4_write")
+    _ready("kv4_write", (qkv, bias, q_out, pages), (positions, slots, inv_freq))
+    _check(_kv4_fns().write(qkv.data_ptr(), _at(bias), q_out.data_ptr(), _at(pages), positions.data_ptr(), _at(slots),
+                            _at(inv_freq), T, H, KV, head_dim, rotary_dim, page_tokens, 1 if interleaved else 0,
+                            pages.shape[0] if pages is not None else 0, dtype, _stream()), "kv4_write")
     return q_out
 
 
 def kv4_read(pages: torch.Tensor, slots: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16):
     """The keys and values that the slots (int32 [T]) of 4-bit pages stand for, lo + s * code: two tensors [T, kv_head,
     head_dim] in ``out_dtype``; zeros where a slot is negative or behind the last page."""
-    _need_contiguous(slots)
     if out_dtype not in (torch.float32, torch.bfloat16):
         raise KernelError(f"kernels take float32 or bfloat16 tensors, got {out_dtype}")
     if pages.dim() != 4 or slots.dtype != torch.int32 or slots.dim() != 1:
         raise KernelError("kv4_read: pages have four dimensions, slots are int32 [T]")
     KV, page_tokens, head_dim = pages.shape[1], pages.shape[2], pages.shape[3] * 4 // 5
     _kv4_pages("kv4_read", pages, KV, page_tokens, head_dim)
-    _need_cuda(pages, slots)
-    _need_here("kv4_read", pages, slots)
-    k, v = torch.empty((2, slots.numel(), KV, head_dim), dtype=out_dtype, device=pages.device)
-    fn = _fn("kv4_write", "pbe_kv4_read", [c_void_p] * 4 + [c_int] * 4 + [c_ll, c_int, c_void_p])
-    _check(fn(_ptr(pages), _ptr(slots), _ptr(k), _ptr(v), slots.numel(), KV, head_dim, page_tokens, pages.shape[0],
-              _dtype_code(k), _stream()), "kv4_read")
+    _ready("kv4_read", (pages,), (slots,))
+    k, v = torch.empty((2, slots.numel(), KV, head_dim), dtype=out_dtype, device=pages.device).unbind()
+    _check(_kv4_fns().read(pages.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), slots.numel(), KV, head_dim,
+                           page_tokens, pages.shape[0], _dtype_code(k), _stream()), "kv4_read")
     return k, v
 
 
@@ -2861,6 +2874,26 @@ class Kv4AttnParams(ctypes.Structure):
 
 
 KV4_MAX_REQUESTS = 8192
+class Kv4Fns(NamedTuple):
+    write: object
+    read: object
+    attention: object
+
+
+@functools.lru_cache(maxsize=None)
+def _kv4_fns() -> Kv4Fns:
+    return Kv4Fns(_fn("kv4_write", "pbe_kv4_write", [c_void_p] * 7 + [c_int] * 7 + [c_ll, c_int, c_void_p]),
+                  _fn("kv4_write", "pbe_kv4_read", [c_void_p] * 4 + [c_int] * 4 + [c_ll, c_int, c_void_p]),
+                  _fn("kv4_attention", "pbe_kv4_attention",
+                      [ctypes.POINTER(Kv4AttnParams), c_void_p] + [c_int] * 5 + [c_void_p]))
+
+
+@functools.lru_cache(maxsize=None)
+def _kv4_prompt_fn():
+    return _fn("kv4_attention_tc5", "pbe_kv4_attention_tc5",
+               [ctypes.POINTER(Kv4AttnParams), c_void_p] + [c_int] * 4 + [c_void_p] * 2)
+
+
 KV4_FEW_PACKED = 64         # packed rows (rows x heads of a key/value head) up to which a request is the mma.sync kernel's
 KV4_SPLIT_KEYS = 512        # keys of a split of the tcgen05 kernel at least
 KV4_MOST_SPLITS = 32
@@ -2880,12 +2913,13 @@ def _kv4_shape(requests: int, heads: int, kv_heads: int, head_dim: int, most_row
 def kv4_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor,
                   seq_len: torch.Tensor, block_table: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int,
                   scale: float, window: Optional[int], page_tokens: int, most_rows: int, most_keys: int) -> torch.Tensor:
-    """Causal attention of every row over 4-bit pages, ``paged_attention`` for a cache in four bits: row i of request r (row
-    ``q_start[r] + i`` of q and out, both [T, H * head_dim], no row of two requests) sees the request's first ``seq_len[r] - q_len[r] + i + 1`` keys, or the last ``window`` of
-    them, at ``block_table[r]`` (int32 [R, width], rows may be strided).  A row that sees no key is 0; rows of no request are left as
-    they are.  A key whose block-table entry is no page, or lies behind the table, is not seen.  ``most_rows`` and ``most_keys`` are the
-    largest of q_len and seq_len as far as the host knows them: they choose the shape of the launch, not the result."""
-    _need_contiguous(q, out, q_start, q_len, seq_len)
+    """Causal attention of every row over 4-bit pages, ``paged_attention`` for a cache in four bits.  Row i of request r (row
+    ``q_start[r] + i`` of q and out, both [T, H * head_dim]; no row belongs to two requests) sees the request's first
+    ``seq_len[r] - q_len[r] + i + 1`` keys, or the last ``window`` of them (None or 0: all), at ``block_table[r]`` (int32 [R,
+    width], rows may be strided).  A row that sees no key is 0; rows of no request are left as they are.  A key whose
+    block-table entry is no page, or lies behind the table, is not seen.  ``most_rows`` and ``most_keys`` are the largest of
+    q_len and seq_len as far as the host knows them: they choose the shape of the launch, not the result (beyond the order
+    of its sums).  At most ``KV4_MAX_REQUESTS`` requests."""
     H, KV, R = num_heads, num_kv_heads, q_len.numel()
     if H < 1 or KV < 1 or H % KV:
         raise KernelError("kv4_attention: num_heads must be a multiple of num_kv_heads")
@@ -2903,14 +2937,14 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, q_sta
     if window is not None and window < 0:
         raise KernelError("kv4_attention: a window is at least 1")
     dtype = _dtype_code(q)
-    _need_aligned("kv4_attention", q, out)
-    _need_cuda(q, pages, out, q_start, q_len, seq_len, block_table)
-    _need_here("kv4_attention", q, pages, out, q_start, q_len, seq_len, block_table)
-    p = Kv4AttnParams(
-        q=q.data_ptr(), pages=pages.data_ptr(), out=out.data_ptr(), q_start=q_start.data_ptr(), q_len=q_len.data_ptr(),
-        seq_len=seq_len.data_ptr(), block_table=block_table.data_ptr(), bt_stride=block_table.stride(0),
-        table_pages=block_table.shape[1], num_pages=pages.shape[0], requests=R, rows=q.shape[0], heads=H, kv_heads=KV,
-        page_tokens=page_tokens, window=int(window or 0), scale=float(scale))
+    if R == 0 or q.shape[0] == 0:
+        return out
+    _ready("kv4_attention", (q, pages, out), (q_start, q_len, seq_len))
+    if block_table.get_device() != q.get_device():
+        raise KernelError("kv4_attention: block_table must lie on the other operands' device")
+    p = Kv4AttnParams(q.data_ptr(), pages.data_ptr(), out.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), seq_len.data_ptr(),
+                      block_table.data_ptr(), block_table.stride(0), block_table.shape[1], pages.shape[0], R, q.shape[0], H, KV,
+                      page_tokens, window or 0, scale)
     bf16, group, T = q.dtype == torch.bfloat16, H // KV, q.shape[0]
     # requests of many packed rows go to the tcgen05 kernel, where the hint says that there may be some (a request alone in
     # its step then goes there whatever its rows); both kernels read from the lengths on the device which are theirs
@@ -2923,15 +2957,14 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, q_sta
         tile_rows, blocks = _kv4_shape(R, H, KV, head_dim, rows, most_keys, bf16, multiprocessors(q.device))
         floats = 8 * blocks + 2 * blocks * tile_rows * (head_dim + 2)
         work = torch.empty(floats, dtype=torch.float32, device=q.device)
-        fn = _fn("kv4_attention", "pbe_kv4_attention", [ctypes.POINTER(Kv4AttnParams), c_void_p] + [c_int] * 5 + [c_void_p])
-        _check(fn(params, _ptr(work), blocks, head_dim, tile_rows, most_packed, dtype, stream), "kv4_attention")
+        _check(_kv4_fns().attention(params, work.data_ptr(), blocks, head_dim, tile_rows, most_packed, dtype, stream),
+               "kv4_attention")
     if most_packed != 0x7fffffff:
         # row tiles of 256: at most one of each request is not full
         tiles = T * group // 256 + min(R, T * group // (most_packed + 1))
         busy = -(-T * group // 256) * KV
         splits = max(1, min(multiprocessors(q.device) // busy, -(-most_keys // KV4_SPLIT_KEYS), KV4_MOST_SPLITS))
         work = torch.empty(tiles * KV * splits * 256 * (head_dim + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
-        fn = _fn("kv4_attention_tc5", "pbe_kv4_attention_tc5", [ctypes.POINTER(Kv4AttnParams), c_void_p] + [c_int] * 4 + [c_void_p] * 2)
-        _check(fn(params, _ptr(work), tiles, splits, head_dim, most_packed, _ptr(tc5_attention_error_buffer(q.device)), stream),
-               "kv4_attention (tcgen05)")
+        err = tc5_attention_error_buffer(q.device).data_ptr()
+        _check(_kv4_prompt_fn()(params, _at(work), tiles, splits, head_dim, most_packed, err, stream), "kv4_attention (tcgen05)")
     return out
