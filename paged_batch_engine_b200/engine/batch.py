@@ -28,6 +28,8 @@ SPLIT_KEYS = 256          # keys per split of a short request's long key range, 
 SPLIT_KEYS_FEW = 512      # the same in steps of at most FEW_REQUESTS requests
 FEW_REQUESTS = 4          # (a bucket edge of the captured decode steps)
 MAX_SPLIT_TILES = 4       # requests with more row tiles than this are never split
+MAPS_ROWS = 4096          # steps of at least this many rows have their row maps and block tables made on the device (one request:
+#                           412 us of host time -> 394, of 2,048 rows 327 -> 331)
 
 
 def choose_split_keys(num_requests: int) -> int:
@@ -284,14 +286,20 @@ class StepContext:
         self.num_tokens, self.num_requests = T, R
         self.q_len_host, self.seq_len_host, self.q_start_host = q_len, seq_len, q_start
         self.context_before_host = ctx_before
+        self.most_rows, self.longest_keys = int(q_len.max()), int(seq_len.max())
         self.state_slots_host = np.array([manager.state_slot(e.handle) for e in entries], dtype=np.int64)
         tokens = np.concatenate([np.asarray(e.tokens, dtype=np.int64) for e in entries])
         if vocab_size is not None and ((tokens < 0) | (tokens >= vocab_size)).any():
             bad = tokens[(tokens < 0) | (tokens >= vocab_size)][0]
             raise ValueError(f"token id {int(bad)} is outside the vocabulary of {vocab_size}")
-        req_of_tok = np.repeat(np.arange(R), q_len)
-        offs = np.arange(T) - q_start[req_of_tok]
-        positions = ctx_before[req_of_tok] + offs
+        # Steps of many rows leave the row maps and block tables to the device (one launch a layer group); the host sends the
+        # lengths and the pages.
+        on_device = T >= MAPS_ROWS and torch.device(device).type == "cuda" and len(manager.groups) > 0 and \
+            all(int(getattr(g, "stride", 1) or 1) == 1 for g in manager.groups)
+        if not on_device:
+            req_of_tok = np.repeat(np.arange(R), q_len)
+            offs = np.arange(T) - q_start[req_of_tok]
+            positions = ctx_before[req_of_tok] + offs
         want_rows = []
         for r, e in enumerate(entries):
             for w in e.want:
@@ -311,16 +319,24 @@ class StepContext:
             pos_ids = np.concatenate(rows_, axis=0)
 
         pk = _Packer()
-        i_tokens, i_pos = pk.add(tokens), pk.add(positions)
+        i_tokens, i_pos = pk.add(tokens), pk.add(ctx_before if on_device else positions)
         i_pos_ids = pk.add(pos_ids) if pos_ids is not None else None
         i_qs, i_ql, i_sl = pk.add(q_start), pk.add(q_len), pk.add(seq_len)
         i_want = pk.add(np.array(want_rows, dtype=np.int64))
         i_state = pk.add(self.state_slots_host)
-        i_req = pk.add(req_of_tok)
+        i_req = None if on_device else pk.add(req_of_tok)
         i_groups = []
         for g in range(len(manager.groups)):
-            tables = [manager.block_table(e.handle, g) for e in entries]
+            tables = [manager.block_table_array(e.handle, g) for e in entries]
             stride = max(min_bt_stride, max(len(t) for t in tables))
+            if on_device:
+                need = -(-seq_len // P)
+                held = [t[:n] for t, n in zip(tables, need)]
+                flat = np.concatenate(held)
+                if len(flat) < need.sum() or ((flat < 0).any() and any((t[c // P:] < 0).any() for t, c in zip(held, ctx_before))):
+                    raise ValueError("a token of this step lies in a page that is not held")
+                i_groups.append((pk.add(flat), stride, None))
+                continue
             bt = np.full((R, stride), -1, dtype=np.int32)
             for r, t in enumerate(tables):
                 bt[r, :len(t)] = t
@@ -343,6 +359,11 @@ class StepContext:
         self._packer = pk
         self.token_ids = pk.view(i_tokens)
         self.positions = pk.view(i_pos)
+        maps = []
+        if on_device:
+            lens, before = pk.view(i_ql), pk.view(i_pos)
+            maps = [ops.page_maps(lens, before, pk.view(i), P, T, stride) for i, stride, _ in i_groups]
+            self.positions = maps[0].positions
         # what a position encoding is given: the explicit ids ([T] for one axis, [T, axes] for
         # several), or the places in the sequence
         self.position_ids = self.positions
@@ -352,9 +373,13 @@ class StepContext:
         self.q_start, self.q_len, self.seq_len = pk.view(i_qs), pk.view(i_ql), pk.view(i_sl)
         self.want_rows = pk.view(i_want)
         self.state_slots = pk.view(i_state)
-        self.request_of_row = pk.view(i_req)       # int32 [T]: which entry of the step a row belongs to
+        # int32 [T]: which entry of the step a row belongs to
+        self.request_of_row = maps[0].request_of_row if on_device else pk.view(i_req)
         self._row_tiles: Dict[int, tuple] = {}
-        self._groups = [GroupArrays(pk.view(ib), stride, pk.view(isl)) for ib, stride, isl in i_groups]
+        if on_device:
+            self._groups = [GroupArrays(m.block_table, stride, m.slots) for m, (_, stride, _) in zip(maps, i_groups)]
+        else:
+            self._groups = [GroupArrays(pk.view(ib), stride, pk.view(isl)) for ib, stride, isl in i_groups]
         self._work: Dict[tuple, AttentionWork] = {}
         for key, (iw, nw, itsr, ist, isc, ns, max_splits, (kinds, small_items)) in i_work.items():
             g = self._groups[key[0]]
