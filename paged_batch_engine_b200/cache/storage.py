@@ -7,7 +7,7 @@ from typing import Dict, List, Optional, Sequence
 
 import torch
 
-from ..parts.base import CompositeNeed, KVNeed, PagedNeed, StateNeed
+from ..parts.base import CompositeNeed, KV4Need, KVNeed, PagedNeed, StateNeed
 from .manager import CacheManager, KVGroupSpec
 
 
@@ -69,9 +69,9 @@ class CacheStorage:
             n = self.manager.pools[g].num_pages
             held = {}
             for t in spec.tensors:
-                x = torch.empty((len(spec.layers), n, t.heads, self.page_tokens, t.width), dtype=dtype, device=device)
+                x = torch.empty((len(spec.layers), n, t.heads, self.page_tokens, t.width), dtype=t.dtype or dtype, device=device)
                 if poison:
-                    x.fill_(float("nan"))
+                    x.fill_(float("nan") if x.is_floating_point() else 0xff)     # the bytes of a NaN too
                 held[t.name] = x
             self.paged.append(held)
 
@@ -83,7 +83,7 @@ class CacheStorage:
                 self._next_layer += 1
                 self._parts[layer][name] = sub_layer
                 self._place(sub_layer, part, keys, members)
-        elif isinstance(need, (KVNeed, PagedNeed)):
+        elif isinstance(need, (KVNeed, KV4Need, PagedNeed)):
             key = (tuple(need.tensors), need.window, int(getattr(need, "stride", 1) or 1))
             if not key[0]:
                 raise TypeError(f"cache layer {layer}: a paged need lists at least one tensor")
@@ -113,10 +113,9 @@ class CacheStorage:
         return self.max_requests
 
     def bytes_per_token(self) -> int:
-        size = torch.empty((), dtype=self.dtype).element_size()
         # a group of one entry per `stride` tokens costs a token that much less
-        return sum(-(-len(g.layers) * sum(t.heads * t.width for t in g.tensors) * size // max(1, g.stride))
-                   for g in self.groups)
+        return sum(-(-len(g.layers) * sum(t.heads * t.width * (t.dtype or self.dtype).itemsize for t in g.tensors)
+                     // max(1, g.stride)) for g in self.groups)
 
     def zero_state(self, slots) -> None:
         """Zeroes the state rows of these request slots in every stateful layer (the step

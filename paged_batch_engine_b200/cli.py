@@ -52,6 +52,7 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--page-size", type=int, default=16)
     ap.add_argument("--kv-cache-memory-utilization", type=float, default=0.80)
     ap.add_argument("--kv-cache-blocks-per-layer", type=int, default=0, help="pages in the pool; 0: from memory")
+    ap.add_argument("--kv-cache-bits", type=int, choices=[4], help="keep keys and values in 4 bits (default: in the dtype)")
     ap.add_argument("--max-model-len", type=int, default=0)
     ap.add_argument("--warmup-rounds", type=int, default=0)
     ap.add_argument("--no-cuda-graphs", action="store_true")
@@ -113,7 +114,8 @@ def main(argv=None) -> int:
                     max_num_batched_tokens=args.max_batched_tokens or 4096,
                     prefill_chunk_cap=args.prefill_chunk_cap or 1024,
                     long_prefill_token_threshold=args.long_prefill_token_threshold,
-                    max_model_len=args.max_model_len or None, use_cuda_graphs=not args.no_cuda_graphs)
+                    max_model_len=args.max_model_len or None, use_cuda_graphs=not args.no_cuda_graphs,
+                    kv_cache_bits=args.kv_cache_bits)
     params = SamplingParams(max_new_tokens=args.max_new_tokens, min_new_tokens=args.min_new_tokens,
                             ignore_eos=args.ignore_eos, temperature=args.temperature, top_k=args.top_k,
                             top_p=args.top_p, repetition_penalty=args.repetition_penalty, seed=args.seed)

@@ -138,7 +138,7 @@ def block_desc(block) -> Optional[BlockDesc]:
         return None
     if f.activation != "silu" or f.bias or n1.on_output or n2.on_output:
         return None
-    if m.dtype != torch.bfloat16 or m.o_bias or m.kernel_kind == "simple":
+    if m.dtype != torch.bfloat16 or m.o_bias or m.kernel_kind == "simple" or m.cache_bits:
         return None
     tensors = [m.w_qkv, m.w_o, f.w_gate_up, f.w_down]
     if any(t is None or t.dtype != torch.bfloat16 or not t.is_contiguous() for t in tensors):

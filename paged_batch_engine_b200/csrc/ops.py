@@ -2873,6 +2873,11 @@ class Kv4AttnParams(ctypes.Structure):
                                                       "page_tokens", "window")] + [("scale", c_float)]
 
 
+def kv4_libraries(dtype: torch.dtype):
+    """The (library, defines) pairs a model with a 4-bit cache needs."""
+    return [("kv4_write", None), ("kv4_attention", None)] + ([("kv4_attention_tc5", None)] if dtype == torch.bfloat16 else [])
+
+
 KV4_MAX_REQUESTS = 8192
 class Kv4Fns(NamedTuple):
     write: object

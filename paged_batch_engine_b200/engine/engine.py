@@ -42,19 +42,22 @@ class Engine:
                  kv_cache_memory_utilization: float = 0.80, max_num_seqs: int = 256,
                  max_num_batched_tokens: int = 2048, prefill_chunk_cap: int = 512,
                  long_prefill_token_threshold: int = 0, max_model_len: Optional[int] = None,
-                 use_cuda_graphs: bool = True, decode_ahead: bool = True):
+                 use_cuda_graphs: bool = True, decode_ahead: bool = True, kv_cache_bits: Optional[int] = None):
         """``model``: a folder with config.json and safetensors, or a typed configuration /
         config dict, in which case the weights are random from ``seed``.  ``num_pages``:
         pages per layer group; if None the cache takes ``kv_cache_memory_utilization`` of the
         free device memory minus a reserve, as the reference plans its pool
-        (infMain/source/model/serving_memory_planner.cpp:41-106)."""
+        (infMain/source/model/serving_memory_planner.cpp:41-106).  ``kv_cache_bits`` 4: keys and values are kept in four
+        bits, 3.2 times the tokens of a bfloat16 cache in the same memory (grouped-query attention of head size 64 or 128,
+        ``page_size`` a multiple of 16)."""
         self.dtype = _parse_dtype(dtype)
         self.device = torch.device(device)
         kw = dict(page_tokens=page_size, max_requests=max(max_num_seqs, 1), max_context=max_model_len)
         if isinstance(model, str):
-            build = lambda **k: ModelRunner.from_folder(model, dtype=self.dtype, device=device, **k)
+            build = lambda **k: ModelRunner.from_folder(model, dtype=self.dtype, device=device, cache_bits=kv_cache_bits, **k)
         else:
-            build = lambda **k: ModelRunner.from_random(model, seed=seed, dtype=self.dtype, device=device, **k)
+            build = lambda **k: ModelRunner.from_random(model, seed=seed, dtype=self.dtype, device=device,
+                                                        cache_bits=kv_cache_bits, **k)
         if num_pages is None:
             # load the weights first with a one-page pool, then size the pool from what is free
             probe = build(num_pages=1, **kw)

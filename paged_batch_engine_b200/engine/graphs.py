@@ -67,6 +67,7 @@ class DecodeStepContext(StepContext):
         self.batch, self.splits = batch, splits
         self.split_keys = choose_split_keys(batch)
         self.num_tokens = self.num_requests = self.num_wanted = batch
+        self.most_rows, self.longest_keys = 1, splits * self.split_keys       # of its capacity
         self.work_keys = list(work_keys)
         B, S = batch, splits
         off = 0
@@ -247,8 +248,10 @@ class DecodeGraphs:
         every request of the step and does not move as the requests grow."""
         m = self.runner.cache
         longest = m.max_reserved_len([e.handle for e in entries])
-        return max([1] + [splits_bound(longest, window, split_keys)
-                          for _, _, _, window in self.runner._work_keys])
+        windows = [window for _, _, _, window in self.runner._work_keys]
+        if self.runner.model.shaped_by_keys():
+            windows.append(None)
+        return max([1] + [splits_bound(longest, window, split_keys) for window in windows])
 
     def run(self, entries: Sequence[StepEntry], device_tokens: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``device_tokens`` (int32 on the device, one per entry): the token ids of this step

@@ -19,7 +19,9 @@ import torch
 
 from ..cache.storage import CacheStorage
 from ..config.registry import load_config
+from ..csrc import ops
 from ..models.decoder import DecoderModel
+from ..parts.base import KV4Need
 from ..weights.loader import load_weights
 from ..weights.random_init import random_tensor
 from .batch import StepContext, StepEntry
@@ -44,17 +46,19 @@ def require_cuda(device) -> torch.device:
     return device
 
 
-def build_model(config, dtype, device) -> DecoderModel:
-    """config: a folder, a config.json path, a dict or a typed config with model_spec()."""
+def build_model(config, dtype, device, cache_bits: Optional[int] = None) -> DecoderModel:
+    """config: a folder, a config.json path, a dict or a typed config with model_spec().  ``cache_bits`` 4: keys and values
+    are kept in four bits (None: in the run dtype)."""
     if hasattr(config, "model_spec"):
         arch_builder, typed = None, config
     else:
         arch, typed = load_config(config)
         arch_builder = arch.builder
     spec = typed.model_spec()
-    if arch_builder is not None:
-        return arch_builder(spec, dtype, device)
-    return DecoderModel(spec, dtype, device)
+    model = arch_builder(spec, dtype, device) if arch_builder is not None else DecoderModel(spec, dtype, device)
+    if cache_bits is not None:
+        model.use_cache_bits(int(cache_bits))
+    return model
 
 
 class ModelRunner:
@@ -67,6 +71,8 @@ class ModelRunner:
             if max_cache_tokens is None:
                 raise ValueError("give num_pages or max_cache_tokens")
             num_pages = (max_cache_tokens + page_tokens - 1) // page_tokens
+        if any(isinstance(need, KV4Need) for need in model.cache_needs) and page_tokens % ops.KV4_PAGE_UNIT:
+            raise ValueError(f"a 4-bit cache has pages of a multiple of {ops.KV4_PAGE_UNIT} tokens, got {page_tokens}")
         self.storage = CacheStorage(model.cache_needs, page_tokens, num_pages, max_requests,
                                     model.dtype, self.device, lifo=lifo, poison=poison)
         self.cache = self.storage.manager
@@ -80,20 +86,22 @@ class ModelRunner:
 
     # ------------------------------------------------------------------ construction
     @classmethod
-    def from_folder(cls, folder: str, dtype="bfloat16", device="cuda:0", **kw) -> "ModelRunner":
+    def from_folder(cls, folder: str, dtype="bfloat16", device="cuda:0", cache_bits: Optional[int] = None,
+                    **kw) -> "ModelRunner":
         device = require_cuda(device)
         dtype = _parse_dtype(dtype)
-        model = build_model(folder, dtype, device)
+        model = build_model(folder, dtype, device, cache_bits)
         model.build_kernels()
         model.load(load_weights(folder, model.param_specs(), dtype, device))
         return cls(model, **kw)
 
     @classmethod
-    def from_random(cls, config, seed: int = 0, dtype="bfloat16", device="cuda:0", **kw) -> "ModelRunner":
+    def from_random(cls, config, seed: int = 0, dtype="bfloat16", device="cuda:0", cache_bits: Optional[int] = None,
+                    **kw) -> "ModelRunner":
         """Random weights made on the device (for measurements; no folder is written)."""
         device = require_cuda(device)
         dtype = _parse_dtype(dtype)
-        model = build_model(config, dtype, device)
+        model = build_model(config, dtype, device, cache_bits)
         model.build_kernels()
         tensors = {}
         for p in model.param_specs():

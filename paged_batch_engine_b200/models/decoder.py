@@ -39,12 +39,22 @@ class DecoderModel:
         self.lm_head = None
         self.position_table = None
         self.input_mixes: Dict[str, torch.Tensor] = {}
+        self.cache_needs = self._cache_needs()
+
+    def _cache_needs(self) -> List[object]:
         # a cache layer's need is stated by the run step that writes it
-        needs: List[object] = [None] * spec.num_cache_layers
-        for step in spec.run_order:
+        needs: List[object] = [None] * self.spec.num_cache_layers
+        for step in self.spec.run_order:
             if step.writes_cache:
                 needs[step.cache_layer] = self.blocks[step.block].mixer.cache_need()
-        self.cache_needs = needs
+        return needs
+
+    def use_cache_bits(self, bits: int) -> None:
+        """Keep the keys and values of every attention in ``bits`` bits; to be called before the kernels are built and the
+        cache is laid out.  An error where a mixer has pages and no such form."""
+        for b in self.blocks:
+            b.mixer.use_cache_bits(bits)
+        self.cache_needs = self._cache_needs()
 
     # ------------------------------------------------------------------ tensors
     def param_specs(self) -> List[ParamSpec]:
@@ -107,6 +117,10 @@ class DecoderModel:
         """True when every mixer says it can step decoded tokens inside a captured CUDA graph
         (``Mixer.decode_capturable``)."""
         return all(getattr(b.mixer, "decode_capturable", False) for b in self.blocks)
+
+    def shaped_by_keys(self) -> bool:
+        """True when a mixer's launches follow the step's longest context without a work list (``Mixer.shaped_by_keys``)."""
+        return any(getattr(b.mixer, "shaped_by_keys", False) for b in self.blocks)
 
     # ------------------------------------------------------------------ what a step needs
     def work_keys(self, storage):

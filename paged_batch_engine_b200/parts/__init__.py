@@ -1,4 +1,4 @@
-from .base import (Block, CacheTensor, CompositeNeed, FeedForward, KVNeed, Mixer, Norm, PagedNeed, Part, PositionEncoding, StateNeed,
+from .base import (Block, CacheTensor, CompositeNeed, FeedForward, KV4Need, KVNeed, Mixer, Norm, PagedNeed, Part, PositionEncoding, StateNeed,
                    build_block, build_part, register_part)
 from .norm import DeltaSum, LayerNorm, NormedDelta, PendingUpdate, RMSNorm, ScalarRMSNorm
 from .rope import NoPositionEncoding, RotaryEncoding
@@ -17,7 +17,7 @@ from .masked_attention import MaskedAttention
 from .time_mixing import TimeMixing
 from .streams import StreamBlock, StreamConnection
 
-__all__ = ["Block", "CacheTensor", "CompositeNeed", "FeedForward", "KVNeed", "Mixer", "Norm", "PagedNeed", "Part", "PositionEncoding",
+__all__ = ["Block", "CacheTensor", "CompositeNeed", "FeedForward", "KV4Need", "KVNeed", "Mixer", "Norm", "PagedNeed", "Part", "PositionEncoding",
            "StateNeed",
            "build_block", "build_part", "register_part", "RMSNorm", "NoPositionEncoding", "RotaryEncoding",
            "GQAttention", "SwiGLU", "PreNormBlock", "LayerNorm", "PendingUpdate", "DecayLinearAttention",

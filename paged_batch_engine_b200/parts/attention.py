@@ -5,11 +5,11 @@ from typing import Optional
 
 import torch
 
-from ..config.specs import PartSpec
+from ..config.specs import ConfigError, PartSpec
 from ..csrc import ops
 
 from ..weights.loader import ParamSpec
-from .base import KVNeed, Mixer, build_part, register_part
+from .base import KV4Need, KVNeed, Mixer, build_part, register_part
 
 
 class GQAttention(Mixer):
@@ -22,7 +22,11 @@ class GQAttention(Mixer):
     Checkpoint tensors: {q,k,v}_proj.weight [heads*head_dim, hidden] (+ .bias),
     o_proj.weight [hidden, heads*head_dim] (+ .bias when o_bias).  ``tensor_names`` renames
     the four projections for checkpoints that call them otherwise, e.g.
-    ``dict(q="wq", k="wk", v="wv", o="wo")``; ``.weight`` / ``.bias`` are appended."""
+    ``dict(q="wq", k="wk", v="wv", o="wo")``; ``.weight`` / ``.bias`` are appended.
+
+    ``use_cache_bits(4)``: keys and values are kept in four bits (``ops.kv4_write``, ``ops.kv4_attention``), head sizes 64 and
+    128, pages of whole 16 tokens; a step then takes one launch to write and one attention call, decoded tokens and prompt
+    portions alike."""
     TENSOR_NAMES = dict(q="q_proj", k="k_proj", v="v_proj", o="o_proj")
     decode_capturable = True      # decoded tokens are stepped from the step's device arrays alone
 
@@ -46,15 +50,28 @@ class GQAttention(Mixer):
             else build_part("position", PartSpec("none"), dtype, device)
         self.kernel_kind, self.tile_rows, self.key_tile = ops.attention_kernel_config(head_dim, dtype, kernel)
         self.w_qkv = self.b_qkv = self.w_o = self.b_o = None
+        self.cache_bits: Optional[int] = None
 
     # ---- what it keeps
     def cache_need(self):
+        if self.cache_bits:
+            return KV4Need(self.num_kv_heads, ops.kv4_width(self.head_dim), self.window)
         return KVNeed(self.num_kv_heads, self.head_dim, self.window)
 
+    def use_cache_bits(self, bits):
+        if bits != 4 or self.head_dim not in ops.KV4_HEAD_DIMS:
+            raise ConfigError(f"attention keeps a cache in 4 bits for head sizes {ops.KV4_HEAD_DIMS}; asked for {bits} bits, "
+                              f"head size {self.head_dim}")
+        self.cache_bits, self.shaped_by_keys = bits, True
+
     def work_keys(self):
+        if self.cache_bits:
+            return []
         return [(self.num_heads // self.num_kv_heads, self.tile_rows, self.window)]
 
     def kernel_libraries(self, dtype):
+        if self.cache_bits:
+            return [("elementwise", None)] + ops.gemm_libraries(dtype) + ops.kv4_libraries(dtype)
         return [("elementwise", None), ("rope_kv", None)] + ops.gemm_libraries(dtype) + \
             ops.attention_libraries(self.head_dim, dtype)
 
@@ -126,6 +143,14 @@ class GQAttention(Mixer):
         if ctx.position_ids.dim() != 1 and not self.position.applies_itself:
             raise ValueError("position ids with several axes need a position encoding with code of its own")
         group = ctx.group(cache.group)
+        if self.cache_bits:
+            pages = cache.tensors["kv4"]
+            q = torch.empty((T, H * hd), dtype=self.dtype, device=x.device)
+            ops.kv4_write(qkv, bias, q, pages if cache.writes else None, kernel_positions, group.slots, inv_freq, H, KV, hd,
+                          rotary_dim, ctx.page_tokens, interleaved)
+            out = ops.kv4_attention(q, pages, torch.empty_like(q), ctx.q_start, ctx.q_len, ctx.seq_len, group.block_table, H, KV,
+                                    hd, self.scale, self.window, ctx.page_tokens, ctx.most_rows, ctx.longest_keys)
+            return ops.linear(out, self.w_o, self.b_o, out_dtype=self.dtype, kind=2)
         k_pages, v_pages = cache.k, cache.v
         meta = ctx.attention_work(cache.group, H // KV, self.tile_rows, self.window, H, hd)
         splits = self.fused_decode_splits(meta, cache, inv_freq, rotary_dim, interleaved)

@@ -38,10 +38,11 @@ from ..weights.loader import ParamSpec
 
 @dataclass(frozen=True)
 class CacheTensor:
-    """One tensor of a paged cache layer: ``[page, heads, page_tokens, width]`` per layer."""
+    """One tensor of a paged cache layer: ``[page, heads, page_tokens, width]`` per layer, in the run dtype or ``dtype``."""
     name: str
     heads: int
     width: int
+    dtype: Optional[torch.dtype] = None
 
 
 @dataclass(frozen=True)
@@ -68,6 +69,19 @@ class KVNeed:
     def tensors(self) -> Tuple[CacheTensor, ...]:
         return (CacheTensor("k", self.num_kv_heads, self.head_dim),
                 CacheTensor("v", self.num_kv_heads, self.head_dim))
+
+
+@dataclass(frozen=True)
+class KV4Need:
+    """Keys and values of equal geometry in 4-bit pages: one tensor of bytes, ``width`` of them for the key and the value of
+    one token of one head together (``ops.kv4_width``)."""
+    num_kv_heads: int
+    width: int
+    window: Optional[int] = None
+
+    @property
+    def tensors(self) -> Tuple[CacheTensor, ...]:
+        return (CacheTensor("kv4", self.num_kv_heads, self.width, torch.uint8),)
 
 
 @dataclass(frozen=True)
@@ -127,9 +141,18 @@ class Mixer(Part):
     # step's arrays, ``ctx.state_slots``), never with values read on the host, which a replay
     # would not see change.  A mixer that loops over the requests on the host leaves it False.
     decode_capturable = False
+    # True: its launches are shaped by the step's longest context without a work list (``ctx.longest_keys``), so captured
+    # steps are kept apart by it as they are by the key splits of a work list.
+    shaped_by_keys = False
 
     def cache_need(self):
         return None
+
+    def use_cache_bits(self, bits: int) -> None:
+        """Keep keys and values in ``bits`` bits (before the cache is laid out).  A mixer with nothing in pages has nothing
+        to do; one that has pages and no such form refuses."""
+        if isinstance(self.cache_need(), (KVNeed, PagedNeed, CompositeNeed)):
+            raise ConfigError(f"{type(self).__name__} keeps no cache in {bits} bits")
 
     def work_keys(self):
         """Attention work lists this mixer needs from the step: (heads per kv head,

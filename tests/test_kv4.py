@@ -118,3 +118,39 @@ def test_map_refusals(change, words):
     a.update(change)
     with pytest.raises(ops.KernelError, match=words):
         ops.page_maps(**a)
+
+
+def _model(cfg, bits=4, dtype=torch.bfloat16):
+    from paged_batch_engine_b200.config import load_config
+    from paged_batch_engine_b200.engine.runner import build_model
+    return build_model(load_config(cfg)[1] if isinstance(cfg, dict) else cfg, dtype, "cpu", cache_bits=bits)
+
+
+def test_a_model_with_a_4_bit_cache():
+    from paged_batch_engine_b200.cache.storage import CacheStorage
+    from tests.helpers import TINY_D
+    model = _model(TINY_D)
+    assert ("kv4_attention", None) in model.kernel_libraries() and not any(b.mixer.work_keys() for b in model.blocks)
+    assert model.shaped_by_keys() and model.decode_capturable()
+    st = CacheStorage(model.cache_needs, 16, 8, 4, torch.bfloat16, "cpu", poison=True)
+    pages = st.layer(0).tensors["kv4"]
+    assert pages.dtype == torch.uint8 and tuple(pages.shape) == (8, 1, 16, 80) and bool((pages == 0xff).all())
+    assert st.layer(0).k is None and len(st.groups) == 2          # a layer with a window has a pool of its own
+    plain_model = _model(TINY_D, bits=None)
+    wide = CacheStorage(plain_model.cache_needs, 16, 8, 4, torch.bfloat16, "cpu")
+    assert wide.bytes_per_token() * 10 == st.bytes_per_token() * 32
+    assert not plain_model.shaped_by_keys()
+
+
+def test_models_that_keep_no_4_bit_cache():
+    from paged_batch_engine_b200.config.specs import ConfigError
+    from paged_batch_engine_b200.engine.runner import ModelRunner
+    from tests import helpers
+    with pytest.raises(ConfigError, match="head sizes"):
+        _model(helpers.TINY_C)
+    with pytest.raises(ConfigError, match="8 bits"):
+        _model(helpers.TINY_D, bits=8)
+    with pytest.raises(ConfigError, match="keeps no cache in 4 bits"):
+        _model(helpers.GUS_A)
+    with pytest.raises(ValueError, match="multiple of 16"):
+        ModelRunner(_model(helpers.TINY_D), page_tokens=8, num_pages=4)
