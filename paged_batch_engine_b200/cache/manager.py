@@ -324,17 +324,13 @@ class CacheManager:
 
     # ------------------------------------------------------------------ views
     def block_table(self, handle: int, group: int = 0) -> List[int]:
-        return self.block_table_array(handle, group).tolist()
-
-    def block_table_array(self, handle: int, group: int = 0) -> np.ndarray:
-        """``block_table`` as int32, which a step of many pages takes as it is."""
         lib = _host()
         n = lib.pbe_cm_block_table(self._h, self._handle(handle), group, None, 0)
         if n < 0:
             self._raise(n, handle)
         out = np.empty(max(n, 1), dtype=np.int32)
         lib.pbe_cm_block_table(self._h, handle, group, out.ctypes.data, n)
-        return out[:n]
+        return out[:n].tolist()
 
     def slot_of_token(self, handle: int, group: int, position: int) -> int:
         """page * page_tokens + offset of a token (infMain/source/base/sequence_kv_manager.cpp:41-52)."""

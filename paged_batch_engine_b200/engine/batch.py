@@ -29,7 +29,7 @@ SPLIT_KEYS_FEW = 512      # the same in steps of at most FEW_REQUESTS requests
 FEW_REQUESTS = 4          # (a bucket edge of the captured decode steps)
 MAX_SPLIT_TILES = 4       # requests with more row tiles than this are never split
 MAPS_ROWS = 4096          # steps of at least this many rows have their row maps and block tables made on the device (one request:
-#                           412 us of host time -> 394, of 2,048 rows 327 -> 331)
+#                           421 us of host time -> 402, of 2,048 rows 329 -> 336)
 
 
 def choose_split_keys(num_requests: int) -> int:
@@ -327,11 +327,11 @@ class StepContext:
         i_req = None if on_device else pk.add(req_of_tok)
         i_groups = []
         for g in range(len(manager.groups)):
-            tables = [manager.block_table_array(e.handle, g) for e in entries]
+            tables = [manager.block_table(e.handle, g) for e in entries]
             stride = max(min_bt_stride, max(len(t) for t in tables))
             if on_device:
                 need = -(-seq_len // P)
-                held = [t[:n] for t, n in zip(tables, need)]
+                held = [np.array(t[:n], dtype=np.int32) for t, n in zip(tables, need)]
                 flat = np.concatenate(held)
                 if len(flat) < need.sum() or ((flat < 0).any() and any((t[c // P:] < 0).any() for t, c in zip(held, ctx_before))):
                     raise ValueError("a token of this step lies in a page that is not held")
