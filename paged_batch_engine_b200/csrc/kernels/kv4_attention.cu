@@ -19,7 +19,10 @@
 // the blocks, so one long context among short ones leaves no block idle.  A block's warps merge their parts in shared memory;
 // an item that several blocks share is merged by a second kernel, always in the blocks' order.
 //
-// Float32: queries and weights as three bfloat16 terms each, the codes are exact as they are.
+// Float32: queries and weights as three bfloat16 terms each.  There the two sums' cancellation would show (a head's output is
+// often a fortieth of its values' lo), so codes come as code - 8 (one OR and one subtraction a pair, exact) beside lo + 8 s, and
+// what they sum to is small where the output is: 2.2e-6 of the output's norm from 64 bits without, 4e-7 so
+// (a plain float32 implementation 9.5e-7).
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -108,6 +111,12 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const unsigned (&a)[4], u
 }
 __device__ __forceinline__ float low_half(unsigned w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float high_half(unsigned w) { return __uint_as_float(w & 0xffff0000u); }
+// the even codes of a word's halves, less 8, as bfloat16: 128 + code is one OR away, and 136 from it exact
+__device__ __forceinline__ unsigned centred(unsigned w) {
+  const unsigned x = (w & 0x000f000fu) | 0x43004300u, mid = 0x43084308u;
+  const __nv_bfloat162 y = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&mid));
+  return *reinterpret_cast<const unsigned*>(&y);
+}
 // x and y as pairs of N bfloat16 terms, the largest first
 template <int N>
 __device__ __forceinline__ void split(float x, float y, unsigned (&t)[N]) {
@@ -179,7 +188,7 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
   }
   const long long per_block = max((long long)MIN_UNITS, quotient(total + gridDim.x - 1, gridDim.x));
   pdl_launch_dependents();
-  const float to_log2 = p.scale * 1.4426950408889634f * CODE;
+  const float to_log2 = p.scale * 1.4426950408889634f * (TERMS == 1 ? CODE : 1.f);
 
   unsigned char* ring = smem + warp * STAGES * REC;
   long long unit = per_block * blockIdx.x;
@@ -250,6 +259,7 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
       }
     // ---- queries: B fragments (row 8 k + r8), and their sums over each group
     unsigned qb[TERMS][G * 2][NT][2], zb[NT][2];
+    float qs[NT][2][G];                                // TERMS > 1: the sums of this lane's rows of the scores
 #pragma unroll
     for (int k = 0; k < NT; ++k) {
       const int pr = pr0 + 8 * k + r8;
@@ -279,14 +289,18 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
         qsum[g] += __shfl_xor_sync(0xffffffffu, qsum[g], 2);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {                  // pair i of the word: its codes come 16 times too large for odd i
-          const float f = i & 1 ? UP / 16.f : UP;
+          const float f = TERMS > 1 ? 1.f : i & 1 ? UP / 16.f : UP;
           unsigned t[TERMS];
           split<TERMS>(x[2 * i] * f, x[2 * i + 1] * f, t);
 #pragma unroll
           for (int e = 0; e < TERMS; ++e) qb[e][2 * g + (i >> 1)][k][i & 1] = t[e];
         }
       }
-      // three terms of the sums along the product's k: term * G + g
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int g = 0; g < G; ++g) qs[k][e][g] = TERMS > 1 ? __shfl_sync(0xffffffffu, qsum[g], (2 * j + e) * 4) : 0.f;
+      // TERMS == 1: three terms of the sums along the product's k: term * G + g
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int at = 2 * j + 8 * half, term = at / G, g0 = at % G;
@@ -306,6 +320,8 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
     for (int k = 0; k < NT; ++k) m[k][0] = m[k][1] = -INFINITY;
     const unsigned mine_half = r8 & 1 ? HALF1 : HALF0, both_halves = r8 & 1 ? 0x7632 : 0x5410;
 
+    auto code = [](unsigned w) { return TERMS > 1 ? centred(w) : w & 0x000f000fu; };
+    auto code16 = [](unsigned w) { return TERMS > 1 ? centred(w >> 4) : w & 0x00f000f0u; };
     for (int i = 0; i < mine; ++i) {
       cp_wait<STAGES - 2>();
       __syncwarp();                                    // the tile has landed, and the one before is read
@@ -322,15 +338,28 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
       unsigned lo[2];
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        unsigned w[G], u[2];
+        unsigned w[G];
         words<G>(kw[n], rec + (n * 8 + r8) * (D / 2) + j * (4 * G));
         words<G>(w, num + K_S * D + (n * 4 + (r8 >> 1)) * (4 * G));
-        words<2>(u, num + K_LO * D + (n * 4 + (r8 >> 1)) * (4 * G) + (G == 4 ? (j & 1) * 8 : 0));
 #pragma unroll
         for (int g = 0; g < G; ++g) ks[n][g] = half_of(w[g], mine_half);
-        lo[n] = __byte_perm(u[0], u[1], both_halves);
+        if constexpr (TERMS == 1) {
+          unsigned u[2];
+          words<2>(u, num + K_LO * D + (n * 4 + (r8 >> 1)) * (4 * G) + (G == 4 ? (j & 1) * 8 : 0));
+          lo[n] = __byte_perm(u[0], u[1], both_halves);
+        } else {
+          words<G>(w, num + K_LO * D + (n * 4 + (r8 >> 1)) * (4 * G));
+#pragma unroll
+          for (int k = 0; k < NT; ++k)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              s[k][2 * n + e] = 0.f;
+#pragma unroll
+              for (int g = 0; g < G; ++g) s[k][2 * n + e] = fmaf(fmaf(8.f, ks[n][g], half_of(w[g], mine_half)), qs[k][e][g], s[k][2 * n + e]);
+            }
+        }
       }
-      {
+      if constexpr (TERMS == 1) {
         const unsigned a[4] = {lo[0], lo[1], lo[0], lo[1]};
 #pragma unroll
         for (int k = 0; k < NT; ++k) mma_first(s[k], a, zb[k][0], zb[k][1]);
@@ -341,7 +370,7 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const unsigned x = h ? kw[0][g] >> 8 : kw[0][g], y = h ? kw[1][g] >> 8 : kw[1][g];
-          const unsigned a[4] = {x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u};
+          const unsigned a[4] = {code(x), code(y), code16(x), code16(y)};
 #pragma unroll
           for (int k = 0; k < NT; ++k)
 #pragma unroll
@@ -424,7 +453,13 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
           }
         e_run = e_now;
       }
-      // ---- weights, and the values' lo that they weigh
+      // ---- weights, and the values' lo (or middle) that they weigh
+      if constexpr (TERMS > 1) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int g = 0; g < G; ++g) vlo[n][g] = fmaf(8.f, vs[n][g], vlo[n][g]);
+      }
       float w[NT][4];
 #pragma unroll
       for (int k = 0; k < NT; ++k)
@@ -432,7 +467,7 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
         for (int e = 0; e < 2; ++e) {
           const float off = m[k][e] == -INFINITY ? 0.f : (TERMS == 1 ? (float)(ROOM - e_run) : 0.f) - m[k][e];
 #pragma unroll
-          for (int n = 0; n < 2; ++n) w[k][2 * n + e] = TERMS == 1 ? ex2(s[k][2 * n + e] + off) : exp2f(s[k][2 * n + e] + off) * UP;
+          for (int n = 0; n < 2; ++n) w[k][2 * n + e] = TERMS == 1 ? ex2(s[k][2 * n + e] + off) : exp2f(s[k][2 * n + e] + off);
           l[k][e] += w[k][e] + w[k][2 + e];
 #pragma unroll
           for (int g = 0; g < G; ++g) z[k][g][e] = fmaf(w[k][e], vlo[0][g], fmaf(w[k][2 + e], vlo[1][g], z[k][g][e]));
@@ -457,7 +492,7 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const unsigned x = h ? v0[g] >> 8 : v0[g], y = h ? v1[g] >> 8 : v1[g];
-          const unsigned a[4] = {x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u};
+          const unsigned a[4] = {code(x), code16(x), code(y), code16(y)};
 #pragma unroll
           for (int k = 0; k < NT; ++k)
 #pragma unroll
@@ -475,7 +510,7 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
     float* om = reinterpret_cast<float*>(smem);        // [warp][row][D]
     float* mm = om + WARPS * MT * D;                   // [warp][row]
     float* lm = mm + WARPS * MT;
-    constexpr float even = TERMS == 1 ? CODE16 : CODE, odd = even / 16.f, down = TERMS == 1 ? 1.f : 1.f / UP;
+    constexpr float even = TERMS == 1 ? CODE16 : 1.f, odd = TERMS == 1 ? even / 16.f : 1.f;
     float* zm = lm + WARPS * MT;                       // [warp][row][G]
 #pragma unroll
     for (int k = 0; k < NT; ++k) {
@@ -495,7 +530,7 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
       }
       if (G == 2) v[0] += __shfl_xor_sync(0xffffffffu, v[0], 4);
       const int which = G == 4 ? r8 : r8 >> 1;
-      zm[(warp * MT + 8 * k + 2 * j + (which & 1)) * G + (which >> 1)] = v[0] * down;
+      zm[(warp * MT + 8 * k + 2 * j + (which & 1)) * G + (which >> 1)] = v[0];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
@@ -503,7 +538,7 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
         const int row = warp * MT + 8 * k + 2 * j + e;
         if (r8 == 0) {
           mm[row] = TERMS == 1 ? m[k][e] + (float)(e_run - ROOM) : m[k][e];
-          lm[row] = l[k][e] * down;
+          lm[row] = l[k][e];
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
