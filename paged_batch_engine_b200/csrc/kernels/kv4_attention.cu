@@ -17,13 +17,18 @@
 //
 // Work is cut by bytes, not by requests: the tiles of all (request, head, row tile) laid end to end are shared out evenly over
 // the blocks, so one long context among short ones leaves no block idle.  A block's warps merge their parts in shared memory;
-// an item that several blocks share is merged by a second kernel, always in the blocks' order.
+// an item that several blocks share is merged by a second kernel, always in the blocks' order.  Few items of not too many keys
+// (CLUSTER) go to a cluster of blocks each instead, which share its tiles and merge through distributed shared memory: one
+// launch less, and no parts in memory.
 //
 // Float32: queries and weights as three bfloat16 terms each.  There the two sums' cancellation would show (a head's output is
 // often a fortieth of its values' lo), so codes come as code - 8 (one OR and one subtraction a pair, exact) beside lo + 8 s, and
 // what they sum to is small where the output is: 2.2e-6 of the output's norm from 64 bits without, 4e-7 so
 // (a plain float32 implementation 9.5e-7).
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
+
+#include <atomic>
 
 #include "common.cuh"
 #include "kv4.cuh"
@@ -35,6 +40,7 @@
 using namespace pbe;
 using namespace pbe::kv4;
 using namespace pbe::mma_sync;
+namespace cg = cooperative_groups;
 
 namespace {
 struct Shared {                // an item that several blocks share, as the block that begins it notes it
@@ -143,16 +149,20 @@ __device__ __forceinline__ void words(unsigned (&w)[N], const unsigned char* p) 
   }
 }
 
-// T: the queries' type; NT: tiles of eight packed rows a warp; TERMS: bfloat16 terms of queries and weights
-template <typename T, int D, int NT, int TERMS>
+// T: the queries' type; NT: tiles of eight packed rows a warp; TERMS: bfloat16 terms of queries and weights; CLUSTER: an item
+// has a cluster of blocks
+template <typename T, int D, int NT, int TERMS, bool CLUSTER>
 __global__ void __launch_bounds__(WARPS * 32, (TERMS == 1 && (NT == 1 || D == 64)) ? 4 : 2)
 kv4_attention_kernel(Kv4AttnParams p, Split sp) {
   constexpr int G = D / GROUP, REC = rec_bytes(D), MT = 8 * NT, RING = WARPS * STAGES * REC;
   constexpr int MERGE = WARPS * MT * (D + 2 + G) * 4;
   constexpr int SHARED = RING > MERGE ? RING : MERGE;
   extern __shared__ __align__(16) unsigned char smem[];
-  long long* ends = reinterpret_cast<long long*>(smem + SHARED);     // where each request's units end
-  int4* known = reinterpret_cast<int4*>(ends + (p.requests + 1) / 2 * 2);      // its q_len, seq_len, q_start
+  float* merged = reinterpret_cast<float*>(smem + SHARED);           // CLUSTER: this block's part [row][D], then [row][2]
+  // where each request's units (CLUSTER: items) end
+  long long* ends = reinterpret_cast<long long*>(smem + SHARED + (CLUSTER ? MT * (D + 2) * 4 : 0));
+  int2* known = reinterpret_cast<int2*>(ends + p.requests);          // its q_len and seq_len
+  int* starts = reinterpret_cast<int*>(known + p.requests);          // its q_start
   __shared__ long long warp_sums[WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r8 = lane >> 2, j = lane & 3;
   const int H = p.heads, KV = p.kv_heads, HG = H / KV, per_page = p.page_tokens / REC_TOKENS;
@@ -165,10 +175,11 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
     const int r = r0 + threadIdx.x;
     long long v = 0;
     if (r < p.requests) {
-      const int4 x = make_int4(p.q_len[r], p.seq_len[r], p.q_start[r], 0);
+      const int2 x = make_int2(p.q_len[r], p.seq_len[r]);
       known[r] = x;
+      starts[r] = p.q_start[r];
       const Request q = request(p, sp, x.x, x.y, MT);
-      v = (long long)q.tiles * q.row_tiles * KV;
+      v = (long long)(CLUSTER ? 1 : q.tiles) * q.row_tiles * KV;
     }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -186,13 +197,14 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
     if (r < p.requests) ends[r] = before + v;
     __syncthreads();
   }
-  const long long per_block = max((long long)MIN_UNITS, quotient(total + gridDim.x - 1, gridDim.x));
+  const long long per_block = CLUSTER ? 0 : max((long long)MIN_UNITS, quotient(total + gridDim.x - 1, gridDim.x));
   pdl_launch_dependents();
   const float to_log2 = p.scale * 1.4426950408889634f * (TERMS == 1 ? CODE : 1.f);
 
   unsigned char* ring = smem + warp * STAGES * REC;
-  long long unit = per_block * blockIdx.x;
-  const long long unit0 = unit, unit_end = min(unit + per_block, total);
+  const int ranks = CLUSTER ? (int)cg::this_cluster().num_blocks() : 1, rank = CLUSTER ? (int)cg::this_cluster().block_rank() : 0;
+  long long unit = CLUSTER ? blockIdx.x / ranks : per_block * blockIdx.x;
+  const long long unit0 = unit, unit_end = CLUSTER ? total : min(unit + per_block, total);
   Shared note = {};
   while (unit < unit_end) {
     // ---- the next item, or this block's part of it
@@ -204,15 +216,15 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
         break;
       }
     }
-    const int4 given = known[req];
+    const int2 given = known[req];
     const Request q = request(p, sp, given.x, given.y, MT);
     const long long begin = req > 0 ? ends[req - 1] : 0;
-    const int item = (int)quotient(unit - begin, q.tiles);
-    const int t_begin = (int)((unit - begin) - (long long)item * q.tiles);
-    const int t_end = (int)min((long long)q.tiles, t_begin + (unit_end - unit));
+    const int item = (int)(CLUSTER ? unit - begin : quotient(unit - begin, q.tiles));
+    const int t_begin = (int)(CLUSTER ? (long long)q.tiles * rank / ranks : (unit - begin) - (long long)item * q.tiles);
+    const int t_end = (int)(CLUSTER ? (long long)q.tiles * (rank + 1) / ranks : min((long long)q.tiles, t_begin + (unit_end - unit)));
     const int kvh = q.row_tiles == 1 ? item : item / q.row_tiles, row_tile = item - kvh * q.row_tiles;
     const int packed = q.rows * HG, pr0 = row_tile * MT;
-    const int q0 = given.z;
+    const int q0 = starts[req];
     auto row_of = [&](int pr) { return q.rows == 1 ? 0 : pr / HG; };     // the request's row of a packed one
     const int pos_min = q.pos0 + row_of(pr0), pos_max = q.pos0 + row_of(min(pr0 + MT, packed) - 1);
     const int low_min = p.window > 0 ? pos_min - p.window + 1 : 0, low_max = p.window > 0 ? pos_max - p.window + 1 : 0;
@@ -548,14 +560,24 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
       }
     }
     __syncthreads();
-    const bool whole = t_begin == 0 && t_end == q.tiles;
+    const bool whole = !CLUSTER && t_begin == 0 && t_end == q.tiles;
     const int slot = 2 * blockIdx.x + (unit == unit0 ? 0 : 1);
-    if (t_begin == 0 && !whole) {
+    auto finish = [&](int row, int c4, float4 x, float sum) {
+      const int pr = pr0 + row, at = row_of(pr);
+      if (pr >= packed || q0 < 0 || q0 + at >= p.rows) return;
+      const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;      // a row whose scores are NaN stays NaN
+      T* dst = (T*)p.out + ((size_t)(q0 + at) * H + kvh * HG + (pr - at * HG)) * D + c4;
+      if constexpr (sizeof(T) == 2)
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(x.x * inv, x.y * inv), pack2(x.z * inv, x.w * inv));
+      else
+        *reinterpret_cast<float4*>(dst) = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+    };
+    if (!CLUSTER && t_begin == 0 && !whole) {
       const int last = (int)quotient(unit + q.tiles - 1, (int)per_block);
       note = {last - (int)blockIdx.x + 1, slot, min(MT, packed - pr0), q0, kvh * HG, pr0, {0, 0}};
     }
     for (int e = threadIdx.x; e < MT * (D / 4); e += WARPS * 32) {
-      const int row = e / (D / 4), c4 = (e % (D / 4)) * 4, pr = pr0 + row;
+      const int row = e / (D / 4), c4 = (e % (D / 4)) * 4;
       float top = -INFINITY;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) top = fmaxf(top, mm[w * MT + row]);
@@ -571,21 +593,48 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
         x.x = fmaf(f, y.x + lean, x.x), x.y = fmaf(f, y.y + lean, x.y);
         x.z = fmaf(f, y.z + lean, x.z), x.w = fmaf(f, y.w + lean, x.w);
       }
-      if (!whole) {
+      if (CLUSTER) {
+        *reinterpret_cast<float4*>(merged + row * D + c4) = x;
+        if (c4 == 0) *reinterpret_cast<float2*>(merged + MT * D + row * 2) = make_float2(top, sum);
+      } else if (!whole) {
         const size_t at = (size_t)slot * MT + row;
         *reinterpret_cast<float4*>(sp.part_o + at * D + c4) = x;
         if (c4 == 0) sp.part_ml[at * 2] = top, sp.part_ml[at * 2 + 1] = sum;
-      } else if (const int at = row_of(pr); pr < packed && q0 >= 0 && q0 + at < p.rows) {
-        const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;      // a row whose scores are NaN stays NaN
-        T* dst = (T*)p.out + ((size_t)(q0 + at) * H + kvh * HG + (pr - at * HG)) * D + c4;
-        if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(x.x * inv, x.y * inv), pack2(x.z * inv, x.w * inv));
-        else *reinterpret_cast<float4*>(dst) = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+      } else {
+        finish(row, c4, x, sum);
       }
+    }
+    if constexpr (CLUSTER) {
+      // every block merges a slice of the rows and channels of all blocks' parts, in the order of their ranks
+      cg::cluster_group cluster = cg::this_cluster();
+      cluster.sync();
+      const int each = (MT * (D / 4) + ranks - 1) / ranks;
+      for (int i = threadIdx.x; i < each && rank * each + i < MT * (D / 4); i += WARPS * 32) {
+        const int row = (rank * each + i) / (D / 4), c4 = ((rank * each + i) % (D / 4)) * 4;
+        float top = -INFINITY, sum = 0.f;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int r = 0; r < ranks; ++r) top = fmaxf(top, cluster.map_shared_rank(merged, r)[MT * D + row * 2]);
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll 8
+        for (int r = 0; r < ranks; ++r) {
+          const float* part = cluster.map_shared_rank(merged, r);
+          const float2 ml = *reinterpret_cast<const float2*>(part + MT * D + row * 2);
+          const float4 y = *reinterpret_cast<const float4*>(part + row * D + c4);
+          const float f = TERMS == 1 ? ex2(ml.x - base) : exp2f(ml.x - base);
+          sum = fmaf(f, ml.y, sum);
+          x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
+        }
+        finish(row, c4, x, sum);
+      }
+      cluster.sync();                                  // nobody's part is written anew, or gone, while it is read
+      unit += gridDim.x / ranks;
+      continue;
     }
     __syncthreads();                                   // the merged parts are read before the ring is filled again
     unit += t_end - t_begin;
   }
-  if (threadIdx.x == 0) sp.shared[blockIdx.x] = note;
+  if (!CLUSTER && threadIdx.x == 0) sp.shared[blockIdx.x] = note;
 }
 
 // Items that several blocks share: block b merges the one that block b of the kernel above began and did not end.  A warp
@@ -660,13 +709,41 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) kv4_merge_kernel(Kv4AttnPara
   }
 }
 
+// a kernel's clusters of more than eight blocks, allowed once a device
+class WideClusters {
+ public:
+  template <typename Kernel>
+  cudaError_t operator()(Kernel* kernel) {
+    int device = 0;
+    if (const cudaError_t e = cudaGetDevice(&device)) return e;
+    if (device < DEVICES && set_[device].load(std::memory_order_acquire)) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && device < DEVICES) set_[device].store(true, std::memory_order_release);
+    return e;
+  }
+
+ private:
+  static constexpr int DEVICES = 16;
+  std::atomic<bool> set_[DEVICES] = {};
+};
+
 template <typename T, int D, int NT, int TERMS>
-int launch(const Kv4AttnParams& p, const Split& sp, int blocks, bool few_items, cudaStream_t stream) {
+int launch(const Kv4AttnParams& p, const Split& sp, int blocks, int cluster, bool few_items, cudaStream_t stream) {
   constexpr int MT = 8 * NT, ring = WARPS * STAGES * rec_bytes(D), merge = WARPS * MT * (D + 2 + D / GROUP) * 4;
-  const size_t smem = (ring > merge ? ring : merge) + (size_t)(p.requests + 1) / 2 * 2 * sizeof(long long) + (size_t)p.requests * sizeof(int4);
+  const size_t lists = (size_t)p.requests * (sizeof(long long) + sizeof(int2) + sizeof(int));
+  const size_t smem = (ring > merge ? ring : merge) + lists;
+  if (cluster > 0) {
+    static OptIn opt_in;
+    static WideClusters wide;
+    const auto kernel = kv4_attention_kernel<T, D, NT, TERMS, true>;
+    if (const cudaError_t e = opt_in(smem + MT * (D + 2) * 4, kernel)) return (int)e;
+    if (const cudaError_t e = wide(kernel)) return (int)e;
+    launch_k_cluster(kernel, blocks, WARPS * 32, smem + MT * (D + 2) * 4, stream, cluster, p, sp);
+    return launch_status();
+  }
   static OptIn opt_in;
-  if (const cudaError_t e = opt_in(smem, kv4_attention_kernel<T, D, NT, TERMS>)) return (int)e;
-  launch_k(kv4_attention_kernel<T, D, NT, TERMS>, blocks, WARPS * 32, smem, stream, p, sp);
+  if (const cudaError_t e = opt_in(smem, kv4_attention_kernel<T, D, NT, TERMS, false>)) return (int)e;
+  launch_k(kv4_attention_kernel<T, D, NT, TERMS, false>, blocks, WARPS * 32, smem, stream, p, sp);
   // few items in many parts (a long context alone in its step): a quarter of an item's rows a block, four times the warps a row
   if (blocks > 1 && few_items) launch_k(kv4_merge_kernel<T, D, MT, MT / 4>, dim3(blocks - 1, 4), MERGE_WARPS * 32, 0, stream, p, sp);
   else if (blocks > 1) launch_k(kv4_merge_kernel<T, D, MT, MT>, blocks - 1, MERGE_WARPS * 32, 0, stream, p, sp);
@@ -675,14 +752,16 @@ int launch(const Kv4AttnParams& p, const Split& sp, int blocks, bool few_items, 
 
 }  // namespace
 
-// workspace: 8 floats a block, then 2 blocks * tile rows * (head_dim + 2).  tile_rows: 8, or 16
-// (bfloat16); requests of more than most_packed packed rows are left out.
+// cluster 0: the tiles are shared evenly; workspace: 8 floats a block, then 2 blocks * tile rows * (head_dim + 2).  cluster 1 to
+// 16: that many blocks an item at a time (blocks a multiple of it), no workspace.  tile_rows: 8, or 16 (bfloat16); requests of
+// more than most_packed packed rows are left out.
 PBE_EXPORT int pbe_kv4_attention(const Kv4AttnParams* params, float* workspace, int blocks, int head_dim, int tile_rows,
-                                 int most_packed, int dtype, cudaStream_t stream) {
+                                 int cluster, int most_packed, int dtype, cudaStream_t stream) {
   const Kv4AttnParams p = *params;
   if (p.requests <= 0 || p.rows <= 0) return 0;
   if (p.requests > MOST_REQUESTS || blocks < 1 || (head_dim != 64 && head_dim != 128) ||
-      !(tile_rows == 8 || (tile_rows == 16 && dtype == PBE_BF16)))
+      !(tile_rows == 8 || (tile_rows == 16 && dtype == PBE_BF16)) || cluster < 0 || cluster > 16 || (cluster > 0 && blocks % cluster) ||
+      (cluster == 0 && workspace == nullptr))
     return (int)cudaErrorInvalidValue;
   Split sp;
   sp.shared = reinterpret_cast<Shared*>(workspace);
@@ -690,10 +769,8 @@ PBE_EXPORT int pbe_kv4_attention(const Kv4AttnParams* params, float* workspace, 
   sp.part_ml = sp.part_o + (size_t)2 * blocks * tile_rows * head_dim;
   sp.most_packed = most_packed;
   const bool few_items = (long long)p.requests * p.kv_heads * 8 <= blocks;
-  if (dtype == PBE_F32)
-    return head_dim == 64 ? launch<float, 64, 1, 3>(p, sp, blocks, few_items, stream) : launch<float, 128, 1, 3>(p, sp, blocks, few_items, stream);
+  auto go = [&](auto d64, auto d128) { return (head_dim == 64 ? d64 : d128)(p, sp, blocks, cluster, few_items, stream); };
   typedef __nv_bfloat16 B;
-  if (tile_rows == 8)
-    return head_dim == 64 ? launch<B, 64, 1, 1>(p, sp, blocks, few_items, stream) : launch<B, 128, 1, 1>(p, sp, blocks, few_items, stream);
-  return head_dim == 64 ? launch<B, 64, 2, 1>(p, sp, blocks, few_items, stream) : launch<B, 128, 2, 1>(p, sp, blocks, few_items, stream);
+  if (dtype == PBE_F32) return go(launch<float, 64, 1, 3>, launch<float, 128, 1, 3>);
+  return tile_rows == 8 ? go(launch<B, 64, 1, 1>, launch<B, 128, 1, 1>) : go(launch<B, 64, 2, 1>, launch<B, 128, 2, 1>);
 }

@@ -2890,7 +2890,7 @@ def _kv4_fns() -> Kv4Fns:
     return Kv4Fns(_fn("kv4_write", "pbe_kv4_write", [c_void_p] * 7 + [c_int] * 7 + [c_ll, c_int, c_void_p]),
                   _fn("kv4_write", "pbe_kv4_read", [c_void_p] * 4 + [c_int] * 4 + [c_ll, c_int, c_void_p]),
                   _fn("kv4_attention", "pbe_kv4_attention",
-                      [ctypes.POINTER(Kv4AttnParams), c_void_p] + [c_int] * 5 + [c_void_p]))
+                      [ctypes.POINTER(Kv4AttnParams), c_void_p] + [c_int] * 6 + [c_void_p]))
 
 
 @functools.lru_cache(maxsize=None)
@@ -2903,16 +2903,29 @@ KV4_FEW_PACKED = 64         # packed rows (rows x heads of a key/value head) up 
 KV4_SPLIT_KEYS = 512        # keys of a split of the tcgen05 kernel at least
 KV4_MOST_SPLITS = 32
 KV4_UNITS = 8               # tiles of 16 keys a block takes at least, two a warp
+KV4_CLUSTER_UNITS = 32      # and at most, where a cluster of blocks takes one item
 
 
 def _kv4_shape(requests: int, heads: int, kv_heads: int, head_dim: int, most_rows: int, most_keys: int, wide: bool, sms: int):
-    """(packed rows of a tile, blocks) of the kernel for decoded tokens and short portions: as many blocks as the GPU holds
-    at once (two a multiprocessor where a warp's registers leave no more), fewer where there is less to do."""
+    """(packed rows of a tile, blocks, blocks of a cluster or 0) of the kernel for decoded tokens and short portions.  Blocks: as
+    many as the GPU holds at once (two a multiprocessor where a warp's registers leave no more), fewer where there is less to
+    do.  A cluster for each item where all are resident at once and a block of it has at most KV4_CLUSTER_UNITS tiles; clusters
+    of 16 take long to place, so they are for at most eight items.
+
+    us with clusters (of) and with tiles shared evenly, 28 heads on 4 of 128 in bfloat16: 1 request of 777 keys 6.5 (16) and
+    11.0, of 8,192 11.4 and 11.6; 8 of 777 8.5 (8) and 14.7, of 2,500 11.6 and 17.3, of 4,096 14.5 and 19.1; 16 of 1,024-4,096
+    17.9 (8) and 20.7; 32 of 375-1,500 16.1 (4) and 18.0; 64 of 194-777 15.9 (2) and 18.8.  Beyond: 64 of 625-2,500 30.9 (2)
+    and 28.7, 32 of 1,024-4,096 27.8 (4) and 25.7.  16 for 8 requests of 2,048 (32 items): 16.3, 8: 10.7."""
     tile_rows = 16 if wide and most_rows * (heads // kv_heads) > 8 else 8
     resident = sms * (4 if wide and (tile_rows == 8 or head_dim == 64) else 2)
-    row_tiles = -(-max(1, most_rows) * (heads // kv_heads) // tile_rows)
-    units = requests * row_tiles * kv_heads * (-(-max(1, most_keys) // KV4_PAGE_UNIT))
-    return tile_rows, max(1, min(-(-units // KV4_UNITS), resident))
+    items = requests * kv_heads * (-(-max(1, most_rows) * (heads // kv_heads) // tile_rows))
+    tiles = -(-max(1, most_keys) // KV4_PAGE_UNIT)
+    for cluster in (16,) if items <= 4 else (8, 16) if items <= 8 else (8, 4, 2):
+        if items * cluster <= resident and tiles <= cluster * KV4_CLUSTER_UNITS:
+            while cluster > 1 and tiles <= cluster * 2:        # half of the blocks have a tile for each of their four warps
+                cluster //= 2
+            return tile_rows, items * cluster, cluster
+    return tile_rows, max(1, min(-(-items * tiles // KV4_UNITS), resident)), 0
 
 
 def kv4_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor,
@@ -2959,10 +2972,10 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, q_sta
     params, stream = ctypes.byref(p), _stream()
     if most_packed:
         rows = min(most_rows, max(1, most_packed // group))
-        tile_rows, blocks = _kv4_shape(R, H, KV, head_dim, rows, most_keys, bf16, multiprocessors(q.device))
-        floats = 8 * blocks + 2 * blocks * tile_rows * (head_dim + 2)
-        work = torch.empty(floats, dtype=torch.float32, device=q.device)
-        _check(_kv4_fns().attention(params, work.data_ptr(), blocks, head_dim, tile_rows, most_packed, dtype, stream),
+        tile_rows, blocks, cluster = _kv4_shape(R, H, KV, head_dim, rows, most_keys, bf16, multiprocessors(q.device))
+        floats = 0 if cluster else 8 * blocks + 2 * blocks * tile_rows * (head_dim + 2)
+        work = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+        _check(_kv4_fns().attention(params, _at(work), blocks, head_dim, tile_rows, cluster, most_packed, dtype, stream),
                "kv4_attention")
     if most_packed != 0x7fffffff:
         # row tiles of 256: at most one of each request is not full

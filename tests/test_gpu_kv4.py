@@ -433,3 +433,19 @@ def test_steps_of_a_cache(dtype):
             got = out[at:at + n].cpu().double().reshape(n, H, D)
             assert float((got - want).norm() / want.norm()) <= (2 ** -7 if dtype == BF else 2 ** -17)
             at += n
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("cluster", [0, 1, 2, 4, 8, 16])
+def test_attention_every_shape_of_launch(cluster, dtype, monkeypatch):
+    """Clusters of every size, fewer of them than items, and tiles shared evenly: right, and the same rows left alone."""
+    o = ops()
+    for heads, step in (((28, 4, 128, 16), [(1, 700), (2, 300), (1, 3), (0, 9), (1, 1100)]), ((14, 2, 64, 32), [(9, 1000), (1, 40)]),
+                        ((5, 5, 128, 16), [(1, 1), (1, 15), (1, 16), (1, 17)])):
+        rows = 16 if dtype == BF and cluster % 3 == 1 else 8
+        monkeypatch.setattr(o, "_kv4_shape", lambda *a: (rows, 3 * max(cluster, 1), cluster))
+        c = Case(*heads, None, step, dtype, seed=cluster)
+        out = o.kv4_attention(*c.args(spare=2))
+        c.check(out)
+        assert (out[c.T:] == 7.0).all()
+        assert torch.equal(o.kv4_attention(*c.args(spare=2)), out)

@@ -154,3 +154,17 @@ def test_models_that_keep_no_4_bit_cache():
         _model(helpers.GUS_A)
     with pytest.raises(ValueError, match="multiple of 16"):
         ModelRunner(_model(helpers.TINY_D), page_tokens=8, num_pages=4)
+
+
+def test_shapes_of_the_direct_kernel():
+    """Blocks of clusters are whole clusters, at most what the GPU holds; what clusters do not take is shared out evenly."""
+    for requests in (1, 2, 7, 64, 500):
+        for kv, group in ((1, 1), (2, 6), (4, 7), (8, 5)):
+            for rows in (1, 3, 9):
+                for keys in (0, 1, 16, 17, 200, 777, 4096, 8192, 100000):
+                    for d, wide in ((64, True), (128, True), (128, False)):
+                        tile, blocks, cluster = ops._kv4_shape(requests, kv * group, kv, d, rows, keys, wide, 148)
+                        assert tile in (8, 16) and 1 <= blocks <= 592 and cluster in (0, 1, 2, 4, 8, 16)
+                        if cluster:
+                            assert blocks == cluster * requests * kv * -(-rows * group // tile)
+                            assert -(-keys // 16) <= cluster * ops.KV4_CLUSTER_UNITS
