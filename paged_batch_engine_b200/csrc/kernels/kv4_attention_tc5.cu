@@ -3,16 +3,22 @@
 // One block owns a row tile of 256 packed rows (query row x head of the group) of one key/value head, two halves of 128, and
 // walks over its keys in tiles of 64, four records, which both halves read once they are operands:
 //   S = Q K^T     tcgen05.mma, 128 x 64 x D, into two alternating score buffers in tensor memory for each half;
-//   softmax       warps 0-3 and 4-7, one thread a row: tcgen05.ld, maximum, exponentials, sum; weights are made against the maximum so far, which
-//                 moves only when they grow too large for it, so the output is rarely rescaled, and only then waited for;
+//   softmax       warps 0-3 and 4-7, one thread a row: tcgen05.ld, maximum, exponentials, sum; weights are made against the
+//                 maximum so far, which moves only when they grow too large for it, so the output is rarely rescaled, and only
+//                 then waited for;
 //   O += P V      P goes back into the columns of its scores and is the A operand from tensor memory.
 // Warps 8-13 turn records into operands, record after record in turn: a record's words are loaded into registers while the
 // one before is converted, and lo + s * code is one float16 multiply-add a pair of channels, since a code in the low bits of
 // a float16 is already a number (code * 2^-24).  Keys become 64 rows of D channels, values D rows of 64 keys (their words
 // hold pairs of keys, so that is how they lie), both K-major under the 128-byte swizzle, four tiles of each in flight; the
 // rows of the values are ordered (group, i, r), so that eight lanes write eight different banks, and the epilogue puts the
-// channels back in order.  Warps 14 and 15 issue the products, each those of its half.  (With one half a block and two blocks a multiprocessor each record
-// was converted twice as often, and four converting warps were what the rest waited for: 4,096 tokens 269 us.)
+// channels back in order.  Warps 14 and 15 issue the products, each those of its half.
+//
+// 4,096 tokens of 28 heads on 4 of 128: 181 us, 664 TFLOP/s (0.40 of the library products' rate; floor 72).  A tile of 256 x 64
+// takes 2,750 clocks, of which its products need 1,024 and its 16,384 exponentials 1,024 of the SM's sixteen a clock; the rest
+// is the softmax's other instructions on the same four schedulers.  With one half a block and two blocks a multiprocessor each
+// record was converted twice as often, and four converting warps were what the rest waited for: 269 us; with key tiles of 128
+// and one score buffer a half: 286.
 //
 // All operands are float16, with sums in float32: eleven bits where bfloat16 keeps eight, so the rounding of keys, values and
 // weights stays below the output's.  Ranges are kept by exponents: a row's queries, and a record's keys and values, are scaled
@@ -687,7 +693,8 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
   }
 }
 
-// The splits of a row tile and key/value head merged, a warp a row.
+// The splits of a row tile and key/value head merged, a warp a row, in MERGE_SLICES blocks.
+constexpr int MOST_SPLITS = 32, MERGE_SLICES = 16;
 template <int D>
 __global__ void __launch_bounds__(256) kv4_tc5_merge_kernel(Kv4AttnParams p, Tc5Split sp) {
   constexpr int C = D / 32;
@@ -701,18 +708,18 @@ __global__ void __launch_bounds__(256) kv4_tc5_merge_kernel(Kv4AttnParams p, Tc5
     const int pr = tile.row_tile * BM + row, q_row = pr / HG;
     if (pr >= packed || q0 < 0 || q0 + q_row >= p.rows) return;
     const size_t part0 = ((size_t)tile.index * KV + kvh) * sp.splits;
-    float top = -INFINITY;
-    for (int s = 0; s < sp.splits; ++s) top = fmaxf(top, sp.part_ml[((part0 + s) * BM + row) * 2]);
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, x[C] = {};
-#pragma unroll 4
+    // a lane's split (there are at most 32): maximum and sum, then its factor
+    const float2 ml = lane < sp.splits ? *reinterpret_cast<const float2*>(sp.part_ml + ((part0 + lane) * BM + row) * 2)
+                                       : make_float2(-INFINITY, 0.f);
+    const float top = warp_max(ml.x), mine = exp2f(ml.x - (top == -INFINITY ? 0.f : top)), sum = warp_sum(mine * ml.y);
+    float x[C] = {};
+#pragma unroll 8
     for (int s = 0; s < sp.splits; ++s) {
-      const size_t at = (part0 + s) * BM + row;
-      const float f = exp2f(sp.part_ml[at * 2] - base);
-      sum = fmaf(f, sp.part_ml[at * 2 + 1], sum);
+      const float f = __shfl_sync(0xffffffffu, mine, s);
+      const float* src = sp.part_o + ((part0 + s) * BM + row) * D + C * lane;
 #pragma unroll
       for (int c = 0; c < C; c += 2) {
-        const float2 y = *reinterpret_cast<const float2*>(sp.part_o + at * D + C * lane + c);
+        const float2 y = *reinterpret_cast<const float2*>(src + c);
         x[c] = fmaf(f, y.x, x[c]);
         x[c + 1] = fmaf(f, y.y, x[c + 1]);
       }
@@ -730,7 +737,7 @@ int launch(const Kv4AttnParams& p, const Tc5Split& sp, int tiles, int* err, cuda
   static OptIn opt_in;
   if (const cudaError_t e = opt_in(smem, kv4_attention_tc5_kernel<D>)) return (int)e;
   launch_k(kv4_attention_tc5_kernel<D>, (unsigned)(tiles * p.kv_heads * sp.splits), THREADS, smem, stream, p, sp, err);
-  if (sp.splits > 1) launch_k(kv4_tc5_merge_kernel<D>, dim3(tiles * p.kv_heads, 8), 256, 0, stream, p, sp);
+  if (sp.splits > 1) launch_k(kv4_tc5_merge_kernel<D>, dim3(tiles * p.kv_heads, MERGE_SLICES), 256, 0, stream, p, sp);
   return launch_status();
 }
 }  // namespace
@@ -741,7 +748,7 @@ PBE_EXPORT int pbe_kv4_attention_tc5(const Kv4AttnParams* params, float* workspa
                                      int most_packed, int* err, cudaStream_t stream) {
   const Kv4AttnParams p = *params;
   if (p.requests <= 0 || p.rows <= 0 || tiles <= 0) return 0;
-  if ((head_dim != 64 && head_dim != 128) || splits < 1 || !(p.scale > 0.f) || (long long)tiles * p.kv_heads * splits > 0x7fffffffLL)
+  if ((head_dim != 64 && head_dim != 128) || splits < 1 || splits > MOST_SPLITS || !(p.scale > 0.f) || (long long)tiles * p.kv_heads * splits > 0x7fffffffLL)
     return (int)cudaErrorInvalidValue;
   Tc5Split sp;
   sp.part_o = workspace;
