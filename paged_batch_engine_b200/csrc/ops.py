@@ -2800,6 +2800,7 @@ def page_maps(q_len: torch.Tensor, context: torch.Tensor, pages: Optional[torch.
 KV4_GROUP = 32              # channels that share a scale
 KV4_HEAD_DIMS = (64, 128)
 KV4_PAGE_UNIT = 16          # pages are whole records of this many tokens
+KV4_MAX_REQUESTS = 8192     # of a call of kv4_attention: their lists lie in shared memory
 
 
 def kv4_width(head_dim: int) -> int:
@@ -2821,8 +2822,9 @@ def kv4_write(qkv: torch.Tensor, bias: Optional[torch.Tensor], q_out: torch.Tens
               num_kv_heads: int, head_dim: int, rotary_dim: int, page_tokens: int, interleaved: bool = False) -> torch.Tensor:
     """q_out = rope(q + b), and rope(k + b) and v + b into 4-bit pages: ``rope_kv_write`` for a cache in four bits.  ``pages``
     is one layer's, uint8 [page, kv_head, page_tokens, kv4_width(head_dim)] (None: nothing is written); a row whose slot is
-    negative or behind the last page writes nothing.  Two rows of one call must not share a slot.  Groups of 32 channels are kept as lo + s * code, code 0..15, each off by at most s / 2 (s: a
-    fifteenth of the group's span, rounded up to bfloat16); NaN is kept as 0, what lies beyond 2^120 as 2^120."""
+    negative or behind the last page writes nothing.  Two rows of one call must not share a slot.  Groups of 32 channels are kept
+    as lo + s * code, code 0..15, each off by at most s / 2 (s: a fifteenth of the group's span, rounded up to bfloat16); NaN is
+    kept as 0, what lies beyond 2^120 as 2^120."""
     T, H, KV = qkv.shape[0], num_heads, num_kv_heads
     width = (H + 2 * KV) * head_dim
     kv4_width(head_dim)
@@ -2878,7 +2880,6 @@ def kv4_libraries(dtype: torch.dtype):
     return [("kv4_write", None), ("kv4_attention", None)] + ([("kv4_attention_tc5", None)] if dtype == torch.bfloat16 else [])
 
 
-KV4_MAX_REQUESTS = 8192
 class Kv4Fns(NamedTuple):
     write: object
     read: object

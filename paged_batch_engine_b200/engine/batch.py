@@ -294,8 +294,8 @@ class StepContext:
             raise ValueError(f"token id {int(bad)} is outside the vocabulary of {vocab_size}")
         # Steps of many rows leave the row maps and block tables to the device (one launch a layer group); the host sends the
         # lengths and the pages.
-        on_device = T >= MAPS_ROWS and torch.device(device).type == "cuda" and len(manager.groups) > 0 and \
-            all(int(getattr(g, "stride", 1) or 1) == 1 for g in manager.groups)
+        on_device = T >= MAPS_ROWS and R <= ops.MAPS_MAX_REQUESTS and torch.device(device).type == "cuda" and \
+            len(manager.groups) > 0 and all(int(getattr(g, "stride", 1) or 1) == 1 for g in manager.groups)
         if not on_device:
             req_of_tok = np.repeat(np.arange(R), q_len)
             offs = np.arange(T) - q_start[req_of_tok]
