@@ -2900,8 +2900,17 @@ def _kv4_prompt_fn():
                [ctypes.POINTER(Kv4AttnParams), c_void_p] + [c_int] * 4 + [c_void_p] * 2)
 
 
-KV4_FEW_PACKED = 64         # packed rows (rows x heads of a key/value head) up to which a request is the mma.sync kernel's
-KV4_SPLIT_KEYS = 512        # keys of a split of the tcgen05 kernel at least
+# Packed rows (rows x heads of a key/value head) up to which a request is the mma.sync kernel's.  us there and with the tcgen05 kernel,
+# 28 heads on 4 of 128: 8 requests of 2,048 keys, 63 packed rows 30.9 and 35.8, 126 45.8 and 36.0; 2 of 8,192 keys, 63 29.9 and
+# 36.5, 126 43.3 and 36.2; 8 of 8,192, 63 68.9 and 98.9, 126 119.6 and 83.4.
+KV4_FEW_PACKED = 64
+# Steps of little work are the mma.sync kernel's whatever their rows: at most two row tiles of 16 a multiprocessor and this much of
+# row tiles x tiles of 16 keys x head size.  1 request of 37 rows and 300 keys 11.9 and 25.0, 128 and 128 11.3 and 19.1 (224 row
+# tiles), 64 and 1,024 17.4 and 29.0; beyond: 8 of 16 and 1,000 30.7 and 27.5, 2 of 128 and 128 (448 row tiles) 26.6 and 21.9.
+KV4_LITTLE_WORK = 3 << 19
+# Keys of a split of the tcgen05 kernel at least: 64 rows of 2,048 keys 29.7 (512: 36.7), of 600 32.7 (34.4), 512 rows of 1,024 with
+# heads of 64 30.7 (36.7), 2 x 64 of 4,096 44.6 (44.2).
+KV4_SPLIT_KEYS = 256
 KV4_MOST_SPLITS = 32
 KV4_UNITS = 8               # tiles of 16 keys a block takes at least, two a warp
 KV4_CLUSTER_UNITS = 32      # and at most, where a cluster of blocks takes one item
@@ -2969,7 +2978,9 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, q_sta
     # its step then goes there whatever its rows); both kernels read from the lengths on the device which are theirs
     most_packed = 0x7fffffff
     if bf16 and scale > 0 and most_rows * group > KV4_FEW_PACKED:
-        most_packed = 0 if R == 1 else KV4_FEW_PACKED
+        row_tiles = R * KV * (-(-most_rows * group // 16))
+        if row_tiles > 2 * multiprocessors(q.device) or row_tiles * (-(-most_keys // 16)) * head_dim > KV4_LITTLE_WORK:
+            most_packed = 0 if R == 1 else KV4_FEW_PACKED
     params, stream = ctypes.byref(p), _stream()
     if most_packed:
         rows = min(most_rows, max(1, most_packed // group))

@@ -449,3 +449,52 @@ def test_attention_every_shape_of_launch(cluster, dtype, monkeypatch):
         c.check(out)
         assert (out[c.T:] == 7.0).all()
         assert torch.equal(o.kv4_attention(*c.args(spare=2)), out)
+
+
+# ------------------------------------------------------------------ small portions with the tcgen05 kernel too
+PORTIONS = {**{k: STEPS[k] for k in ("short_portions", "portions", "prompt", "none")}, "alone": [(3, 40)], "tail": [(129, 2000), (9, 9)]}
+
+
+@pytest.mark.parametrize("step", PORTIONS, ids=str)
+@pytest.mark.parametrize("heads", HEADS, ids=str)
+@pytest.mark.parametrize("window", [None, 37])
+def test_attention_of_portions_by_tcgen05(heads, step, window, monkeypatch):
+    """Portions too small for that kernel to be chosen: it takes them all the same."""
+    o = ops()
+    monkeypatch.setattr(o, "KV4_LITTLE_WORK", 0)
+    monkeypatch.setattr(o, "KV4_FEW_PACKED", 16)
+    c = Case(*heads, window, PORTIONS[step], BF, seed=len(step) + 1)
+    out = o.kv4_attention(*c.args(spare=3))
+    c.check(out)
+    assert (out[c.T:] == 7.0).all()
+    for splits in (1, 2, 5):                                       # shared along the keys, more splits than tiles too
+        monkeypatch.setattr(o, "multiprocessors", lambda device: 1 << 20)
+        monkeypatch.setattr(o, "KV4_SPLIT_KEYS", 1)
+        monkeypatch.setattr(o, "KV4_MOST_SPLITS", splits)
+        c.check(o.kv4_attention(*c.args(spare=3)))
+
+
+@pytest.mark.parametrize("test", [lambda: test_attention_far_scores_and_sizes(40), test_attention_pages_that_are_none,
+                                  test_attention_strided_table_and_hints, test_attention_same_bits_twice,
+                                  test_attention_captured_and_on_two_streams, lambda: test_steps_of_a_cache(BF)],
+                         ids=["sizes", "pages", "hints", "bits", "captured", "steps"])
+def test_tcgen05_again(test, monkeypatch):
+    monkeypatch.setattr(ops(), "KV4_LITTLE_WORK", 0)
+    monkeypatch.setattr(ops(), "KV4_FEW_PACKED", 1)
+    test()
+
+
+def test_little_work_goes_to_one_kernel(monkeypatch):
+    """Which kernels a call launches, by its hints."""
+    o = ops()
+    calls = []
+    real = o._kv4_prompt_fn()
+    monkeypatch.setattr(o, "_kv4_prompt_fn", lambda: lambda *a: calls.append(a[2:4]) or real(*a))
+    for step, rows, keys, there in (([(37, 300)], 37, 300, 0), ([(600, 600)], 600, 600, 1), ([(37, 300)] * 9, 37, 300, 1),
+                                    ([(37, 300)], 37, 1 << 17, 1), ([(1, 300)], 1, 1 << 17, 0)):
+        calls.clear()
+        c = Case(28, 4, 128, 16, None, step, BF, seed=7)
+        args = c.args()
+        args[13:] = [rows, keys]
+        c.check(o.kv4_attention(*args))
+        assert len(calls) == there, (step, rows, keys)

@@ -206,3 +206,13 @@ def test_step_maps_made_on_the_device(monkeypatch, window):
             assert torch.equal(x.block_table[r, :pages], y.block_table[r, :pages])
             assert (y.block_table[r, pages:] == -1).all()
     assert a.most_rows == b.most_rows == 40 and a.longest_keys == 290
+
+
+@pytest.mark.parametrize("schedule", ["whole", "mixed"])
+@pytest.mark.parametrize("name", MODELS, ids=str)
+def test_portions_by_tcgen05(folders, monkeypatch, name, schedule):
+    """The same where the tcgen05 kernel takes the portions, which it does for larger ones."""
+    from paged_batch_engine_b200.csrc import ops
+    monkeypatch.setattr(ops, "KV4_LITTLE_WORK", 0)
+    monkeypatch.setattr(ops, "KV4_FEW_PACKED", 8)
+    test_schedules_agree_with_plain(folders, monkeypatch, name, schedule, "bfloat16")
