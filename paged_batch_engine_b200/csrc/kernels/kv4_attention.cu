@@ -167,7 +167,10 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r8 = lane >> 2, j = lane & 3;
   const int H = p.heads, KV = p.kv_heads, HG = H / KV, per_page = p.page_tokens / REC_TOKENS;
   const int page_shift = (per_page & (per_page - 1)) == 0 ? 31 - __clz(per_page) : -1;
-  pdl_wait();
+  // With settled inputs only the queries and the newest keys are waited for: the lists are made, and the first tiles asked for,
+  // beside the launch that writes those.
+  bool waited = !p.settled;
+  if (waited) pdl_wait();
 
   // a unit: one tile of 16 keys for one head and row tile
   long long total = 0;
@@ -257,8 +260,17 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
       }
       cp_commit();
     };
+    if (!waited && mine > 0) {                         // tiles that hold keys of this step's own rows come after the wait
+      const int last = q.first + t_begin + warp + min(STAGES - 2, mine - 1) * WARPS;
+      if ((long long)(last + 1) * REC_TOKENS > q.pos0) {
+        pdl_wait();
+        waited = true;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i) issue(i);
+    if (!waited) pdl_wait();
+    waited = true;
 
     // this lane's rows of the scores, 8 k + 2 j and the next, and their positions
     int pos[NT][2];
@@ -634,6 +646,7 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
     __syncthreads();                                   // the merged parts are read before the ring is filled again
     unit += t_end - t_begin;
   }
+  if (!waited) pdl_wait();                             // what comes after this kernel counts on all that came before it
   if (!CLUSTER && threadIdx.x == 0) sp.shared[blockIdx.x] = note;
 }
 

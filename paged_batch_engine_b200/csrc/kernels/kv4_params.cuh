@@ -12,5 +12,6 @@ struct Kv4AttnParams {
   const int32_t* block_table;  // [requests][bt_stride], table_pages of them
   long long bt_stride;
   int table_pages, num_pages, requests, rows, heads, kv_heads, page_tokens, window;
+  int settled;                 // lengths, table and the keys before the requests' rows are older than the launch before this one
   float scale;
 };

@@ -2872,7 +2872,7 @@ def kv4_read(pages: torch.Tensor, slots: torch.Tensor, out_dtype: torch.dtype = 
 class Kv4AttnParams(ctypes.Structure):
     _fields_ = [(n, c_void_p) for n in ("q", "pages", "out", "q_start", "q_len", "seq_len", "block_table")] + \
         [("bt_stride", c_ll)] + [(n, c_int) for n in ("table_pages", "num_pages", "requests", "rows", "heads", "kv_heads",
-                                                      "page_tokens", "window")] + [("scale", c_float)]
+                                                      "page_tokens", "window", "settled")] + [("scale", c_float)]
 
 
 def kv4_libraries(dtype: torch.dtype):
@@ -2913,7 +2913,7 @@ KV4_LITTLE_WORK = 3 << 19
 KV4_SPLIT_KEYS = 256
 KV4_MOST_SPLITS = 32
 KV4_UNITS = 8               # tiles of 16 keys a block takes at least, two a warp
-KV4_CLUSTER_UNITS = 32      # and at most, where a cluster of blocks takes one item
+KV4_CLUSTER_UNITS = 48      # and at most, where a cluster of blocks takes one item
 
 
 def _kv4_shape(requests: int, heads: int, kv_heads: int, head_dim: int, most_rows: int, most_keys: int, wide: bool, sms: int):
@@ -2940,14 +2940,16 @@ def _kv4_shape(requests: int, heads: int, kv_heads: int, head_dim: int, most_row
 
 def kv4_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor,
                   seq_len: torch.Tensor, block_table: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int,
-                  scale: float, window: Optional[int], page_tokens: int, most_rows: int, most_keys: int) -> torch.Tensor:
+                  scale: float, window: Optional[int], page_tokens: int, most_rows: int, most_keys: int, settled: bool = False) -> torch.Tensor:
     """Causal attention of every row over 4-bit pages, ``paged_attention`` for a cache in four bits.  Row i of request r (row
     ``q_start[r] + i`` of q and out, both [T, H * head_dim]; no row belongs to two requests) sees the request's first
     ``seq_len[r] - q_len[r] + i + 1`` keys, or the last ``window`` of them (None or 0: all), at ``block_table[r]`` (int32 [R,
     width], rows may be strided).  A row that sees no key is 0; rows of no request are left as they are.  A key whose
     block-table entry is no page, or lies behind the table, is not seen.  ``most_rows`` and ``most_keys`` are the largest of
     q_len and seq_len as far as the host knows them: they choose the shape of the launch, not the result (beyond the order
-    of its sums).  At most ``KV4_MAX_REQUESTS`` requests."""
+    of its sums).  ``settled``: the lengths, the block table and the keys before each request's rows were complete before the
+    launch that precedes this call on the stream began (the step's own ``kv4_write``, in a step whose arrays the host sent), so
+    the kernel may begin beside it and wait for the rest.  At most ``KV4_MAX_REQUESTS`` requests."""
     H, KV, R = num_heads, num_kv_heads, q_len.numel()
     if H < 1 or KV < 1 or H % KV:
         raise KernelError("kv4_attention: num_heads must be a multiple of num_kv_heads")
@@ -2972,7 +2974,7 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, q_sta
         raise KernelError("kv4_attention: block_table must lie on the other operands' device")
     p = Kv4AttnParams(q.data_ptr(), pages.data_ptr(), out.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), seq_len.data_ptr(),
                       block_table.data_ptr(), block_table.stride(0), block_table.shape[1], pages.shape[0], R, q.shape[0], H, KV,
-                      page_tokens, window or 0, scale)
+                      page_tokens, window or 0, 1 if settled else 0, scale)
     bf16, group, T = q.dtype == torch.bfloat16, H // KV, q.shape[0]
     # requests of many packed rows go to the tcgen05 kernel, where the hint says that there may be some (a request alone in
     # its step then goes there whatever its rows); both kernels read from the lengths on the device which are theirs

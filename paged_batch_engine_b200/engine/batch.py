@@ -296,6 +296,7 @@ class StepContext:
         # lengths and the pages.
         on_device = T >= MAPS_ROWS and R <= ops.MAPS_MAX_REQUESTS and torch.device(device).type == "cuda" and \
             len(manager.groups) > 0 and all(int(getattr(g, "stride", 1) or 1) == 1 for g in manager.groups)
+        self.sent_by_host = not on_device          # all of the step's arrays: they are older than its first launch
         if not on_device:
             req_of_tok = np.repeat(np.arange(R), q_len)
             offs = np.arange(T) - q_start[req_of_tok]

@@ -68,6 +68,7 @@ class DecodeStepContext(StepContext):
         self.split_keys = choose_split_keys(batch)
         self.num_tokens = self.num_requests = self.num_wanted = batch
         self.most_rows, self.longest_keys = 1, splits * self.split_keys       # of its capacity
+        self.sent_by_host = True
         self.work_keys = list(work_keys)
         B, S = batch, splits
         off = 0

@@ -149,7 +149,7 @@ class GQAttention(Mixer):
             ops.kv4_write(qkv, bias, q, pages if cache.writes else None, kernel_positions, group.slots, inv_freq, H, KV, hd,
                           rotary_dim, ctx.page_tokens, interleaved)
             out = ops.kv4_attention(q, pages, torch.empty_like(q), ctx.q_start, ctx.q_len, ctx.seq_len, group.block_table, H, KV,
-                                    hd, self.scale, self.window, ctx.page_tokens, ctx.most_rows, ctx.longest_keys)
+                                    hd, self.scale, self.window, ctx.page_tokens, ctx.most_rows, ctx.longest_keys, ctx.sent_by_host)
             return ops.linear(out, self.w_o, self.b_o, out_dtype=self.dtype, kind=2)
         k_pages, v_pages = cache.k, cache.v
         meta = ctx.attention_work(cache.group, H // KV, self.tile_rows, self.window, H, hd)

@@ -498,3 +498,47 @@ def test_little_work_goes_to_one_kernel(monkeypatch):
         args[13:] = [rows, keys]
         c.check(o.kv4_attention(*args))
         assert len(calls) == there, (step, rows, keys)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("lens", [[0], [5, 15, 16, 17, 31, 32], [700] * 3, [4000, 3, 100], [300 + 16 * i for i in range(40)]], ids=len)
+@pytest.mark.parametrize("captured", [False, True])
+def test_attention_beside_the_write(lens, dtype, captured):
+    """``settled``: lists and older keys may be read beside the write of the step's own keys, which are waited for.  The same bits
+    as a call that waits for everything, token after token, as a record fills and the next begins."""
+    o, g = ops(), torch.Generator().manual_seed(len(lens))
+    H, KV, D, P, R = 12, 2, 128, 16, len(lens)
+    width = (max(lens) + 24) // P + 1
+    table = torch.randperm(R * width, generator=g).to(torch.int32).reshape(R, width)
+    pages = torch.full((R * width, KV, P, o.kv4_width(D)), 0xff, dtype=torch.uint8, device=DEV)
+    for r, n in enumerate(lens):
+        if n:
+            x = torch.randn(n, (H + 2 * KV) * D, generator=g).to(dtype).to(DEV)
+            slots = ints([int(table[r, p // P]) * P + p % P for p in range(n)])
+            o.kv4_write(x, None, torch.empty(n, H * D, dtype=dtype, device=DEV), pages, ints(range(n)), slots, None, H, KV, D, 0, P)
+    qkv = torch.empty(R, (H + 2 * KV) * D, dtype=dtype, device=DEV)
+    positions, slots, seq, starts, ones = (ints([0] * R) for _ in range(5))
+    starts.copy_(torch.arange(R)), ones.fill_(1)
+    q, out, want = (torch.empty(R, H * D, dtype=dtype, device=DEV) for _ in range(3))
+    bt = table.to(DEV)
+
+    def step(into, settled):
+        o.kv4_write(qkv, None, q, pages, positions, slots, None, H, KV, D, 0, P)
+        o.kv4_attention(q, pages, into, starts, ones, seq, bt, H, KV, D, D ** -0.5, None, P, 1, max(lens) + 24, settled)
+
+    graph = torch.cuda.CUDAGraph()
+    if captured:
+        slots.fill_(-1), seq.fill_(0)
+        step(out, True)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            step(out, True)
+    for t in range(20):
+        at = [n + t for n in lens]
+        qkv.copy_(torch.randn(R, (H + 2 * KV) * D, generator=g))
+        positions.copy_(torch.tensor(at)), seq.copy_(torch.tensor(at) + 1)
+        slots.copy_(torch.tensor([int(table[r, p // P]) * P + p % P for r, p in enumerate(at)]))
+        graph.replay() if captured else step(out, True)
+        torch.cuda.synchronize()
+        o.kv4_attention(q, pages, want, starts, ones, seq, bt, H, KV, D, D ** -0.5, None, P, 1, max(lens) + 24)
+        assert torch.isfinite(out).all() and torch.equal(out, want)
