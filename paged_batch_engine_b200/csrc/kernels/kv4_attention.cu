@@ -21,6 +21,11 @@
 // (CLUSTER) go to a cluster of blocks each instead, which share its tiles and merge through distributed shared memory: one
 // launch less, and no parts in memory.
 //
+// 28 heads on 4 of 128, bfloat16: 64 requests of 300 to 8,192 keys (175 MB) 57 us, 3.1 TB/s; a tile more costs what 4.7 TB/s would, the
+// rest, about 11 us, is the lists, the first loads and the merge.  A tile takes 409 instructions a warp, 185 of them on the ALU pipe
+// (80 to take codes out), and four blocks a multiprocessor issue 0.57 a scheduler and clock: bound by instructions, not by bytes.
+// One request of 131,071 keys (40 heads on 8, 168 MB) 52 us; in clusters, 8 of 2,048 keys 11 us, one of 777 7 us: chains of latency.
+//
 // Float32: queries and weights as three bfloat16 terms each.  There the two sums' cancellation would show (a head's output is
 // often a fortieth of its values' lo), so codes come as code - 8 (one OR and one subtraction a pair, exact) beside lo + 8 s, and
 // what they sum to is small where the output is: 2.2e-6 of the output's norm from 64 bits without, 4e-7 so
@@ -379,7 +384,10 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
             for (int e = 0; e < 2; ++e) {
               s[k][2 * n + e] = 0.f;
 #pragma unroll
-              for (int g = 0; g < G; ++g) s[k][2 * n + e] = fmaf(fmaf(8.f, ks[n][g], half_of(w[g], mine_half)), qs[k][e][g], s[k][2 * n + e]);
+              for (int g = 0; g < G; ++g) {
+                const float middle = fmaf(8.f, ks[n][g], half_of(w[g], mine_half));
+                s[k][2 * n + e] = fmaf(middle, qs[k][e][g], s[k][2 * n + e]);
+              }
             }
         }
       }

@@ -542,3 +542,30 @@ def test_attention_beside_the_write(lens, dtype, captured):
         torch.cuda.synchronize()
         o.kv4_attention(q, pages, want, starts, ones, seq, bt, H, KV, D, D ** -0.5, None, P, 1, max(lens) + 24)
         assert torch.isfinite(out).all() and torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("shape", [(28, 4, 128, 128, False), (14, 2, 64, 64, False), (40, 8, 128, 128, True), (1, 1, 64, 0, False),
+                                   (6, 2, 128, 96, False)], ids=str)
+def test_write_many_rows(shape, dtype):
+    """More rows than blocks: the same bytes and queries as row by row in calls of 50, also where rows in between write nothing."""
+    H, KV, D, rot, interleaved = shape
+    o, g = ops(), torch.Generator().manual_seed(H)
+    T, P = 1901, 32
+    qkv = (torch.randn(T, (H + 2 * KV) * D, generator=g) * torch.logspace(-3, 3, T)[:, None]).to(dtype).to(DEV)
+    bias = torch.randn((H + 2 * KV) * D, generator=g).to(DEV)
+    positions, order = ints(torch.randint(0, 100000, (T,), generator=g).tolist()), torch.randperm(64 * P, generator=g)[:T]
+    order[::7] = -1
+    slots = ints(order.tolist())
+    inv = (1e4 ** (-torch.arange(0, rot, 2).double() / max(rot, 1))).float().to(DEV) if rot else None
+    made = []
+    for portion in (T, 50):
+        pages = torch.full((64, KV, P, o.kv4_width(D)), 0xa5, dtype=torch.uint8, device=DEV)
+        q = torch.empty(T, H * D, dtype=dtype, device=DEV)
+        for at in range(0, T, portion):
+            some = slice(at, at + portion)
+            o.kv4_write(qkv[some], bias, q[some], pages, positions[some].clone(), slots[some].clone(), inv, H, KV, D, rot, P,
+                        interleaved)
+        made.append((pages, q))
+    assert torch.equal(made[0][0], made[1][0])
+    assert torch.equal(made[0][1], made[1][1])
