@@ -2758,11 +2758,13 @@ def _page_maps_fn():
 
 @functools.lru_cache(maxsize=256)
 def _maps_pieces(requests: int, rows: int, width: int):
-    """Sizes of the arrays of ``PageMaps`` in one buffer, each with what is left to a 16-byte boundary behind it."""
-    sizes = []
+    """Sizes of the arrays of ``PageMaps`` in one buffer, each with what is left to a 16-byte boundary behind it (where something
+    is: a view costs half a microsecond), their sum, and which pieces are the arrays."""
+    sizes, arrays = [], []
     for n in (requests, requests, rows, rows, rows, requests * width):
-        sizes += [n, -n % 4]
-    return tuple(sizes), sum(sizes)
+        arrays.append(len(sizes))
+        sizes += [n] if n % 4 == 0 else [n, -n % 4]
+    return tuple(sizes), sum(sizes), tuple(arrays)
 
 
 def page_maps(q_len: torch.Tensor, context: torch.Tensor, pages: Optional[torch.Tensor], page_tokens: int, rows: int,
@@ -2784,7 +2786,7 @@ def page_maps(q_len: torch.Tensor, context: torch.Tensor, pages: Optional[torch.
         raise KernelError("page_maps: page_tokens and stride are at least 1, rows and width not negative")
     if not 1 <= R <= MAPS_MAX_REQUESTS:
         raise KernelError(f"page_maps takes 1 to {MAPS_MAX_REQUESTS} requests, got {R}")
-    sizes, total = _maps_pieces(R, int(rows), int(width))
+    sizes, total, arrays = _maps_pieces(R, int(rows), int(width))
     if total > 0x7fffffff:
         raise KernelError("page_maps: more rows or table entries than int32 counts")
     _ready("page_maps", (), (q_len, context, pages))
@@ -2793,7 +2795,8 @@ def page_maps(q_len: torch.Tensor, context: torch.Tensor, pages: Optional[torch.
                            pages.numel() if pages is not None else 1 << 31, held.data_ptr(), R, rows, width, page_tokens, stride,
                            _stream()), "page_maps")
     parts = held.split_with_sizes(sizes)
-    return PageMaps(parts[0], parts[2], parts[4], parts[6], parts[8], parts[10].view(R, width))
+    a, b, c, d, e, table = arrays
+    return PageMaps(parts[a], parts[b], parts[c], parts[d], parts[e], parts[table].view(R, width))
 
 
 # ------------------------------------------------------------------ key/value cache in four bits
