@@ -569,3 +569,27 @@ def test_write_many_rows(shape, dtype):
         made.append((pages, q))
     assert torch.equal(made[0][0], made[1][0])
     assert torch.equal(made[0][1], made[1][1])
+
+
+@pytest.mark.parametrize("rows", [1, 460])
+def test_pages_beyond_4_gigabytes(rows):
+    """Write, read and attention (either kernel) at pages whose bytes lie behind 2^32."""
+    o, g = ops(), torch.Generator().manual_seed(rows)
+    H, KV, D, P, n = 14, 2, 128, 16, 460
+    count = (1 << 32) // (KV * P * o.kv4_width(D)) + 200
+    pages = torch.empty((count, KV, P, o.kv4_width(D)), dtype=torch.uint8, device=DEV)
+    pages[:64].fill_(0xff)
+    far = count - 1 - torch.randperm(100, generator=g)[:-(-n // P)]
+    slots = ints([int(far[p // P]) * P + p % P for p in range(n)])
+    x = torch.randn(n, (H + 2 * KV) * D, generator=g).to(BF)
+    q = torch.empty(n, H * D, dtype=BF, device=DEV)
+    o.kv4_write(x.to(DEV), None, q, pages, ints(range(n)), slots, None, H, KV, D, 0, P)
+    k, v = (y.cpu() for y in o.kv4_read(pages, slots, F32))
+    for have, want in ((k, x[:, H * D:(H + KV) * D]), (v, x[:, (H + KV) * D:])):
+        assert torch.equal(have.double(), plain.dequantise(*plain.quantise(want.double().reshape(n, KV, D))).float().double())
+    own = q[n - rows:].contiguous()
+    out = o.kv4_attention(own, pages, torch.empty_like(own), ints([0]), ints([rows]), ints([n]), far.to(torch.int32)[None].to(DEV), H,
+                          KV, D, D ** -0.5, None, P, rows, n)
+    want, *_ = plain.attention(own.cpu().reshape(rows, H, D), k, v, D ** -0.5)
+    err = (out.cpu().double().reshape(rows, H, D) - want).norm() / want.norm()
+    assert float(err) <= 2 ** -7                                   # as Case.check bounds the mean error
