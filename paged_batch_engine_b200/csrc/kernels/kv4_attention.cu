@@ -665,6 +665,7 @@ constexpr int MERGE_WARPS = 16;
 
 template <typename T, int D, int MT, int ROWS>         // MT rows a tile, ROWS of them a block
 __global__ void __launch_bounds__(MERGE_WARPS * 32) kv4_merge_kernel(Kv4AttnParams p, Split sp) {
+  static_assert(MT % ROWS == 0 && MERGE_WARPS % ROWS == 0, "a warp a row and part");
   constexpr int PARTS = MERGE_WARPS / ROWS, C = D / 32;  // C: columns a lane
   __shared__ float held[PARTS > 1 ? PARTS : 1][ROWS][D], held_m[MERGE_WARPS], held_l[MERGE_WARPS];
   pdl_launch_dependents();
