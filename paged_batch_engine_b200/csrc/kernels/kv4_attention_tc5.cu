@@ -380,6 +380,7 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
       ok = ok && mbar_wait(&empty[st], (round & 1) ^ 1, err);
       if (lane == 0) key_unit[st][rec] = seen ? pow2(e) : -1.f;
       if (lane == 16) value_exp[st][rec] = e;
+      __syncwarp();                                    // the numbers are there: each is read by other lanes than its own
       // ---- keys
       // (a record that is not seen, or a place without a key, has numbers that are zero, whatever its codes)
       unsigned char* kd = Ks + st * T_BYTES + rec * (REC_TOKENS * 128) + kt * 128;
