@@ -624,12 +624,15 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
     if (n_tiles > 0) {
       ok = ok && mbar_wait(&o_done[h], 0, err);        // o_ready may be two products behind: its parity would not tell
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    } else {
+      ok = ok && mbar_wait(&q_full[h], 0, err);        // another warp's queries still come to where this one's rows are laid
     }
     // l is in units of 2^(m_run - ROOM), the output in units of 2^e_run more
     const float back = n_tiles > 0 ? pow2(e_run) : 0.f;
     const float inv = sp.splits > 1 ? back : l_run > 0.f ? back / l_run : l_run == 0.f ? 0.f : l_run;
     const size_t part = ((size_t)tile.index * KV + kvh) * sp.splits + split;
-    // rows are stored whole too, through shared memory that held queries (no product of this half reads them any more)
+    // rows are stored whole too, through shared memory that held queries (all of the half's warps have laid theirs down, and no
+    // product reads them any more)
     unsigned char* stage = Qs + h * (HALF * D * 2) + (warp & 3) * (32 * D * 2);        // [32 rows][LANES chunks of 16 bytes]
     auto place = [&](int to, int c) { return stage + (to * LANES + (c ^ (to & 7))) * 16; };
     const unsigned own = held ? (unsigned)(((size_t)(q0 + q_row) * H + head) * LANES) : 0xffffffffu;

@@ -20,3 +20,12 @@ def test_numbers_of_a_record_are_read_behind_a_barrier_of_the_warp():
     assert len(stores) == 3 and len(reads) == 4                     # the code was found and understood
     assert max(stores) < min(reads) and "__syncwarp()" in loop[max(stores):min(reads)]
     assert "__syncwarp()" in loop[:min(stores)] and "__syncwarp()" in loop[max(reads):]
+
+
+def test_rows_are_staged_behind_all_queries_of_their_half():
+    """Outputs are laid where queries were.  The last product has waited for all of a half's queries; a block without a key tile has
+    no product, and waits for the queries themselves."""
+    text = _source("kv4_attention_tc5.cu")
+    staged = text.index("unsigned char* stage = Qs")
+    before = text[text.rindex("pdl_launch_dependents()", 0, staged):staged]
+    assert re.search(r"if \(n_tiles > 0\) \{[^}]*mbar_wait\(&o_done\[h\][^}]*\} else \{[^}]*mbar_wait\(&q_full\[h\]", before)
