@@ -346,9 +346,16 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
     }
 
     float o[NT][2 * G][4] = {}, z[NT][G][2] = {}, m[NT][2], l[NT][2] = {};
-    int e_run = -MOST_E;
+    float e_run[NT][2];                                // a row's exponent: whole numbers, as they enter the weights' exponent
+    int e_low = MOST_E;                                // the least of the lane's; rows that are none have the most
 #pragma unroll
-    for (int k = 0; k < NT; ++k) m[k][0] = m[k][1] = -INFINITY;
+    for (int k = 0; k < NT; ++k)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[k][e] = -INFINITY;
+        e_run[k][e] = pos[k][e] < 0 ? MOST_E : -MOST_E;
+        e_low = min(e_low, pos[k][e] < 0 ? MOST_E : -MOST_E);
+      }
     const unsigned mine_half = r8 & 1 ? HALF1 : HALF0, both_halves = r8 & 1 ? 0x7632 : 0x5410;
 
     auto code = [](unsigned w) { return TERMS > 1 ? centred(w) : w & 0x000f000fu; };
@@ -452,40 +459,44 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
           }
         }
       }
-      // ---- the running maximum, moved only when it grew by more than 2^8, or with it the largest exponent of the values' s
+      // ---- the running maximum, moved only when it grew by more than 2^8, or with it the largest exponent of the values' s that
+      // the row has seen (a row's own: what it does not see leaves its weights as they are)
       bool grew = false;
 #pragma unroll
       for (int k = 0; k < NT; ++k)
 #pragma unroll
         for (int e = 0; e < 2; ++e) grew = grew || fmaxf(s[k][e], s[k][2 + e]) > m[k][e] + 8.f;
-      unsigned large = 0;
+      float large[2] = {0.f, 0.f};
       if constexpr (TERMS == 1) {
-        float most = 0.f;
 #pragma unroll
-        for (int g = 0; g < G; ++g) most = fmaxf(most, fmaxf(vs[0][g], vs[1][g]));
-        large = __float_as_uint(most) >> 23;
-        grew = grew || (int)large - 127 > e_run;
+        for (int g = 0; g < G; ++g) large[0] = fmaxf(large[0], vs[0][g]), large[1] = fmaxf(large[1], vs[1][g]);
+        grew = grew || (int)(__float_as_uint(fmaxf(large[0], large[1])) >> 23) - 127 > e_low;
       }
       if (__any_sync(0xffffffffu, grew)) {
-        int e_now = e_run;
-        if constexpr (TERMS == 1) e_now = max(e_run, min((int)__reduce_max_sync(0xffffffffu, large) - 127, MOST_E));
+        e_low = MOST_E;
 #pragma unroll
         for (int k = 0; k < NT; ++k)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             float top = fmaxf(s[k][e], s[k][2 + e]);
+            float most = fmaxf(s[k][e] == -INFINITY ? 0.f : large[0], s[k][2 + e] == -INFINITY ? 0.f : large[1]);
 #pragma unroll
-            for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            for (int off = 4; off < 32; off <<= 1) {
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+              if constexpr (TERMS == 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+            }
             top = fmaxf(top, m[k][e]);
-            const float a = top == -INFINITY ? 1.f : ex2(m[k][e] - top + (float)(e_run - e_now));
+            const int e_now = TERMS == 1 ? max((int)e_run[k][e], min((int)(__float_as_uint(most) >> 23) - 127, MOST_E)) : 0;
+            const float a = top == -INFINITY ? 1.f : ex2(m[k][e] - top + (TERMS == 1 ? e_run[k][e] - (float)e_now : 0.f));
             m[k][e] = top;
+            e_run[k][e] = e_now;
+            e_low = min(e_low, e_now);
             l[k][e] *= a;
 #pragma unroll
             for (int c = 0; c < 2 * G; ++c) o[k][c][e] *= a, o[k][c][2 + e] *= a;
 #pragma unroll
             for (int g = 0; g < G; ++g) z[k][g][e] *= a;
           }
-        e_run = e_now;
       }
       // ---- weights, and the values' lo (or middle) that they weigh
       if constexpr (TERMS > 1) {
@@ -499,7 +510,7 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
       for (int k = 0; k < NT; ++k)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float off = m[k][e] == -INFINITY ? 0.f : (TERMS == 1 ? (float)(ROOM - e_run) : 0.f) - m[k][e];
+          const float off = m[k][e] == -INFINITY ? 0.f : (TERMS == 1 ? ROOM - e_run[k][e] : 0.f) - m[k][e];
 #pragma unroll
           for (int n = 0; n < 2; ++n) w[k][2 * n + e] = TERMS == 1 ? ex2(s[k][2 * n + e] + off) : exp2f(s[k][2 * n + e] + off);
           l[k][e] += w[k][e] + w[k][2 + e];
@@ -571,7 +582,7 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
         for (int off = 4; off < 32; off <<= 1) l[k][e] += __shfl_xor_sync(0xffffffffu, l[k][e], off);
         const int row = warp * MT + 8 * k + 2 * j + e;
         if (r8 == 0) {
-          mm[row] = TERMS == 1 ? m[k][e] + (float)(e_run - ROOM) : m[k][e];
+          mm[row] = TERMS == 1 ? m[k][e] + (e_run[k][e] - ROOM) : m[k][e];
           lm[row] = l[k][e];
         }
 #pragma unroll

@@ -1,4 +1,5 @@
-"""Attention over 4-bit pages where it can go wrong at its edges: row tiles without a key, queries that are NaN, pages that are none.
+"""Attention over 4-bit pages where it can go wrong at its edges: row tiles without a key, queries that are NaN, pages that are
+none, tokens that a row does not see.
 
 Tolerances are those of ``test_gpu_kv4.Case.check`` unless a test says otherwise; outputs of rows without a key are zero exactly.
 """
@@ -94,3 +95,54 @@ def test_portions_see_no_key_of_a_page_that_is_none(short, splits, dtype, monkey
         assert (got[blind] == 0).all()
         err = (got - o).norm(dim=(1, 2)) / o.norm(dim=(1, 2)).clamp_min(2 ** -10)
         assert float(err.max()) <= (2 ** -6 if dtype == BF else 2 ** -16)
+
+
+# ------------------------------------------------------------------ what a row does not see
+def check_rows(c, out):
+    """``Case.check`` row by row: nothing but the keys that a row sees enters its tolerance."""
+    at = 0
+    for (rows, n), (k, v) in zip(c.step, c.kv):
+        q = c.q[at:at + rows].reshape(rows, c.H, c.D)
+        got = out[at:at + rows].cpu().double().reshape(rows, c.H, c.D)
+        at += rows
+        o, heavy, spread, reach = plain.attention(q, k, v, c.scale, c.window)
+        pos, key = torch.arange(n - rows, n)[:, None], torch.arange(n)[None]
+        see = (key <= pos) & (key > pos - (c.window or n))
+        lean = 2 * torch.where(see, v.abs().amax((1, 2))[None], 0.0).amax(1)[:, None, None]
+        step, d = 2 ** -8 if c.dtype == BF else 2 ** -22, 2 ** -8 if c.dtype == BF else 2 ** -18
+        tol = 2 * step * (heavy + lean) + 2 ** -24 * (n / 16 + 64) * (heavy + lean) + step * o.abs() \
+            + 2 * d * c.scale * reach[..., None] * spread
+        err = (got - o).abs()
+        assert torch.isfinite(got).all() and (err <= tol).all(), (rows, n, float((err / tol).max()))
+        # and in a row's mean far nearer, but for rows whose scores a large key decides
+        calm = ~(see & (k.abs().amax((1, 2)) > 50)[None]).any(1)
+        rel = (err.norm(dim=(1, 2)) / o.norm(dim=(1, 2)))[calm]
+        assert (rel <= (2 ** -6 if c.dtype == BF else 2 ** -16)).all(), (rows, n, rel)
+
+
+def large_token(place, size, which):
+    def edit(k, v):
+        for x in which:
+            if place < len(k):
+                (k if x == "k" else v)[place] *= 2.0 ** size
+    return edit
+
+
+FORMS = [(BF, False), (F32, False)]
+
+
+@pytest.mark.parametrize("dtype,prompt", FORMS, ids=str)
+@pytest.mark.parametrize("heads", [(14, 2, 64, 16), (4, 4, 128, 32)], ids=str)
+@pytest.mark.parametrize("window", [None, 3])
+@pytest.mark.parametrize("which", ["v", "k"])
+@pytest.mark.parametrize("size", [7, 12, 20, 30, 50])
+@pytest.mark.parametrize("place", [71, 72, 79, 80])
+def test_a_token_that_a_row_does_not_see_leaves_it_alone(place, size, which, window, heads, dtype, prompt, monkeypatch):
+    """A token of 2^size times the others' keys or values, in the record of the rows' own keys and behind it: rows before it are as
+    near as without it, and so are rows whose window has left it behind."""
+    if "k" in which and size > 30:
+        size = 30                                                  # scores of such keys leave float32 sooner than values
+    if prompt:
+        by_tcgen05(monkeypatch)
+    c = Case(*heads, window, [(9, 76), (9, 84)], dtype, seed=place, edit=large_token(place, size, which))
+    check_rows(c, ops().kv4_attention(*c.args()))
