@@ -510,9 +510,13 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
       for (int k = 0; k < NT; ++k)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float off = m[k][e] == -INFINITY ? 0.f : (TERMS == 1 ? ROOM - e_run[k][e] : 0.f) - m[k][e];
+          // the difference first: it is exact near the maximum, however far that is from zero
+          const float top = m[k][e] == -INFINITY ? 0.f : m[k][e];
 #pragma unroll
-          for (int n = 0; n < 2; ++n) w[k][2 * n + e] = TERMS == 1 ? ex2(s[k][2 * n + e] + off) : exp2f(s[k][2 * n + e] + off);
+          for (int n = 0; n < 2; ++n) {
+            const float d = s[k][2 * n + e] - top;
+            w[k][2 * n + e] = TERMS == 1 ? ex2(d + (ROOM - e_run[k][e])) : exp2f(d);
+          }
           l[k][e] += w[k][e] + w[k][2 + e];
 #pragma unroll
           for (int g = 0; g < G; ++g) z[k][g][e] = fmaf(w[k][e], vlo[0][g], fmaf(w[k][2 + e], vlo[1][g], z[k][g][e]));
@@ -559,11 +563,14 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
     float* zm = lm + WARPS * MT;                       // [warp][row][G]
 #pragma unroll
     for (int k = 0; k < NT; ++k) {
+      float unit[2];                                   // of the row's weights
+#pragma unroll
+      for (int e = 0; e < 2; ++e) unit[e] = TERMS == 1 ? ex2(e_run[k][e] - ROOM) : 1.f;
       // the sums over the keys' lanes of the values' lo: by halves, so that lane r8 is left with one of the 2 G sums (two
       // lanes with the same one where there are four)
       float v[2 * G];
 #pragma unroll
-      for (int i = 0; i < 2 * G; ++i) v[i] = z[k][i >> 1][i & 1];
+      for (int i = 0; i < 2 * G; ++i) v[i] = z[k][i >> 1][i & 1] * unit[i & 1];
 #pragma unroll
       for (int n = G, off = 16; n > 0; n >>= 1, off >>= 1) {
         const bool up = lane & off;
@@ -582,13 +589,13 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
         for (int off = 4; off < 32; off <<= 1) l[k][e] += __shfl_xor_sync(0xffffffffu, l[k][e], off);
         const int row = warp * MT + 8 * k + 2 * j + e;
         if (r8 == 0) {
-          mm[row] = TERMS == 1 ? m[k][e] + (e_run[k][e] - ROOM) : m[k][e];
-          lm[row] = l[k][e];
+          mm[row] = m[k][e];
+          lm[row] = l[k][e] * unit[e];
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          const float(&a)[4] = o[k][2 * g], (&b)[4] = o[k][2 * g + 1];
-          *reinterpret_cast<float4*>(om + row * D + 32 * g + 4 * r8) = make_float4(a[e] * even, a[2 + e] * odd, b[e] * even, b[2 + e] * odd);
+          const float(&a)[4] = o[k][2 * g], (&b)[4] = o[k][2 * g + 1], x = even * unit[e], y = odd * unit[e];
+          *reinterpret_cast<float4*>(om + row * D + 32 * g + 4 * r8) = make_float4(a[e] * x, a[2 + e] * y, b[e] * x, b[2 + e] * y);
         }
       }
     }

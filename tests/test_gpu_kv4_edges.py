@@ -146,3 +146,51 @@ def test_a_token_that_a_row_does_not_see_leaves_it_alone(place, size, which, win
         by_tcgen05(monkeypatch)
     c = Case(*heads, window, [(9, 76), (9, 84)], dtype, seed=place, edit=large_token(place, size, which))
     check_rows(c, ops().kv4_attention(*c.args()))
+
+
+# ------------------------------------------------------------------ scores far from zero
+FAR = [(BF, False), (F32, False)]
+
+
+@pytest.mark.parametrize("dtype,prompt", FAR, ids=str)
+@pytest.mark.parametrize("heads", [(14, 2, 64, 16), (4, 4, 128, 32)], ids=str)
+@pytest.mark.parametrize("rows", [1, 9])
+@pytest.mark.parametrize("size", [10, 20, 23, 25, 30, 45])
+def test_scores_far_from_zero(size, rows, heads, dtype, prompt, monkeypatch):
+    """Queries of 2^size: one key has all of a row's weight, and the output is its value, where no other key's score comes near.
+
+    A score is off by at most 2^-8 of its reach (as in ``Case.check``): rows whose second score is within twice that of the
+    first are not looked at, but for being finite."""
+    if prompt:
+        by_tcgen05(monkeypatch)
+    step = [(rows, 500), (rows, 77)]
+    c = Case(*heads, None, step, dtype, seed=size, q_scale=2.0 ** size)
+    out = ops().kv4_attention(*c.args()).cpu().double().reshape(c.T, c.H, c.D)
+    assert torch.isfinite(out).all()
+    at, looked = 0, 0
+    for (n, keys), (k, v) in zip(step, c.kv):
+        q = c.q[at:at + n].double().reshape(n, c.KV, -1, c.D)
+        s = torch.einsum("nkgd,tkd->nkgt", q, k) * c.scale
+        reach = torch.einsum("nkgd,tkd->nkgt", q.abs(), k.abs()).amax(-1) * c.scale
+        see = torch.arange(keys)[None] <= torch.arange(keys - n, keys)[:, None]
+        two = s.masked_fill(~see[:, None, None], float("-inf")).topk(2, -1)
+        clear = two.values[..., 0] - two.values[..., 1] > 2 * 2 ** -8 * reach + 60.0
+        want = torch.gather(v.permute(1, 0, 2)[None, :, None].expand(n, -1, q.shape[2], -1, -1), 3,
+                            two.indices[..., :1, None].expand(-1, -1, -1, -1, c.D))[..., 0, :]
+        err = (out[at:at + n].reshape(want.shape) - want).abs()[clear]
+        assert (err <= (2 ** -7 if dtype == BF else 2 ** -17) * 3 * v.abs().max()).all()
+        looked += int(clear.sum())
+        at += n
+    assert looked > c.T * c.H // 2
+
+
+@pytest.mark.parametrize("dtype,prompt", FAR, ids=str)
+@pytest.mark.parametrize("size", [20, 30, 50])
+@pytest.mark.parametrize("place", [71, 72, 79, 80])
+def test_a_token_of_large_key_and_value(place, size, dtype, prompt, monkeypatch):
+    """Its score decides the rows that see it, whatever its size; the rows that do not stay as near as without it."""
+    if prompt:
+        by_tcgen05(monkeypatch)
+    for heads in ((14, 2, 64, 16), (4, 4, 128, 32)):
+        c = Case(*heads, None, [(9, 76), (9, 84)], dtype, seed=place, edit=large_token(place, size, "kv"))
+        check_rows(c, ops().kv4_attention(*c.args()))
