@@ -23,7 +23,10 @@
 // All operands are float16, with sums in float32: eleven bits where bfloat16 keeps eight, so the rounding of keys, values and
 // weights stays below the output's.  Ranges are kept by exponents: a row's queries, and a record's keys and values, are scaled
 // by powers of two that the softmax takes out again (keys in the factor before the exponential, values as an offset within
-// it, with a running reference for the output's unit).  Spans of keys and values from 2^-60 to 2^60 are held.
+// it, with a running reference for the output's unit).  Spans of keys and values from 2^-60 to 2^60 are held.  The reference is a
+// row's own, made of what it sees, and a record whose tokens lie far apart has units for each (weigh_one_by_one), so no token
+// that a row does not see takes its bits.  A value whose span is 2^-20 of the largest that the row sees has its weight in eleven
+// bits; below that it loses them, and counts for nothing from 2^-31 on.
 //
 // A block takes all of tensor memory (two halves of two score buffers of 64 columns and an output of up to 128).  Few row
 // tiles with many keys are split along the keys and merged by a second kernel.  Every mbarrier wait is bounded; one that runs
@@ -52,6 +55,7 @@ constexpr int TMEM_COLS = 512;
 constexpr int S_COL = 0, O_COL = 256;   // of half h: two score buffers at 128 h, the output at 256 + 128 h
 constexpr int ROOM = 6;                 // weights are kept 2^6 times too large: float16 reaches further down
 constexpr int MOST_E = 60;
+constexpr int EVEN = 8, UNEVEN = 1024;  // exponents that the tokens of a record may lie apart and share a unit; the mark of others
 
 struct Tc5Split {
   float* part_o;               // [tiles * KV * splits][256][D]
@@ -191,6 +195,62 @@ __device__ __forceinline__ Tile tile_of(const Kv4AttnParams& p, int most_packed,
   return {-1, 0, target, 0, 0, 0};
 }
 
+// what a tile's operands count in
+struct alignas(16) Units {
+  float key[RECS];             // 2^exponent of a record's keys, negative: no key of it is seen
+  int value[RECS];             // exponent of its values, and UNEVEN more where its tokens have exponents of their own:
+  int key_exp[BN], value_exp[BN];
+};
+
+// A row's weights of one tile, one by one: for tiles with uneven records.  The same steps as in the kernel's loop below, out of
+// its way and its registers.
+struct Weighed {
+  float m, shrink, alpha, sum;
+  int e;
+};
+__device__ __noinline__ Weighed weigh_one_by_one(const Units* u, uint32_t s_addr, int ts, int lo, int pos, float row_unit, float m_run, int e_run) {
+  float mx = -INFINITY, s[REC_TOKENS];
+  int e_new = e_run;
+  auto scores = [&](int g) {
+    tmem_ld16(s_addr + g * REC_TOKENS, s);
+    const float key = u->key[g];
+    const bool own = u->value[g] >= UNEVEN / 2;
+#pragma unroll
+    for (int i = 0; i < REC_TOKENS; ++i) {
+      const int at = ts + g * REC_TOKENS + i;
+      s[i] = at <= pos && at >= lo && key > 0.f ? s[i] * ((own ? pow2(u->key_exp[g * REC_TOKENS + i]) : key) * row_unit) : -INFINITY;
+    }
+  };
+  auto exponent = [&](int g, int i) { return u->value[g] >= UNEVEN / 2 ? u->value_exp[g * REC_TOKENS + i] : u->value[g]; };
+#pragma unroll 1
+  for (int g = 0; g < RECS; ++g) {
+    scores(g);
+#pragma unroll
+    for (int i = 0; i < REC_TOKENS; ++i) {
+      mx = fmaxf(mx, s[i]);
+      if (s[i] != -INFINITY) e_new = max(e_new, exponent(g, i));
+    }
+  }
+  float m_new = fmaxf(m_run, mx);
+  if (m_run != -INFINITY && m_new - m_run <= 8.0f) m_new = m_run;
+  const float m_use = m_new == -INFINITY ? 0.f : m_new;
+  uint32_t w[BN / 2];
+  float sum = 0.f;
+#pragma unroll
+  for (int g = 0; g < RECS; ++g) {
+    scores(g);
+#pragma unroll
+    for (int i = 0; i < REC_TOKENS; i += 2) {
+      const float x = ex2(s[i] - m_use + ROOM), y = ex2(s[i + 1] - m_use + ROOM);
+      sum += x + y;
+      w[(g * REC_TOKENS + i) / 2] = h2(x * pow2(exponent(g, i) - e_new), y * pow2(exponent(g, i + 1) - e_new));
+    }
+  }
+  tmem_st32_nowait(s_addr, &w[0]);
+  const float shrink = ex2(m_run - m_use);
+  return {m_new, shrink, shrink * ex2((float)(e_run - e_new)), sum, e_new};
+}
+
 // N words from shared memory, as wide as they come
 template <int N>
 __device__ __forceinline__ void words(unsigned (&w)[N], const unsigned* p) {
@@ -217,8 +277,7 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
   unsigned char* Vs = Ks + STAGES * T_BYTES;           // [STAGES][D rows][64 keys: 128 B]
   unsigned* nums = reinterpret_cast<unsigned*>(Vs + STAGES * T_BYTES);   // [CONV][keys s, lo: 16 tokens x G; values s, lo: 8 pairs x G]
   __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], s_full[2][2], p_full[2][2], o_ready[2], o_done[2], q_full[2];
-  __shared__ float key_unit[STAGES][RECS];              // 2^exponent of a record's keys, negative: no key of it is seen
-  __shared__ int value_exp[STAGES][RECS];
+  __shared__ Units units[STAGES];
   __shared__ uint32_t tmem_base_smem;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
@@ -349,21 +408,35 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
       // places that hold no key of this row tile may hold anything: their numbers count as zero
       const unsigned keep = !seen ? 0u : (key <= pos_max && key >= low_min ? 0xffffu : 0u) |
                                              (key + 1 <= pos_max && key + 1 >= low_min ? 0xffff0000u : 0u);
-      unsigned most = 0;
+      unsigned most[2] = {0, 0};                       // of the two tokens
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         nw[g] &= keep;
-        most = max(most, max(nw[g] & 0x7fffu, (nw[g] >> 16) & 0x7fffu));
+        most[0] = max(most[0], nw[g] & 0x7fffu);
+        most[1] = max(most[1], (nw[g] >> 16) & 0x7fffu);
       }
       // kinds by eights of lanes: lo and s of keys, lo and s of values.  The unit is such that s reaches up to 2^-8 and lo
       // stays within float16
-      const int e_own = (int)(most >> 7) - 127 + (kind & 1 ? 9 : -14);
+      const int e_own = (int)(max(most[0], most[1]) >> 7) - 127 + (kind & 1 ? 9 : -14);
       const int e = max(-MOST_E, min(MOST_E + 9, lane < 16 ? __reduce_max_sync(0x0000ffffu, e_own) : __reduce_max_sync(0xffff0000u, e_own)));
-      const float by = pow2((kind & 1 ? 24 : 0) - e);
+      // A token whose s is far below the record's largest number would lose its bits to that, and to rows that see no larger one it
+      // is all there is: the tokens of such a record have units of their own.  (Within EVEN the shared unit leaves 2^-12 of s * 15.)
+      const bool far = (kind & 1) && ((keep & 0xffffu && (int)(most[0] >> 7) - 127 + 9 < e - EVEN) ||
+                                      (keep >> 16 && (int)(most[1] >> 7) - 127 + 9 < e - EVEN));
+      const bool own_units = __any_sync(0xffffffffu, far);
+      int e_tok[2] = {e, e};
+      if (own_units) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int e_i = (int)(most[i] >> 7) - 127 + (kind & 1 ? 9 : -14);
+          e_tok[i] = max(-MOST_E, min(MOST_E + 9, max(e_i, __shfl_xor_sync(0xffffffffu, e_i, 8))));
+        }
+      }
+      const float by[2] = {pow2((kind & 1 ? 24 : 0) - e_tok[0]), pow2((kind & 1 ? 24 : 0) - e_tok[1])};
       unsigned half[G];
 #pragma unroll
       for (int g = 0; g < G; ++g)
-        half[g] = h2(__uint_as_float(nw[g] << 16) * by, __uint_as_float(nw[g] & 0xffff0000u) * by);
+        half[g] = h2(__uint_as_float(nw[g] << 16) * by[0], __uint_as_float(nw[g] & 0xffff0000u) * by[1]);
       __syncwarp();                                    // the numbers of the tile before are read
       if (kind < 2) {
         unsigned* dst = kn + (kind == K_S ? 0 : 16 * G) + 2 * np * G;
@@ -378,8 +451,13 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
         for (int g = 0; g < G; ++g) dst[g] = half[g];
       }
       ok = ok && mbar_wait(&empty[st], (round & 1) ^ 1, err);
-      if (lane == 0) key_unit[st][rec] = seen ? pow2(e) : -1.f;
-      if (lane == 16) value_exp[st][rec] = e;
+      if (lane == 0) units[st].key[rec] = seen ? pow2(e) : -1.f;
+      if (lane == 16) units[st].value[rec] = own_units ? e + UNEVEN : e;
+      if (own_units && !(kind & 1)) {
+        int* exps = (kind == K_LO ? units[st].key_exp : units[st].value_exp) + rec * REC_TOKENS + 2 * np;
+        exps[0] = e_tok[0];
+        exps[1] = e_tok[1];
+      }
       __syncwarp();                                    // the numbers are there: each is read by other lanes than its own
       // ---- keys
       // (a record that is not seen, or a place without a key, has numbers that are zero, whatever its codes)
@@ -510,95 +588,111 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
     const uint32_t lane_addr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t s_addr = lane_addr + S_COL + h * 128, o_addr = lane_addr + O_COL + h * 128;
     float m_run = -INFINITY, l_run = 0.f;              // maximum in units of log2
-    int e_run = -2 * MOST_E;                           // the output's unit: 2^(e_run - ROOM + m_run)
+    int e_run = row_valid ? -2 * MOST_E : MOST_E + 9;  // the output's unit: 2^(e_run - ROOM + m_run); rows that are none have the most
     bool ok = true;
     for (int j = 0; j < n_tiles; ++j) {
       const int st = j & 1, kst = j % STAGES, ts = (t_begin + j) * BN;
       ok = ok && mbar_wait(&s_full[h][st], (j >> 1) & 1, err);
       ok = ok && mbar_wait(&full[kst], (j / STAGES) & 1, err);              // complete, but for the exponents beside it
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      float s[BN];
-      auto fetch = [&]() {
+      const Units& u = units[kst];
+      float m_new = m_run, alpha = 1.f;
+      int e_new = max(max(u.value[0], u.value[1]), max(u.value[2], u.value[3]));
+      if (e_new >= UNEVEN / 2) {                       // tokens with units of their own: a few tiles if any
+        const Weighed x = weigh_one_by_one(&u, s_addr + st * BN, ts, lo, pos, row_unit, m_run, e_run);
+        m_new = x.m, e_new = x.e, alpha = x.alpha;
+        l_run = fmaf(l_run, x.shrink, x.sum);
+      } else {
+        float s[BN];
+        auto fetch = [&]() {
 #pragma unroll
-        for (int c = 0; c < BN / 32; ++c) tmem_ld32_nowait(s_addr + st * BN + c * 32, &s[c * 32]);
-      };
-      fetch();
-      float unit[RECS];
-      int ev[RECS];
-      bool whole = ts + BN - 1 <= pos_min && ts >= low_max;
-#pragma unroll
-      for (int g = 0; g < RECS; ++g) {
-        unit[g] = key_unit[kst][g] * row_unit;
-        ev[g] = value_exp[kst][g];
-        whole = whole && unit[g] > 0.f;
-      }
-      int e_new = max(e_run, max(max(ev[0], ev[1]), max(ev[2], ev[3])));
-      float m_new = m_run, sum, most;
-      uint32_t w[BN / 2];
-      // weights from the scores, against the maximum so far; their sum, in units of 2^(m_new - ROOM), and the largest part of it
-      auto weigh = [&]() {
-        const float m_use = m_new == -INFINITY ? 0.f : m_new;
-        sum = most = 0.f;
+          for (int c = 0; c < BN / 32; ++c) tmem_ld32_nowait(s_addr + st * BN + c * 32, &s[c * 32]);
+        };
+        fetch();
+        float unit[RECS];
+        int ev[RECS];
+        bool whole = ts + BN - 1 <= pos_min && ts >= low_max;
 #pragma unroll
         for (int g = 0; g < RECS; ++g) {
-          const float off = (float)(ROOM + ev[g] - e_new) - m_use;
-          const f32x2 unit2 = both(unit[g], unit[g]), off2 = both(off, off);
-          f32x2 part = both(0.f, 0.f);
+          unit[g] = u.key[g] * row_unit;
+          ev[g] = u.value[g];
+          whole = whole && unit[g] > 0.f;
+        }
+        if (!whole) {                                  // of the records that the row sees
+          e_new = e_run;
 #pragma unroll
-          for (int i = g * 16; i < g * 16 + 16; i += 2) {
-            float x, y;
-            apart(fma2(both(s[i], s[i + 1]), unit2, off2), x, y);
-            x = ex2(x);
-            y = ex2(y);
-            part = add2(part, both(x, y));
-            w[i / 2] = h2(x, y);
+          for (int g = 0; g < RECS; ++g) {
+            const int first = ts + g * REC_TOKENS;
+            if (first <= pos && first + REC_TOKENS > lo) e_new = max(e_new, ev[g]);
           }
-          float x, y;
-          apart(part, x, y);
-          most = fmaxf(most, x + y);
-          sum = fmaf(x + y, ex2((float)min(e_new - ev[g], 126)), sum);
         }
-      };
-      auto masked = [&]() {
+        e_new = max(e_run, e_new);
+        float sum, most, shrink = 1.f;
+        uint32_t w[BN / 2];
+        // weights from the scores, against the maximum so far; their sum, in units of 2^(m_new - ROOM), and the largest part of it
+        auto weigh = [&]() {
+          const float m_use = m_new == -INFINITY ? 0.f : m_new;
+          sum = most = 0.f;
 #pragma unroll
-        for (int i = 0; i < BN; ++i) {
-          const int key = ts + i;
-          if (key > pos || key < lo || !(key_unit[kst][i / REC_TOKENS] > 0.f)) s[i] = -INFINITY;
-        }
+          for (int g = 0; g < RECS; ++g) {
+            const float off = (float)(ROOM + ev[g] - e_new) - m_use;
+            const f32x2 unit2 = both(unit[g], unit[g]), off2 = both(off, off);
+            f32x2 part = both(0.f, 0.f);
 #pragma unroll
-        for (int g = 0; g < RECS; ++g) unit[g] = fabsf(unit[g]);
-      };
-      tmem_landed(s);
-      if (!whole) masked();
-      // Weights first, without a look at this tile's maximum: while no sum of 16 passes 2^15 none of them is too large for
-      // float16.  Where one does, or none was seen before, or larger values come, the maximum is found and moved (to no more
-      // than 2^8 below it) and the weights are made again: a few tiles of a row.
-      weigh();
-      float alpha = 1.f, shrink = 1.f;
-      const bool again = !(most <= 32768.f) || m_run == -INFINITY || e_new > e_run;
-      if (__any_sync(0xffffffffu, again)) {
-        fetch();
+            for (int i = g * 16; i < g * 16 + 16; i += 2) {
+              float x, y;
+              apart(fma2(both(s[i], s[i + 1]), unit2, off2), x, y);
+              x = ex2(x);
+              y = ex2(y);
+              part = add2(part, both(x, y));
+              w[i / 2] = h2(x, y);
+            }
+            float x, y;
+            apart(part, x, y);
+            most = fmaxf(most, x + y);
+            sum = fmaf(x + y, ex2((float)min(e_new - ev[g], 126)), sum);
+          }
+        };
+        auto masked = [&]() {
+#pragma unroll
+          for (int i = 0; i < BN; ++i) {
+            const int key = ts + i;
+            if (key > pos || key < lo || !(u.key[i / REC_TOKENS] > 0.f)) s[i] = -INFINITY;
+          }
+#pragma unroll
+          for (int g = 0; g < RECS; ++g) unit[g] = fabsf(unit[g]);
+        };
         tmem_landed(s);
         if (!whole) masked();
-        float mx = -INFINITY;
-#pragma unroll
-        for (int g = 0; g < RECS; ++g) {
-          float a = s[g * 16], b = s[g * 16 + 1];
-#pragma unroll
-          for (int i = 2; i < 16; i += 2) {
-            a = fmaxf(a, s[g * 16 + i]);
-            b = fmaxf(b, s[g * 16 + i + 1]);
-          }
-          mx = fmaxf(mx, fmaxf(a, b) * unit[g]);
-        }
-        m_new = fmaxf(m_run, mx);
-        if (m_run != -INFINITY && m_new - m_run <= 8.0f) m_new = m_run;
-        shrink = ex2(m_run - (m_new == -INFINITY ? 0.f : m_new));
-        alpha = shrink * ex2((float)(e_run - e_new));
+        // Weights first, without a look at this tile's maximum: while no sum of 16 passes 2^15 none of them is too large for
+        // float16.  Where one does, or none was seen before, or larger values come, the maximum is found and moved (to no more
+        // than 2^8 below it) and the weights are made again: a few tiles of a row.
         weigh();
+        const bool again = !(most <= 32768.f) || m_run == -INFINITY || e_new > e_run;
+        if (__any_sync(0xffffffffu, again)) {
+          fetch();
+          tmem_landed(s);
+          if (!whole) masked();
+          float mx = -INFINITY;
+#pragma unroll
+          for (int g = 0; g < RECS; ++g) {
+            float a = s[g * 16], b = s[g * 16 + 1];
+#pragma unroll
+            for (int i = 2; i < 16; i += 2) {
+              a = fmaxf(a, s[g * 16 + i]);
+              b = fmaxf(b, s[g * 16 + i + 1]);
+            }
+            mx = fmaxf(mx, fmaxf(a, b) * unit[g]);
+          }
+          m_new = fmaxf(m_run, mx);
+          if (m_run != -INFINITY && m_new - m_run <= 8.0f) m_new = m_run;
+          shrink = ex2(m_run - (m_new == -INFINITY ? 0.f : m_new));
+          alpha = shrink * ex2((float)(e_run - e_new));
+          weigh();
+        }
+        l_run = fmaf(l_run, shrink, sum);
+        tmem_st32_nowait(s_addr + st * BN, &w[0]);
       }
-      l_run = fmaf(l_run, shrink, sum);
-      tmem_st32_nowait(s_addr + st * BN, &w[0]);
       // only a rescaled output has to wait for the product before (the scores of tile j came after that of tile j - 2)
       if (j > 0 && __any_sync(0xffffffffu, m_new > m_run || e_new > e_run)) {
         ok = ok && mbar_wait(&o_ready[h], (j - 1) & 1, err);

@@ -128,7 +128,7 @@ def large_token(place, size, which):
     return edit
 
 
-FORMS = [(BF, False), (F32, False)]
+FORMS = [(BF, False), (F32, False), (BF, True)]
 
 
 @pytest.mark.parametrize("dtype,prompt", FORMS, ids=str)
