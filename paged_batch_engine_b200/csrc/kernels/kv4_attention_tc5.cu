@@ -55,6 +55,7 @@ constexpr int TMEM_COLS = 512;
 constexpr int S_COL = 0, O_COL = 256;   // of half h: two score buffers at 128 h, the output at 256 + 128 h
 constexpr int ROOM = 6;                 // weights are kept 2^6 times too large: float16 reaches further down
 constexpr int MOST_E = 60;
+constexpr float FAR = 16384.f;          // beyond this maximum weights are made one by one: its rounding in float32 is 2^-11
 constexpr int EVEN = 8, UNEVEN = 1024;  // exponents that the tokens of a record may lie apart and share a unit; the mark of others
 
 struct Tc5Split {
@@ -202,8 +203,8 @@ struct alignas(16) Units {
   int key_exp[BN], value_exp[BN];
 };
 
-// A row's weights of one tile, one by one: for tiles with uneven records.  The same steps as in the kernel's loop below, out of
-// its way and its registers.
+// A row's weights of one tile, one by one: for tiles with uneven records, and for rows whose scores are so far from zero that the
+// exponents cannot be added to the maximum.  The same steps as in the kernel's loop below, out of its way and its registers.
 struct Weighed {
   float m, shrink, alpha, sum;
   int e;
@@ -589,20 +590,20 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
     const uint32_t s_addr = lane_addr + S_COL + h * 128, o_addr = lane_addr + O_COL + h * 128;
     float m_run = -INFINITY, l_run = 0.f;              // maximum in units of log2
     int e_run = row_valid ? -2 * MOST_E : MOST_E + 9;  // the output's unit: 2^(e_run - ROOM + m_run); rows that are none have the most
-    bool ok = true;
+    bool ok = true, far = false;                       // far: a row of the warp has its maximum far from zero
+    auto is_far = [](float m) { return __any_sync(0xffffffffu, fabsf(m) > FAR && m != -INFINITY) != 0; };
     for (int j = 0; j < n_tiles; ++j) {
       const int st = j & 1, kst = j % STAGES, ts = (t_begin + j) * BN;
       ok = ok && mbar_wait(&s_full[h][st], (j >> 1) & 1, err);
       ok = ok && mbar_wait(&full[kst], (j / STAGES) & 1, err);              // complete, but for the exponents beside it
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const Units& u = units[kst];
+      const float l_was = l_run;
       float m_new = m_run, alpha = 1.f;
       int e_new = max(max(u.value[0], u.value[1]), max(u.value[2], u.value[3]));
-      if (e_new >= UNEVEN / 2) {                       // tokens with units of their own: a few tiles if any
-        const Weighed x = weigh_one_by_one(&u, s_addr + st * BN, ts, lo, pos, row_unit, m_run, e_run);
-        m_new = x.m, e_new = x.e, alpha = x.alpha;
-        l_run = fmaf(l_run, x.shrink, x.sum);
-      } else {
+      // tokens with units of their own, or scores far from zero: a few tiles if any
+      bool one_by_one = far || e_new >= UNEVEN / 2;
+      if (!one_by_one) {
         float s[BN];
         auto fetch = [&]() {
 #pragma unroll
@@ -688,10 +689,17 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
           if (m_run != -INFINITY && m_new - m_run <= 8.0f) m_new = m_run;
           shrink = ex2(m_run - (m_new == -INFINITY ? 0.f : m_new));
           alpha = shrink * ex2((float)(e_run - e_new));
+          one_by_one = far = is_far(m_new);
           weigh();
         }
         l_run = fmaf(l_run, shrink, sum);
-        tmem_st32_nowait(s_addr + st * BN, &w[0]);
+        if (!one_by_one) tmem_st32_nowait(s_addr + st * BN, &w[0]);
+      }
+      if (one_by_one) {
+        const Weighed x = weigh_one_by_one(&u, s_addr + st * BN, ts, lo, pos, row_unit, m_run, e_run);
+        m_new = x.m, e_new = x.e, alpha = x.alpha;
+        l_run = fmaf(l_was, x.shrink, x.sum);
+        far = is_far(m_new);
       }
       // only a rescaled output has to wait for the product before (the scores of tile j came after that of tile j - 2)
       if (j > 0 && __any_sync(0xffffffffu, m_new > m_run || e_new > e_run)) {

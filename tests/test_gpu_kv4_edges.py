@@ -149,7 +149,7 @@ def test_a_token_that_a_row_does_not_see_leaves_it_alone(place, size, which, win
 
 
 # ------------------------------------------------------------------ scores far from zero
-FAR = [(BF, False), (F32, False)]
+FAR = [(BF, False), (F32, False), (BF, True)]
 
 
 @pytest.mark.parametrize("dtype,prompt", FAR, ids=str)
