@@ -83,7 +83,7 @@ __device__ __forceinline__ Request request(const Kv4AttnParams& p, const Split& 
   q.pos0 = q.seq - q.rows;
   const long long packed = (long long)q.rows * (p.heads / p.kv_heads);
   q.row_tiles = packed > s.most_packed ? 0 : (int)((packed + tile_rows - 1) / tile_rows);      // tile_rows: 8 or 16
-  const int low = p.window > 0 ? max(0, q.pos0 - p.window + 1) : 0;
+  const int low = p.window > 0 ? max(0, max(0, q.pos0) - p.window + 1) : 0;    // (rows before the first key see none)
   q.first = low / REC_TOKENS;
   q.tiles = max(1, (int)(((unsigned)q.seq + REC_TOKENS - 1) / REC_TOKENS) - q.first);
   return q;
@@ -237,7 +237,7 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
     const int q0 = starts[req];
     auto row_of = [&](int pr) { return q.rows == 1 ? 0 : pr / HG; };     // the request's row of a packed one
     const int pos_min = q.pos0 + row_of(pr0), pos_max = q.pos0 + row_of(min(pr0 + MT, packed) - 1);
-    const int low_min = p.window > 0 ? pos_min - p.window + 1 : 0, low_max = p.window > 0 ? pos_max - p.window + 1 : 0;
+    const int low_min = p.window > 0 ? max(0, pos_min) - p.window + 1 : 0, low_max = p.window > 0 ? max(0, pos_max) - p.window + 1 : 0;
 
     // ---- this warp's tiles, t_begin + warp, + 8, ...: the first are on their way before the queries are looked at
     const int mine = t_end - t_begin > warp ? (t_end - t_begin - warp + WARPS - 1) / WARPS : 0;

@@ -291,7 +291,8 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
   const int packed = nq * HG, pr0 = tile.row_tile * BM, rows_here = min(BM, packed - pr0);
   const int pos0 = seq - nq;
   const int pos_min = pos0 + pr0 / HG, pos_max = pos0 + (pr0 + rows_here - 1) / HG;
-  const int low_min = p.window > 0 ? max(0, pos_min - p.window + 1) : 0, low_max = p.window > 0 ? pos_max - p.window + 1 : 0;
+  // (rows before the first key see none; a window of 2^31 - 1 taken from their positions would not fit an int)
+  const int low_min = p.window > 0 ? max(0, max(0, pos_min) - p.window + 1) : 0, low_max = p.window > 0 ? max(0, pos_max) - p.window + 1 : 0;
   const int tile_lo = low_min / BN, tile_hi = pos_max >= 0 ? pos_max / BN + 1 : 0;
   const int all_tiles = max(0, tile_hi - tile_lo);
   const int t_begin = tile_lo + (int)((long long)all_tiles * split / sp.splits);
@@ -548,7 +549,7 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
     const int q_row = row_valid ? pr / HG : 0, head = kvh * HG + (row_valid ? pr - q_row * HG : 0);
     const bool held = row_valid && q0 >= 0 && q0 + q_row < p.rows;
     const int pos = row_valid ? pos0 + q_row : -1;
-    const int lo = p.window > 0 ? pos - p.window + 1 : 0;
+    const int lo = p.window > 0 ? max(0, pos) - p.window + 1 : 0;
     // ---- the warp's 32 rows of queries as float16, each scaled by a power of two so that its largest lies in [1, 2); the lanes
     // load whole rows (a thread loading its own asks for 32 lines an instruction, and the first records wait behind them)
     float row_unit;

@@ -2977,7 +2977,7 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, q_sta
         raise KernelError("kv4_attention: block_table must lie on the other operands' device")
     p = Kv4AttnParams(q.data_ptr(), pages.data_ptr(), out.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), seq_len.data_ptr(),
                       block_table.data_ptr(), block_table.stride(0), block_table.shape[1], pages.shape[0], R, q.shape[0], H, KV,
-                      page_tokens, window or 0, 1 if settled else 0, scale)
+                      page_tokens, min(window or 0, 0x7fffffff), 1 if settled else 0, scale)
     bf16, group, T = q.dtype == torch.bfloat16, H // KV, q.shape[0]
     # requests of many packed rows go to the tcgen05 kernel, where the hint says that there may be some (a request alone in
     # its step then goes there whatever its rows); both kernels read from the lengths on the device which are theirs

@@ -194,3 +194,19 @@ def test_a_token_of_large_key_and_value(place, size, dtype, prompt, monkeypatch)
     for heads in ((14, 2, 64, 16), (4, 4, 128, 32)):
         c = Case(*heads, None, [(9, 76), (9, 84)], dtype, seed=place, edit=large_token(place, size, "kv"))
         check_rows(c, ops().kv4_attention(*c.args()))
+
+
+# ------------------------------------------------------------------ windows that hold every key
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5], ids=str)
+@pytest.mark.parametrize("step", [[(3, 2), (5, 40), (1, 0)], [(300, 20), (2, 0), (40, 40)]], ids=str)
+def test_windows_longer_than_any_request(step, window, prompt, monkeypatch):
+    """The same bits as without a window, for rows before the first key too."""
+    if prompt:
+        by_tcgen05(monkeypatch)
+    c = Case(14, 2, 64, 16, None, step, BF, seed=3)
+    want = ops().kv4_attention(*c.args()).clone()
+    c.check(want)
+    args = c.args()
+    args[11] = window
+    assert torch.equal(ops().kv4_attention(*args), want)
