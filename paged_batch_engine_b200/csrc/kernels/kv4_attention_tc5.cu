@@ -662,7 +662,7 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
             if (key > pos || key < lo || !(u.key[i / REC_TOKENS] > 0.f)) s[i] = -INFINITY;
           }
 #pragma unroll
-          for (int g = 0; g < RECS; ++g) unit[g] = fabsf(unit[g]);
+          for (int g = 0; g < RECS; ++g) unit[g] = fmaxf(fabsf(unit[g]), 1e-37f);      // times minus infinity: not 0
         };
         tmem_landed(s);
         if (!whole) masked();

@@ -196,7 +196,7 @@ def test_a_token_of_large_key_and_value(place, size, dtype, prompt, monkeypatch)
         check_rows(c, ops().kv4_attention(*c.args()))
 
 
-# ------------------------------------------------------------------ windows that hold every key
+# ------------------------------------------------------------------ windows that hold every key, scales that leave nothing
 @pytest.mark.parametrize("prompt", [False, True])
 @pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5], ids=str)
 @pytest.mark.parametrize("step", [[(3, 2), (5, 40), (1, 0)], [(300, 20), (2, 0), (40, 40)]], ids=str)
@@ -210,3 +210,16 @@ def test_windows_longer_than_any_request(step, window, prompt, monkeypatch):
     args = c.args()
     args[11] = window
     assert torch.equal(ops().kv4_attention(*args), want)
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("scale", [1e-10, 1e-30])
+def test_scores_that_are_nothing(scale, prompt, monkeypatch):
+    """Queries, or queries and keys, of zero under a scale that brings their units out of float32's range: plain means of the values."""
+    if prompt:
+        by_tcgen05(monkeypatch)
+    for edit in (None, lambda k, v: k.zero_()):
+        c = Case(14, 2, 64, 16, 37, [(40, 90), (1, 70)], BF, seed=4, edit=edit)
+        c.q.zero_()
+        c.scale = scale
+        c.check(ops().kv4_attention(*c.args()))
