@@ -359,7 +359,8 @@ PBE_EXPORT int pbe_kv4_write(const void* qkv, const float* bias, void* q_out, vo
                              int rotary_dim, int page_tokens, int interleaved, long long num_pages, int dtype,
                              cudaStream_t stream) {
   if (rows <= 0) return 0;
-  if (rotary_dim < 0 || rotary_dim > head_dim || (rotary_dim & 1) || head_dim % GROUP != 0 || page_tokens % REC_TOKENS != 0)
+  if (heads < 1 || kv_heads < 1 || rotary_dim < 0 || rotary_dim > head_dim || (rotary_dim & 1) || head_dim % GROUP != 0 ||
+      page_tokens % REC_TOKENS != 0)
     return (int)cudaErrorInvalidValue;
   WriteParams p{qkv, bias, q_out, (unsigned char*)pages, positions, slots, inv_freq, rows, heads, kv_heads, head_dim,
                 rotary_dim, page_tokens, interleaved, num_pages * page_tokens};
@@ -387,7 +388,8 @@ PBE_EXPORT int pbe_kv4_write(const void* qkv, const float* bias, void* q_out, vo
 PBE_EXPORT int pbe_kv4_read(const void* pages, const int32_t* slots, void* k, void* v, int rows, int kv_heads, int head_dim,
                             int page_tokens, long long num_pages, int dtype, cudaStream_t stream) {
   if (rows <= 0) return 0;
-  if (head_dim % GROUP != 0 || page_tokens % REC_TOKENS != 0) return (int)cudaErrorInvalidValue;
+  if (kv_heads < 1 || head_dim < GROUP || head_dim % GROUP != 0 || page_tokens < 1 || page_tokens % REC_TOKENS != 0)
+    return (int)cudaErrorInvalidValue;
   const int across = kv_heads * (head_dim / 8) < 128 ? kv_heads * (head_dim / 8) : 128;
   const dim3 threads(across, 128 / across);
   const unsigned blocks = (unsigned)((rows + threads.y - 1) / threads.y);

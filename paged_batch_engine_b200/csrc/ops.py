@@ -2814,6 +2814,8 @@ def kv4_width(head_dim: int) -> int:
 
 
 def _kv4_pages(what: str, pages: torch.Tensor, kv_heads: int, page_tokens: int, head_dim: int) -> None:
+    if kv_heads < 1:
+        raise KernelError(f"{what}: a page has at least one key/value head, got {kv_heads}")
     if page_tokens < 1 or page_tokens % KV4_PAGE_UNIT:
         raise KernelError(f"{what}: a page holds a multiple of {KV4_PAGE_UNIT} tokens, got {page_tokens}")
     if pages.dtype != torch.uint8 or pages.dim() != 4 or pages.shape[1:] != (kv_heads, page_tokens, kv4_width(head_dim)):
@@ -2832,6 +2834,8 @@ def kv4_write(qkv: torch.Tensor, bias: Optional[torch.Tensor], q_out: torch.Tens
     width = (H + 2 * KV) * head_dim
     kv4_width(head_dim)
     dtype = _dtype_code(qkv)
+    if H < 1 or KV < 1:
+        raise KernelError(f"kv4_write: at least one query head and one key/value head, got {H} and {KV}")
     if qkv.dim() != 2 or qkv.shape[1] != width or q_out.shape != (T, H * head_dim) or q_out.dtype != qkv.dtype:
         raise KernelError("kv4_write: shapes or dtypes do not agree")
     if bias is not None and (bias.dtype != torch.float32 or bias.numel() != width):
