@@ -855,7 +855,9 @@ PBE_EXPORT int pbe_kv4_attention_tc5(const Kv4AttnParams* params, float* workspa
                                      int most_packed, int* err, cudaStream_t stream) {
   const Kv4AttnParams p = *params;
   if (p.requests <= 0 || p.rows <= 0 || tiles <= 0) return 0;
-  if ((head_dim != 64 && head_dim != 128) || splits < 1 || splits > MOST_SPLITS || !(p.scale > 0.f) || (long long)tiles * p.kv_heads * splits > 0x7fffffffLL)
+  // (rows of queries and outputs are counted by eight numbers in 32 bits)
+  if ((head_dim != 64 && head_dim != 128) || splits < 1 || splits > MOST_SPLITS || !(p.scale > 0.f) ||
+      (long long)tiles * p.kv_heads * splits > 0x7fffffffLL || (long long)p.rows * p.heads * (head_dim / 8) >= 0xffffffffLL)
     return (int)cudaErrorInvalidValue;
   Tc5Split sp;
   sp.part_o = workspace;

@@ -2919,6 +2919,7 @@ KV4_LITTLE_WORK = 3 << 19
 # heads of 64 30.7 (36.7), 2 x 64 of 4,096 44.6 (44.2).
 KV4_SPLIT_KEYS = 256
 KV4_MOST_SPLITS = 32
+KV4_PROMPT_NUMBERS = 1 << 34  # most numbers of q for the tcgen05 kernel, which counts them by eights in 32 bits
 KV4_UNITS = 8               # tiles of 16 keys a block takes at least, two a warp
 KV4_CLUSTER_UNITS = 48      # and at most, where a cluster of blocks takes one item
 
@@ -2986,7 +2987,7 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, q_sta
     # requests of many packed rows go to the tcgen05 kernel, where the hint says that there may be some (a request alone in
     # its step then goes there whatever its rows); both kernels read from the lengths on the device which are theirs
     most_packed = 0x7fffffff
-    if bf16 and scale > 0 and most_rows * group > KV4_FEW_PACKED:
+    if bf16 and scale > 0 and most_rows * group > KV4_FEW_PACKED and q.numel() <= KV4_PROMPT_NUMBERS:
         row_tiles = R * KV * (-(-most_rows * group // 16))
         if row_tiles > 2 * multiprocessors(q.device) or row_tiles * (-(-most_keys // 16)) * head_dim > KV4_LITTLE_WORK:
             most_packed = 0 if R == 1 else KV4_FEW_PACKED

@@ -20,3 +20,24 @@ def test_no_heads():
             ops.kv4_write(**_write_args(**change))
     with pytest.raises(ops.KernelError, match="multiple"):
         ops.kv4_attention(**_attn_args(num_heads=0, num_kv_heads=0, q=wide, out=wide, pages=none))
+
+
+def test_queries_beyond_the_prompt_kernels_counting(monkeypatch):
+    """The tcgen05 kernel counts rows of queries by eight numbers in 32 bits: calls with more go to the other kernel."""
+    calls = []
+
+    def library(name):
+        return lambda *a: calls.append(name) or 0
+    monkeypatch.setattr(ops, "_ready", lambda *a: None)
+    monkeypatch.setattr(ops, "_stream", lambda: None)
+    monkeypatch.setattr(ops, "multiprocessors", lambda device: 148)
+    monkeypatch.setattr(ops, "tc5_attention_error_buffer", lambda device: torch.zeros(1, dtype=torch.int32))
+    monkeypatch.setattr(ops, "_kv4_prompt_fn", lambda: library("prompt"))
+    monkeypatch.setattr(ops, "_kv4_fns", lambda: ops.Kv4Fns(None, None, library("few")))
+    for rows, there in ((1 << 20, ["prompt"]), (1 << 25, ["few"])):
+        calls.clear()
+        q = torch.empty(rows, 16 * 64, dtype=torch.bfloat16, device="meta")
+        one = torch.zeros(1, dtype=torch.int32, device="meta")
+        ops.kv4_attention(q, torch.empty(5, 2, 16, 80, dtype=torch.uint8, device="meta"), torch.empty_like(q), one, one, one,
+                          torch.zeros(1, 4, dtype=torch.int32, device="meta"), 16, 2, 64, 0.1, None, 16, rows, rows)
+        assert calls == there
