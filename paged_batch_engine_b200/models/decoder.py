@@ -13,7 +13,7 @@ import torch
 from ..config.specs import ModelSpec
 from ..csrc import ops
 from ..csrc.build import compile_many
-from ..parts.base import build_block, build_part
+from ..parts.base import build_block, build_part, has_pages
 from ..weights.loader import ParamSpec
 
 
@@ -96,6 +96,8 @@ class DecoderModel:
     def kernel_libraries(self):
         from ..csrc import ops
         jobs = [("elementwise", None)] + ops.gemm_libraries(self.dtype)
+        if any(has_pages(need) for need in self.cache_needs):
+            jobs.append(("page_maps", None))          # a step of many rows has its maps made by it (StepContext)
         for b in self.blocks:
             jobs += b.kernel_libraries(self.dtype)
         for norm in (self.embedding_norm, self.final_norm):

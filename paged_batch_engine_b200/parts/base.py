@@ -108,6 +108,13 @@ class CompositeNeed:
         return CompositeNeed(tuple(parts.items()))
 
 
+def has_pages(need) -> bool:
+    """Whether a cache need, or a part of it, lies in pages."""
+    if isinstance(need, CompositeNeed):
+        return any(has_pages(part) for _, part in need.parts)
+    return need is not None and not isinstance(need, StateNeed)
+
+
 class Part:
     def param_specs(self, prefix: str) -> List[ParamSpec]:
         return []
