@@ -2822,6 +2822,12 @@ def _kv4_pages(what: str, pages: torch.Tensor, kv_heads: int, page_tokens: int, 
         raise KernelError(f"{what}: pages must be uint8 [page, kv_head, page_tokens, {kv4_width(head_dim)}]")
 
 
+def kv4_write_fits(num_kv_heads: int, head_dim: int, rotary_dim: int, interleaved: bool = False) -> bool:
+    """Whether ``kv4_write`` takes these heads: the form for rotations by halves of a part of the channels lays all keys and values
+    of a row in 48 KB of shared memory; the others keep rows in registers and take any number."""
+    return interleaved or rotary_dim in (0, head_dim) or 2 * num_kv_heads * head_dim * 4 + rotary_dim * 4 <= 48 * 1024
+
+
 def kv4_write(qkv: torch.Tensor, bias: Optional[torch.Tensor], q_out: torch.Tensor, pages: Optional[torch.Tensor],
               positions: torch.Tensor, slots: Optional[torch.Tensor], inv_freq: Optional[torch.Tensor], num_heads: int,
               num_kv_heads: int, head_dim: int, rotary_dim: int, page_tokens: int, interleaved: bool = False) -> torch.Tensor:
@@ -2851,8 +2857,9 @@ def kv4_write(qkv: torch.Tensor, bias: Optional[torch.Tensor], q_out: torch.Tens
     elif rotary_dim % 2 or not 0 <= rotary_dim <= head_dim or inv_freq.dtype != torch.float32 \
             or inv_freq.numel() != rotary_dim // 2:
         raise KernelError("kv4_write: inv_freq must be float32 [rotary_dim / 2], rotary_dim even and at most head_dim")
-    if 2 * KV * head_dim * 4 + rotary_dim * 4 > 48 * 1024:
-        raise KernelError(f"kv4_write: {KV} key/value heads of {head_dim} do not fit in shared memory")
+    if not kv4_write_fits(KV, head_dim, rotary_dim, interleaved):
+        raise KernelError(f"kv4_write: {KV} key/value heads of {head_dim}, {rotary_dim} channels rotated by halves, do not fit in "
+                          "shared memory")
     _ready("kv4_write", (qkv, bias, q_out, pages), (positions, slots, inv_freq))
     _check(_kv4_fns().write(qkv.data_ptr(), _at(bias), q_out.data_ptr(), _at(pages), positions.data_ptr(), _at(slots),
                             _at(inv_freq), T, H, KV, head_dim, rotary_dim, page_tokens, 1 if interleaved else 0,

@@ -62,6 +62,10 @@ class GQAttention(Mixer):
         if bits != 4 or self.head_dim not in ops.KV4_HEAD_DIMS:
             raise ConfigError(f"attention keeps a cache in 4 bits for head sizes {ops.KV4_HEAD_DIMS}; asked for {bits} bits, "
                               f"head size {self.head_dim}")
+        inv_freq, rotary_dim, interleaved = (None, 0, False) if self.position.applies_itself else self.position.kernel_args()
+        if not ops.kv4_write_fits(self.num_kv_heads, self.head_dim, rotary_dim if inv_freq is not None else 0, interleaved):
+            raise ConfigError(f"attention keeps no cache in 4 bits for {self.num_kv_heads} key/value heads of {self.head_dim} of which "
+                              f"{rotary_dim} channels are rotated by halves")
         self.cache_bits, self.shaped_by_keys = bits, True
 
     def work_keys(self):

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from tests.plain import plain_kv4 as plain
+from tests import test_gpu_kv4
 from tests.test_gpu_kv4 import BF, DEV, F32, Case, ops
 
 pytestmark = pytest.mark.gpu
@@ -222,4 +223,20 @@ def test_scores_that_are_nothing(scale, prompt, monkeypatch):
         c = Case(14, 2, 64, 16, 37, [(40, 90), (1, 70)], BF, seed=4, edit=edit)
         c.q.zero_()
         c.scale = scale
+        c.check(ops().kv4_attention(*c.args()))
+
+
+# ------------------------------------------------------------------ many key/value heads
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("shape", [(64, 64, 128, 16, 128, False, True, 5), (128, 64, 128, 16, 0, False, True, 3),
+                                   (96, 96, 64, 32, 32, True, True, 7)], ids=str)
+def test_write_of_many_key_value_heads(shape, dtype):
+    """Rotations that keep rows in registers have no limit on heads."""
+    test_gpu_kv4.test_write_and_read(shape, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+def test_attention_of_many_key_value_heads(dtype):
+    for step in ([(1, 70), (1, 3)], [(40, 90)]):
+        c = Case(64, 64, 128, 16, None, step, dtype, seed=6)
         c.check(ops().kv4_attention(*c.args()))

@@ -41,3 +41,31 @@ def test_queries_beyond_the_prompt_kernels_counting(monkeypatch):
         ops.kv4_attention(q, torch.empty(5, 2, 16, 80, dtype=torch.uint8, device="meta"), torch.empty_like(q), one, one, one,
                           torch.zeros(1, 4, dtype=torch.int32, device="meta"), 16, 2, 64, 0.1, None, 16, rows, rows)
         assert calls == there
+
+
+FITS = [(64, 128, 128, False, True), (64, 128, 0, False, True), (64, 128, 64, True, True), (47, 128, 64, False, True),
+        (48, 128, 64, False, False), (95, 64, 32, False, True), (96, 64, 32, False, False)]
+
+
+@pytest.mark.parametrize("KV,D,rot,interleaved,fits", FITS)
+def test_many_key_value_heads(KV, D, rot, interleaved, fits):
+    """Only a rotation by halves of a part of the channels has a limit, which a model meets when it is built."""
+    from paged_batch_engine_b200.config.specs import ConfigError, PartSpec
+    from paged_batch_engine_b200.parts.attention import GQAttention
+    qkv = torch.zeros(3, 3 * KV * D, dtype=torch.bfloat16)
+    args = _write_args(qkv=qkv, bias=None, q_out=torch.zeros(3, KV * D, dtype=torch.bfloat16),
+                       pages=torch.zeros(2, KV, 16, D * 5 // 4, dtype=torch.uint8), inv_freq=torch.zeros(rot // 2),
+                       num_heads=KV, num_kv_heads=KV, head_dim=D, rotary_dim=rot)
+    with pytest.raises(ops.KernelError, match="CUDA devices only" if fits else "shared memory"):
+        ops.kv4_write(**args, interleaved=interleaved)
+    position = PartSpec("rope", dict(theta=1e4, head_dim=D, rotary_dim=rot, pairing="interleaved" if interleaved else "half")) \
+        if rot else None
+    mixer = GQAttention(hidden_size=64, num_heads=KV, num_kv_heads=KV, head_dim=D, position=position, dtype=torch.bfloat16,
+                        device="cpu")
+    if fits:
+        mixer.use_cache_bits(4)
+        assert mixer.cache_bits == 4
+    else:
+        with pytest.raises(ConfigError, match="key/value heads"):
+            mixer.use_cache_bits(4)
+        assert mixer.cache_bits is None
