@@ -438,8 +438,8 @@ attn_mma_kernel(AttnParams p, AttnFusedParams f, const __grid_constant__ CUtenso
   __shared__ bf16 s_newkv[FUSED_NEWKV];                // fused mode: the new token's key and value rows
   __shared__ __align__(8) unsigned long long s_full[NST];   // tile buffer i holds its tile
 
-  // The work list, the lengths and the block tables are written by the host before the
-  // step's first kernel: they are read before the dependency on the previous kernel is awaited.
+  // The work list, the lengths and the block tables are complete before the step's first kernel
+  // begins (pdl.cuh): they are read before the dependency on the previous kernel is awaited.
   // rows mode: a one-dimensional grid, work-major, so that the heavy tiles at the head of
   // the work list start first for every key/value head
   const int H = p.num_heads, KV = p.num_kv_heads, G = H / KV, P = p.page_tokens;

@@ -3,7 +3,10 @@
 // pdl_wait(), which returns once the previous kernel has completed and its writes are
 // visible; everything a kernel reads from or writes to activations, the cache or any
 // other buffer of the step comes after that call.  What does not depend on the previous
-// kernel (weights, above all) may be fetched before it.  The order of loads and the wait is the compiler's
+// kernel (weights, above all) may be fetched before it.  So may a step's lists, lengths and block tables and the cache's older
+// entries, which attention reads early (attention_mma.cu; kv4_attention.cu where it is told that they are settled): they are
+// complete before the step's first kernel begins, since a copy from the host, or a launch without the attribute
+// (complete_before_what_follows in engine/batch.py), lies between.  The order of loads and the wait is the compiler's
 // to keep, and it need not keep it for pointers marked __restrict__ (nothing else may write what they
 // name, so neither may the wait), nor for loads through the read-only cache: in a kernel that waits
 // only weights are marked so (tests/test_kernel_sources.py).  pdl_launch_dependents() tells

@@ -258,6 +258,14 @@ def recurrence_plan_arrays(q_start, q_len, slots, chunk: int):
     return first, scan, second, entries
 
 
+def complete_before_what_follows(device) -> None:
+    """What the stream holds so far is complete before any kernel launched from here on begins.  This package's kernels may begin
+    beside the one before them (pdl.cuh), and some read a step's lists, lengths and block tables before they wait: lists that the
+    host sent lie behind a copy, lists that a kernel makes lie behind this, a small fill, which begins when all before it has ended
+    and ends before the next kernel begins."""
+    torch.zeros(1, dtype=torch.int32, device=device)
+
+
 class StepContext:
     """Everything the parts read about the step besides their input rows."""
     captured = False              # True for the fixed-layout context of a captured decode step
@@ -364,6 +372,7 @@ class StepContext:
         if on_device:
             lens, before = pk.view(i_ql), pk.view(i_pos)
             maps = [ops.page_maps(lens, before, pk.view(i), P, T, stride) for i, stride, _ in i_groups]
+            complete_before_what_follows(device)
             self.positions = maps[0].positions
         # what a position encoding is given: the explicit ids ([T] for one axis, [T, axes] for
         # several), or the places in the sequence

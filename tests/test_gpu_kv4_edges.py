@@ -240,3 +240,26 @@ def test_attention_of_many_key_value_heads(dtype):
     for step in ([(1, 70), (1, 3)], [(40, 90)]):
         c = Case(64, 64, 128, 16, None, step, dtype, seed=6)
         c.check(ops().kv4_attention(*c.args()))
+
+
+# ------------------------------------------------------------------ lists that a kernel makes
+def test_maps_made_on_the_device_are_complete_before_the_steps_kernels(monkeypatch):
+    """Attention kernels read block tables before they wait for the kernel before them: behind the launches that make the
+    tables comes one that no kernel begins beside."""
+    from paged_batch_engine_b200.cache import CacheManager, KVGroupSpec
+    from paged_batch_engine_b200.engine import batch
+    seen = []
+    maps, fence = batch.ops.page_maps, batch.complete_before_what_follows
+    monkeypatch.setattr(batch.ops, "page_maps", lambda *a: seen.append("maps") or maps(*a))
+    monkeypatch.setattr(batch, "complete_before_what_follows", lambda device: seen.append("fence") or fence(device))
+    groups = [KVGroupSpec((0,), 2, 64, None), KVGroupSpec((1,), 2, 64, 20)]
+    for limit, want in ((1 << 30, []), (1, ["maps", "maps", "fence"])):
+        monkeypatch.setattr(batch, "MAPS_ROWS", limit)
+        seen.clear()
+        m, entries = CacheManager(groups, 16, [40, 40], max_requests=4), []
+        for rows in (40, 1):
+            h = m.add_request()
+            assert m.reserve(h, rows)
+            entries.append(batch.StepEntry(h, [1] * rows, [0]))
+        batch.StepContext(m, entries, torch.device(DEV), [])
+        assert seen == want
