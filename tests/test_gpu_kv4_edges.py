@@ -263,3 +263,98 @@ def test_maps_made_on_the_device_are_complete_before_the_steps_kernels(monkeypat
             entries.append(batch.StepEntry(h, [1] * rows, [0]))
         batch.StepContext(m, entries, torch.device(DEV), [])
         assert seen == want
+
+
+# ------------------------------------------------------------------ attention beside the write, as a step calls the two
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("window", [None, 37])
+@pytest.mark.parametrize("heads", [(28, 4, 128, 16), (14, 2, 64, 32), (24, 1, 64, 16), (40, 8, 128, 64)], ids=str)
+@pytest.mark.parametrize("step", [[(1, 0), (1, 15), (1, 700)], [(5, 0), (3, 16), (1, 300), (40, 100)], [(2, 3001)], [(130, 40), (1, 64)]],
+                         ids=str)
+def test_attention_beside_the_write_of_portions(step, heads, window, prompt, monkeypatch):
+    """``settled`` with portions: rows of ``step`` (rows, tokens before them) follow a projection and their own write, and have the
+    bits of a call that waits for everything."""
+    if prompt:
+        by_tcgen05(monkeypatch)
+    o, g = ops(), torch.Generator().manual_seed(len(step))
+    H, KV, D, P = heads
+    lens = [b + r for r, b in step]
+    width = max(-(-n // P) for n in lens) + 1
+    table = torch.randperm(len(step) * width, generator=g).to(torch.int32).reshape(len(step), width)
+    pages = torch.full((len(step) * width, KV, P, o.kv4_width(D)), 0xff, dtype=torch.uint8, device=DEV)
+    every = lambda first: [int(table[r, p // P]) * P + p % P for r, (n, b) in enumerate(step) for p in first(n, b)]  # noqa: E731
+    old = test_gpu_kv4.ints(every(lambda n, b: range(b)))
+    if len(old):
+        x = torch.randn(len(old), (H + 2 * KV) * D, generator=g).to(BF).to(DEV)
+        o.kv4_write(x, None, torch.empty(len(old), H * D, dtype=BF, device=DEV), pages, torch.zeros_like(old), old, None, H, KV, D, 0, P)
+    T = sum(r for r, _ in step)
+    slots = test_gpu_kv4.ints(every(lambda n, b: range(b, b + n)))
+    rows, at = test_gpu_kv4.ints([r for r, _ in step]), test_gpu_kv4.ints([0] + [r for r, _ in step][:-1]).cumsum(0, dtype=torch.int32)
+    seq, bt = test_gpu_kv4.ints(lens), table.to(DEV)
+    weight = (torch.randn((H + 2 * KV) * D, 256, generator=g) / 16).to(BF).to(DEV)
+    hidden = torch.randn(4, T, 256, generator=g).to(BF).to(DEV)
+    torch.cuda.synchronize()
+    for x in hidden:
+        q, out, want = (torch.empty(T, H * D, dtype=BF, device=DEV) for _ in range(3))
+        for into, settled in ((out, True), (want, False)):
+            pages.view(-1)[:1].add_(0)                             # the call before it is behind a launch of its own
+            qkv = o.linear(x, weight, None, out_dtype=BF, kind=1)
+            o.kv4_write(qkv, None, q, pages, torch.zeros_like(slots), slots, None, H, KV, D, 0, P)
+            o.kv4_attention(q, pages, into, at, rows, seq, bt, H, KV, D, D ** -0.5, window, P, max(r for r, _ in step), max(lens), settled)
+        assert torch.isfinite(out).all() and torch.equal(out, want)
+
+
+# ------------------------------------------------------------------ keys and values that lean
+@pytest.mark.parametrize("dtype,prompt", FORMS, ids=str)
+@pytest.mark.parametrize("heads", [(14, 2, 64, 16), (28, 4, 128, 16)], ids=str)
+def test_keys_and_values_that_lean_by_many_spans(heads, dtype, prompt, monkeypatch):
+    """Channels that lie far from zero in every token, as a bias on the projection makes them: groups' lo many times their s."""
+    if prompt:
+        by_tcgen05(monkeypatch)
+
+    def edit(k, v):
+        k[:, :, ::7] += 40.0
+        k[:, :, 32:48] += 25.0
+        v[:, :, 5::9] -= 60.0
+    c = Case(*heads, None, [(40, 200), (1, 333), (3, 3)], dtype, seed=8, q_scale=0.25, edit=edit)
+    check_rows(c, ops().kv4_attention(*c.args()))
+
+
+def test_as_many_requests_as_a_call_takes():
+    """Their lists fill the block's shared memory; the last request is as right as the first."""
+    n = ops().KV4_MAX_REQUESTS
+    c = Case(2, 1, 64, 16, None, [(1, 3 + i % 5) if i % 1000 == 0 or i == n - 1 else (0, 0) for i in range(n)], BF, seed=9)
+    c.check(ops().kv4_attention(*c.args()))
+    c = Case(2, 1, 64, 16, None, [(70, 75) if i == n - 1 else (0, 0) for i in range(n)], BF, seed=9)
+    for few in (64, 1):
+        args = c.args()
+        ops().KV4_FEW_PACKED, kept = few, ops().KV4_FEW_PACKED
+        try:
+            c.check(ops().kv4_attention(*args))
+        finally:
+            ops().KV4_FEW_PACKED = kept
+
+
+@pytest.mark.parametrize("dtype,prompt", FORMS, ids=str)
+@pytest.mark.parametrize("place", [0, 33, 64, 90])
+def test_large_values_that_weigh_nothing(place, dtype, prompt, monkeypatch):
+    """A row that sees a value 2^16 times the others', at a score far below theirs: the others' mean, as near as without it (weights
+    keep their eleven bits down to 2^-20 of the largest value that a row sees)."""
+    if prompt:
+        by_tcgen05(monkeypatch)
+
+    def edit(k, v):
+        k.zero_()
+        k[place, :, 0] = -15.0
+        v[place] *= 2.0 ** 16
+    c = Case(4, 2, 64, 16, None, [(9, 110)], dtype, seed=place, edit=edit)
+    c.q.zero_()
+    c.q.view(-1, 4, 64)[:, :, 0] = 60.0                            # a score of -112: a weight of 2^-162
+    out = ops().kv4_attention(*c.args()).cpu().double().reshape(9, 4, 64)
+    v = c.kv[0][1].repeat_interleave(2, 1)
+    for i in range(9):
+        n = 110 - 8 + i
+        seen = [t for t in range(n) if t != place]
+        # weights are equal: rounded once with s (2^-11, to float32 nothing), and the output once
+        tol = (2 ** -8 + 2 ** -11 if dtype == BF else 2 ** -17) * 3 * v[seen].abs().amax()
+        assert ((out[i] - v[seen].mean(0)).abs() <= tol).all()

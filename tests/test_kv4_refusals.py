@@ -69,3 +69,8 @@ def test_many_key_value_heads(KV, D, rot, interleaved, fits):
         with pytest.raises(ConfigError, match="key/value heads"):
             mixer.use_cache_bits(4)
         assert mixer.cache_bits is None
+
+
+def test_more_requests_than_a_call_takes():
+    with pytest.raises(ops.KernelError, match="at most 8192 requests"):
+        ops.kv4_attention(**_attn_args(q_start=_ints(8193), q_len=_ints(8193), seq_len=_ints(8193), block_table=_ints(8193, 4)))
