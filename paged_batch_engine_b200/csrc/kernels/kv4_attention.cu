@@ -11,8 +11,8 @@
 //
 // Both products have the keys' or the channels' codes as A (16 keys, 16 channels) and the rows (packed: query row x head of the
 // group) as B, eight at a time, so eight rows leave no lane idle; the weights pass from the one's result to the other's operand
-// through movmatrix.  Sums are float32; weights times s are rounded to float16 once (2^-12; a running exponent over the
-// values' s keeps them in its range).  A warp takes tiles of 16 keys, one record each, through a ring of its own in shared
+// through movmatrix.  Sums are float32; weights times s are rounded to float16 once (2^-11; a running exponent of each row, over
+// the s of the values that it sees, keeps them in its range: 2^-20 of the largest keeps all bits, 2^-31 none).  A warp takes tiles of 16 keys, one record each, through a ring of its own in shared
 // memory (cp.async, four deep), and keeps a running maximum that moves only when it grew by 2^8.
 //
 // Work is cut by bytes, not by requests: the tiles of all (request, head, row tile) laid end to end are shared out evenly over
@@ -65,7 +65,7 @@ struct Split {
 
 constexpr int WARPS = 4;
 constexpr int STAGES = 4;
-constexpr int MIN_UNITS = 8;   // tiles a block takes at least: two a warp
+constexpr int MIN_UNITS = 8;   // tiles a block takes at least, two a warp: KV4_UNITS of ops.py, which sizes the grid by it
 constexpr int MOST_REQUESTS = 8192;
 constexpr float UP = 18446744073709551616.f;           // 2^64
 constexpr float CODE = 590295810358705651712.f;        // 2^69 = 2^133 / 2^64: products of bfloat16 codes
@@ -239,7 +239,7 @@ kv4_attention_kernel(Kv4AttnParams p, Split sp) {
     const int pos_min = q.pos0 + row_of(pr0), pos_max = q.pos0 + row_of(min(pr0 + MT, packed) - 1);
     const int low_min = p.window > 0 ? max(0, pos_min) - p.window + 1 : 0, low_max = p.window > 0 ? max(0, pos_max) - p.window + 1 : 0;
 
-    // ---- this warp's tiles, t_begin + warp, + 8, ...: the first are on their way before the queries are looked at
+    // ---- this warp's tiles, t_begin + warp, + WARPS, ...: the first are on their way before the queries are looked at
     const int mine = t_end - t_begin > warp ? (t_end - t_begin - warp + WARPS - 1) / WARPS : 0;
     const int32_t* table = p.block_table + (long long)req * p.bt_stride;
     auto record = [&](int i) {                         // the record of this warp's tile i, -1: none to be seen

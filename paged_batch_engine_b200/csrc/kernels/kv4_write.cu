@@ -9,7 +9,7 @@
 // beyond 2^120 as 2^120: four bits hold no mark for them, and a cache that held them would hand them to every later row.
 //
 // The angle position * frequency is formed in 64 bits and brought within a turn before its sine and cosine are taken in 32:
-// the float32 product alone is off by 0.004 at position 65,536.
+// the float32 product alone is off by up to 0.002 below position 65,536.  (rope_kv.cu takes it as it is.)
 #include "common.cuh"
 #include "kv4.cuh"
 #include "pdl.cuh"

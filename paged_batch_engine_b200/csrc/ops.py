@@ -2835,7 +2835,8 @@ def kv4_write(qkv: torch.Tensor, bias: Optional[torch.Tensor], q_out: torch.Tens
     is one layer's, uint8 [page, kv_head, page_tokens, kv4_width(head_dim)] (None: nothing is written); a row whose slot is
     negative or behind the last page writes nothing.  Two rows of one call must not share a slot.  Groups of 32 channels are kept
     as lo + s * code, code 0..15, each off by at most s / 2 (s: a fifteenth of the group's span, rounded up to bfloat16); NaN is
-    kept as 0, what lies beyond 2^120 as 2^120."""
+    kept as 0, what lies beyond 2^120 as 2^120 (``kv4_attention`` has narrower ranges).  The angles position * inv_freq are formed in
+    64 bits, where ``rope_kv_write`` has 32: below position 2,048 its angles are off by up to 0.00006, below 65,536 by 0.002."""
     T, H, KV = qkv.shape[0], num_heads, num_kv_heads
     width = (H + 2 * KV) * head_dim
     kv4_width(head_dim)
@@ -2964,7 +2965,14 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, q_sta
     q_len and seq_len as far as the host knows them: they choose the shape of the launch, not the result (beyond the order
     of its sums).  ``settled``: the lengths, the block table and the keys before each request's rows were complete before the
     launch that precedes this call on the stream began (the step's own ``kv4_write``, in a step whose arrays the host sent), so
-    the kernel may begin beside it and wait for the rest.  At most ``KV4_MAX_REQUESTS`` requests."""
+    the kernel may begin beside it and wait for the rest.  At most ``KV4_MAX_REQUESTS`` requests; every row of a request lies
+    within q.
+
+    Ranges: queries below 2^60; spans of keys and values (a group's 15 s) from 2^-60 to 2^60, and values below 2^36 where every span
+    that the row has seen is less; scores that float32 holds.  With bfloat16 queries a weight is rounded to float16 once (2^-11 of
+    it), against the largest span of a value that the row sees: the weight of a value whose span is 2^-20 of that keeps its eleven
+    bits, below it loses them, and from 2^-31 on the value counts for nothing.  Keys and values that a row does not see never
+    enter.  A row with a query that is NaN or infinite is NaN; others stay as they are."""
     H, KV, R = num_heads, num_kv_heads, q_len.numel()
     if H < 1 or KV < 1 or H % KV:
         raise KernelError("kv4_attention: num_heads must be a multiple of num_kv_heads")

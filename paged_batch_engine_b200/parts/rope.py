@@ -12,7 +12,9 @@ class RotaryEncoding(PositionEncoding):
     rope_kernel.cu:163-176) or (2i, 2i+1) ("interleaved").  Dimensions at or above
     ``rotary_dim`` pass through.  The inverse frequencies are computed in float32 the way
     the reference builds its table (``1/powf(theta, d/head_size)``, rope_kernel.cu:69-94);
-    the angle, sine and cosine are float32 in the kernel."""
+    the angle, sine and cosine are float32 in the kernel.  Where keys are kept in four bits the
+    angle is formed in 64 bits and brought within a turn first (``ops.kv4_write``), so queries and
+    keys of far positions differ from those of a 16-bit cache by the angle's rounding."""
 
     def __init__(self, theta: float, head_dim: int, dtype, device, rotary_dim: int = None,
                  pairing: str = "half"):
