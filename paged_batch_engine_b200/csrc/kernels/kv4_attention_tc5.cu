@@ -56,6 +56,7 @@ constexpr int S_COL = 0, O_COL = 256;   // of half h: two score buffers at 128 h
 constexpr int ROOM = 6;                 // weights are kept 2^6 times too large: float16 reaches further down
 constexpr int MOST_E = 60;
 constexpr float FAR = 16384.f;          // beyond this maximum weights are made one by one: its rounding in float32 is 2^-11
+constexpr int NOTHING = -(1 << 20);     // the exponent of a token whose numbers are all zero
 constexpr int EVEN = 8, UNEVEN = 1024;  // exponents that the tokens of a record may lie apart and share a unit; the mark of others
 
 struct Tc5Split {
@@ -196,58 +197,86 @@ __device__ __forceinline__ Tile tile_of(const Kv4AttnParams& p, int most_packed,
   return {-1, 0, target, 0, 0, 0};
 }
 
+__device__ __forceinline__ void tmem_st8_nowait(uint32_t taddr, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
 // what a tile's operands count in
 struct alignas(16) Units {
   float key[RECS];             // 2^exponent of a record's keys, negative: no key of it is seen
-  int value[RECS];             // exponent of its values, and UNEVEN more where its tokens have exponents of their own:
-  int key_exp[BN], value_exp[BN];
+  int value[RECS];             // exponent of its values, and UNEVEN more where its tokens have units of their own:
+  float key_of[BN], value_of[BN];
 };
 
 // A row's weights of one tile, one by one: for tiles with uneven records, and for rows whose scores are so far from zero that the
 // exponents cannot be added to the maximum.  The same steps as in the kernel's loop below, out of its way and its registers.
+// clear: the row sees every place of the tile that holds a key.
 struct Weighed {
   float m, shrink, alpha, sum;
   int e;
 };
-__device__ __noinline__ Weighed weigh_one_by_one(const Units* u, uint32_t s_addr, int ts, int lo, int pos, float row_unit, float m_run, int e_run) {
-  float mx = -INFINITY, s[REC_TOKENS];
-  int e_new = e_run;
-  auto scores = [&](int g) {
-    tmem_ld16(s_addr + g * REC_TOKENS, s);
-    const float key = u->key[g];
-    const bool own = u->value[g] >= UNEVEN / 2;
-#pragma unroll
-    for (int i = 0; i < REC_TOKENS; ++i) {
-      const int at = ts + g * REC_TOKENS + i;
-      s[i] = at <= pos && at >= lo && key > 0.f ? s[i] * ((own ? pow2(u->key_exp[g * REC_TOKENS + i]) : key) * row_unit) : -INFINITY;
-    }
+__device__ __noinline__ Weighed weigh_one_by_one(const Units* u, uint32_t s_addr, int ts, int lo, int pos, bool clear, float row_unit, float m_run, int e_run) {
+  float s[REC_TOKENS], mx = -INFINITY, most = 0.f;     // most: 2^exponent of the largest values that the row sees
+  // units of four tokens, from memory that may hold anything where the record has one (no branch: the loads go ahead together)
+  auto four = [](bool own, const float* from, float one, float (&to)[4]) {
+    const float4 x = *reinterpret_cast<const float4*>(from);
+    to[0] = own ? x.x : one, to[1] = own ? x.y : one, to[2] = own ? x.z : one, to[3] = own ? x.w : one;
   };
-  auto exponent = [&](int g, int i) { return u->value[g] >= UNEVEN / 2 ? u->value_exp[g * REC_TOKENS + i] : u->value[g]; };
+  auto scores = [&](int g) {
+    const bool own = u->value[g] >= UNEVEN / 2;
+    const float key = u->key[g];
+    const int at = ts + g * REC_TOKENS;
+    tmem_ld16(s_addr + g * REC_TOKENS, s);
+#pragma unroll
+    for (int c = 0; c < REC_TOKENS; c += 4) {
+      float kf[4];
+      four(own, u->key_of + g * REC_TOKENS + c, key, kf);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool see = (clear || (at + c + i <= pos && at + c + i >= lo)) && key > 0.f;
+        s[c + i] = see ? s[c + i] * (kf[i] * row_unit) : -INFINITY;
+      }
+    }
+    return own;
+  };
 #pragma unroll 1
   for (int g = 0; g < RECS; ++g) {
-    scores(g);
+    const bool own = scores(g);
+    const float value = pow2(u->value[g]);
 #pragma unroll
-    for (int i = 0; i < REC_TOKENS; ++i) {
-      mx = fmaxf(mx, s[i]);
-      if (s[i] != -INFINITY) e_new = max(e_new, exponent(g, i));
+    for (int c = 0; c < REC_TOKENS; c += 4) {
+      float vf[4];
+      four(own, u->value_of + g * REC_TOKENS + c, value, vf);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        mx = fmaxf(mx, s[c + i]);
+        most = fmaxf(most, s[c + i] != -INFINITY ? vf[i] : 0.f);
+      }
     }
   }
+  const int e_new = max(e_run, (__float_as_int(most) >> 23) - 127);
   float m_new = fmaxf(m_run, mx);
   if (m_run != -INFINITY && m_new - m_run <= 8.0f) m_new = m_run;
-  const float m_use = m_new == -INFINITY ? 0.f : m_new;
-  uint32_t w[BN / 2];
+  const float m_use = m_new == -INFINITY ? 0.f : m_new, down = pow2(-e_new);
   float sum = 0.f;
+#pragma unroll 1
+  for (int g = 0; g < RECS; ++g) {                     // a record's weights take the place of scores that have been read
+    const bool own = scores(g);
+    const float value = pow2(u->value[g]);
+    uint32_t w[REC_TOKENS / 2];
 #pragma unroll
-  for (int g = 0; g < RECS; ++g) {
-    scores(g);
+    for (int c = 0; c < REC_TOKENS; c += 4) {
+      float vf[4];
+      four(own, u->value_of + g * REC_TOKENS + c, value, vf);
 #pragma unroll
-    for (int i = 0; i < REC_TOKENS; i += 2) {
-      const float x = ex2(s[i] - m_use + ROOM), y = ex2(s[i + 1] - m_use + ROOM);
-      sum += x + y;
-      w[(g * REC_TOKENS + i) / 2] = h2(x * pow2(exponent(g, i) - e_new), y * pow2(exponent(g, i + 1) - e_new));
+      for (int i = 0; i < 4; i += 2) {
+        const float x = ex2(s[c + i] - m_use + ROOM), y = ex2(s[c + i + 1] - m_use + ROOM);
+        sum += x + y;
+        w[(c + i) / 2] = h2(x * down * vf[i], y * down * vf[i + 1]);
+      }
     }
+    tmem_st8_nowait(s_addr + g * (REC_TOKENS / 2), w);
   }
-  tmem_st32_nowait(s_addr, &w[0]);
   const float shrink = ex2(m_run - m_use);
   return {m_new, shrink, shrink * ex2((float)(e_run - e_new)), sum, e_new};
 }
@@ -425,14 +454,21 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
       // is all there is: the tokens of such a record have units of their own.  (Within EVEN the shared unit leaves 2^-12 of s * 15.)
       const bool far = (kind & 1) && ((keep & 0xffffu && (int)(most[0] >> 7) - 127 + 9 < e - EVEN) ||
                                       (keep >> 16 && (int)(most[1] >> 7) - 127 + 9 < e - EVEN));
-      const bool own_units = __any_sync(0xffffffffu, far);
+      bool own_units = __any_sync(0xffffffffu, far);
       int e_tok[2] = {e, e};
       if (own_units) {
+        // looked at once more with the token's lo: one whose numbers are all zero has nothing to lose
+        int e_i[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int e_i = (int)(most[i] >> 7) - 127 + (kind & 1 ? 9 : -14);
-          e_tok[i] = max(-MOST_E, min(MOST_E + 9, max(e_i, __shfl_xor_sync(0xffffffffu, e_i, 8))));
+          e_i[i] = most[i] ? (int)(most[i] >> 7) - 127 + (kind & 1 ? 9 : -14) : NOTHING;
+          e_i[i] = max(e_i[i], __shfl_xor_sync(0xffffffffu, e_i[i], 8));
         }
+        own_units = __any_sync(0xffffffffu, (e_i[0] != NOTHING && max(-MOST_E, e_i[0]) < e - EVEN) ||
+                                                (e_i[1] != NOTHING && max(-MOST_E, e_i[1]) < e - EVEN));
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (own_units) e_tok[i] = max(-MOST_E, min(MOST_E + 9, e_i[i]));
       }
       const float by[2] = {pow2((kind & 1 ? 24 : 0) - e_tok[0]), pow2((kind & 1 ? 24 : 0) - e_tok[1])};
       unsigned half[G];
@@ -455,11 +491,9 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
       ok = ok && mbar_wait(&empty[st], (round & 1) ^ 1, err);
       if (lane == 0) units[st].key[rec] = seen ? pow2(e) : -1.f;
       if (lane == 16) units[st].value[rec] = own_units ? e + UNEVEN : e;
-      if (own_units && !(kind & 1)) {
-        int* exps = (kind == K_LO ? units[st].key_exp : units[st].value_exp) + rec * REC_TOKENS + 2 * np;
-        exps[0] = e_tok[0];
-        exps[1] = e_tok[1];
-      }
+      if (own_units && !(kind & 1))
+        *reinterpret_cast<float2*>((kind == K_LO ? units[st].key_of : units[st].value_of) + rec * REC_TOKENS + 2 * np) =
+            make_float2(pow2(e_tok[0]), pow2(e_tok[1]));
       __syncwarp();                                    // the numbers are there: each is read by other lanes than its own
       // ---- keys
       // (a record that is not seen, or a place without a key, has numbers that are zero, whatever its codes)
@@ -697,7 +731,8 @@ kv4_attention_tc5_kernel(Kv4AttnParams p, Tc5Split sp, int* err) {
         if (!one_by_one) tmem_st32_nowait(s_addr + st * BN, &w[0]);
       }
       if (one_by_one) {
-        const Weighed x = weigh_one_by_one(&u, s_addr + st * BN, ts, lo, pos, row_unit, m_run, e_run);
+        const Weighed x = weigh_one_by_one(&u, s_addr + st * BN, ts, lo, pos, ts + BN - 1 <= pos_min && ts >= low_max, row_unit,
+                                           m_run, e_run);
         m_new = x.m, e_new = x.e, alpha = x.alpha;
         l_run = fmaf(l_was, x.shrink, x.sum);
         far = is_far(m_new);

@@ -358,3 +358,21 @@ def test_large_values_that_weigh_nothing(place, dtype, prompt, monkeypatch):
         # weights are equal: rounded once with s (2^-11, to float32 nothing), and the output once
         tol = (2 ** -8 + 2 ** -11 if dtype == BF else 2 ** -17) * 3 * v[seen].abs().amax()
         assert ((out[i] - v[seen].mean(0)).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("window", [None, 100])
+@pytest.mark.parametrize("heads", [(28, 4, 128, 16), (14, 2, 64, 32)], ids=str)
+def test_records_of_tokens_far_apart(heads, window, splits, monkeypatch):
+    """Tokens 2^-12 and 2^-14 of the others' size, constant ones and zero ones, all over a prompt."""
+    by_tcgen05(monkeypatch, splits)
+
+    def edit(k, v):
+        v[::7] *= 2.0 ** -12
+        k[::5] *= 2.0 ** -14
+        v[3::50], k[4::50], v[9::90] = 0.0, 0.0, 0.75
+        k[100:140], v[100:140] = 0.0, 0.0
+    c = Case(*heads, window, [(300, 700), (45, 45)], BF, seed=11, edit=edit)
+    out = ops().kv4_attention(*c.args(spare=2))
+    c.check(out)
+    assert (out[c.T:] == 7.0).all()
