@@ -21,11 +21,11 @@
 // (CLUSTER) go to a cluster of blocks each instead, which share its tiles and merge through distributed shared memory: one
 // launch less, and no parts in memory.
 //
-// 28 heads on 4 of 128, bfloat16: 64 requests of 300 to 8,192 keys (175 MB) 57 us, 3.1 TB/s; a tile more costs what 4.9 TB/s
+// 28 heads on 4 of 128, bfloat16: 64 requests of 300 to 8,192 keys (175 MB) 58 us, 3.0 TB/s; a tile more costs what 4.9 TB/s
 // would, the rest, some 18 us, is the lists, the beginning and end of each block's pieces of items (2.5 us each) and the second
-// kernel.  A tile takes 409 instructions a warp, 185 of them on the ALU pipe (80 to take codes out; eight fewer changed
+// kernel.  A tile takes 406 instructions a warp, some 185 of them on the ALU pipe (80 to take codes out; eight fewer changed
 // nothing), and four blocks a multiprocessor issue 0.57 a scheduler and clock over the whole call: bound by instructions and
-// their latencies, not by bytes.  One request of 131,071 keys (40 heads on 8, 168 MB) 52 us; in clusters, 8 of 2,048 keys 11 us,
+// their latencies, not by bytes.  One request of 131,071 keys (40 heads on 8, 168 MB) 53 us; in clusters, 8 of 2,048 keys 11 us,
 // one of 777 7 us: chains of latency.
 //
 // Float32: queries and weights as three bfloat16 terms each.  There the two sums' cancellation would show (a head's output is

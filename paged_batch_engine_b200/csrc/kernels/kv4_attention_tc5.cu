@@ -14,9 +14,12 @@
 // rows of the values are ordered (group, i, r), so that eight lanes write eight different banks, and the epilogue puts the
 // channels back in order.  Warps 14 and 15 issue the products, each those of its half.
 //
-// 4,096 tokens of 28 heads on 4 of 128: 181 us, 664 TFLOP/s (0.40 of the library products' rate; floor 72).  A tile of 256 x 64
-// takes 2,750 clocks, of which its products need 1,024 and its 16,384 exponentials 1,024 of the SM's sixteen a clock; the rest
-// is the softmax's other instructions on the same four schedulers.  With one half a block and two blocks a multiprocessor each
+// 4,096 tokens of 28 heads on 4 of 128: 187 us, 643 TFLOP/s (0.39 of the library products' rate; floor 72).  A tile of 256 x 64
+// takes some 2,840 clocks, of which its products need 1,024 and its 16,384 exponentials 1,024 of the SM's sixteen a clock: no
+// pipe is busy for two fifths of the time.  What is long is each softmax thread's chain (wait, load, multiply-add, exponential,
+// rounding, store, fence), with two warps a scheduler to hide it; attention_tc5.cu, two blocks a multiprocessor, takes 1,750 for
+// the same exponentials.  512 threads leave 128 registers each, and some spill (head size 128: 92 bytes stored and 244 loaded, 64: 64
+// and 188).  With one half a block and two blocks a multiprocessor each
 // record was converted twice as often, and four converting warps were what the rest waited for: 269 us; with key tiles of 128
 // and one score buffer a half: 286.
 //
