@@ -28,8 +28,9 @@ SPLIT_KEYS = 256          # keys per split of a short request's long key range, 
 SPLIT_KEYS_FEW = 512      # the same in steps of at most FEW_REQUESTS requests
 FEW_REQUESTS = 4          # (a bucket edge of the captured decode steps)
 MAX_SPLIT_TILES = 4       # requests with more row tiles than this are never split
-MAPS_ROWS = 4096          # steps of at least this many rows have their row maps and block tables made on the device (one request:
-#                           421 us of host time -> 402, of 2,048 rows 329 -> 336)
+MAPS_ROWS = 8192          # steps of at least this many rows have their row maps and block tables made on the device (us of host time
+#                           with the lists made by the host and by the device: one request of 8,192 rows 633 and 563, of 4,096 438
+#                           and 436, of 2,048 348 and 371; eight portions and six tokens, 4,102 rows, 615 and 625)
 
 
 def choose_split_keys(num_requests: int) -> int:
