@@ -9,7 +9,7 @@
 // Every block makes both running sums over the requests for itself (a few hundred additions beside a launch) and then takes
 // its share of the rows and table entries; a row finds its request by bisection.  Bound by latency: the integers of 64
 // requests of 8,192 tokens are 170 KB and take 4.2 us, those of 15,292 rows of 64 requests (1.7 MB) 5.3.  Sums are 64 bits wide;
-// what does not fit an output (a page list that ends early, a slot beyond 2^31) is written as -1.
+// what does not fit an output (a page list that ends early; a slot, position, length or start beyond 2^31 - 1) is written as -1.
 #include "common.cuh"
 #include "opt_in.cuh"
 #include "pdl.cuh"
@@ -55,6 +55,7 @@ __device__ __forceinline__ long long block_scan(long long v, long long* warp_sum
   return before + v;
 }
 
+__device__ __forceinline__ int fitting(long long x) { return x > 0x7fffffffLL ? -1 : (int)x; }
 __device__ __forceinline__ int page_at(const MapsParams& p, long long i) {
   if (p.pages == nullptr) return i < p.num_pages ? (int)i : -1;
   return i < p.num_pages ? p.pages[i] : -1;
@@ -81,8 +82,8 @@ __global__ void __launch_bounds__(THREADS) page_maps_kernel(MapsParams p) {
       row_end[r] = end;
       first[r] = last - need;
       if (blockIdx.x == 0) {
-        p.q_start[r] = (int)(end - q);
-        p.seq_len[r] = (int)seq;
+        p.q_start[r] = fitting(end - q);
+        p.seq_len[r] = fitting(seq);
       }
     }
   }
@@ -102,11 +103,10 @@ __global__ void __launch_bounds__(THREADS) page_maps_kernel(MapsParams p) {
         const long long entry = pos / p.stride;
         const int page = page_at(p, first[lo] + entry / p.page_tokens);
         if (page >= 0) slot = (long long)page * p.page_tokens + entry % p.page_tokens;
-        if (slot > 0x7fffffffLL) slot = -1;
       }
-      p.positions[item] = (int)pos;
+      p.positions[item] = fitting(pos);
       p.request_of_row[item] = lo < p.requests ? lo : -1;
-      p.slots[item] = (int)slot;
+      p.slots[item] = fitting(slot);
     } else {
       const long long at = item - p.rows;
       const int r = (int)(at / p.width), i = (int)(at - (long long)r * p.width);

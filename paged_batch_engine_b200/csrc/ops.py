@@ -2775,7 +2775,8 @@ def page_maps(q_len: torch.Tensor, context: torch.Tensor, pages: Optional[torch.
     end to end: ``q_start`` is a request's first row and ``seq_len`` its tokens with them; a row has its request, its position
     and the slot (page * page_tokens + place) of its entry, one entry for every ``stride`` tokens.  ``block_table`` has
     ``width`` entries a request, -1 behind its last page.  Of ``rows`` rows those behind the last request have request and
-    slot -1 and position 0.  A row whose page is negative or lies behind the end of ``pages`` has slot -1.  At most
+    slot -1 and position 0.  A row whose page is negative or lies behind the end of ``pages`` has slot -1; a slot, position,
+    length or start beyond 2^31 - 1 is -1.  At most
     ``MAPS_MAX_REQUESTS`` requests; the arrays are views of one buffer."""
     R = q_len.numel()
     if q_len.dtype != torch.int32 or context.dtype != torch.int32 or q_len.dim() != 1 or context.shape != q_len.shape:

@@ -37,3 +37,16 @@ def test_logits_do_not_depend_on_who_makes_the_maps(name, dtype, bits, monkeypat
         made.append(rows)
     for a, b in zip(*made):
         assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
+def test_what_int32_does_not_hold_is_minus_one():
+    """Positions and lengths beyond 2^31 - 1, and starts behind so many rows."""
+    from paged_batch_engine_b200.csrc import ops
+    top = 2 ** 31 - 1
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda:0")  # noqa: E731
+    m = ops.page_maps(ints([5, 2]), ints([top - 2, top - 2]), None, 16, 8, 0)
+    assert m.positions.tolist() == [top - 2, top - 1, top, -1, -1, top - 2, top - 1, 0]
+    assert m.request_of_row.tolist() == [0] * 5 + [1] * 2 + [-1]
+    assert m.seq_len.tolist() == [-1, top] and m.q_start.tolist() == [0, 5]
+    m = ops.page_maps(ints([top, top, 1]), ints([0, 0, 0]), None, 16, 1, 0)
+    assert m.q_start.tolist() == [0, top, -1] and m.positions.tolist() == [0]
